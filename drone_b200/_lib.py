@@ -15,6 +15,11 @@ PLAN_A = 1
 PLAN_AT = 2
 PLAN_BOTH = 3
 LOSS_SCRATCH = 2368      # doubles
+F32, BF16, F16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+NORM_MAX_WIDTH = 65536
+DISTILLATION_MAX_TOP = 256
+DISTILLATION_SCRATCH = 4736      # doubles
 
 
 class DroneError(RuntimeError):
@@ -99,6 +104,15 @@ def _declare(lib):
         "drone_relu_mask": (i, [i, i, vp, i, vp, i, vp]),
         "drone_weight_gradient_scratch": (i, [i, i, i, C.POINTER(ll)]),
         "drone_weight_gradient": (i, [i, i, i, vp, i, vp, i, vp, vp, ll, vp]),
+        "drone_linear": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, i, vp, i, vp, i, vp]),
+        "drone_activation_gradient_scratch": (i, [i, i, C.POINTER(ll)]),
+        "drone_activation_gradient": (i, [i, i, i, vp, i, vp, i, i, vp, i, vp, vp, ll, vp]),
+        "drone_linear_weight_gradient_scratch": (i, [i, i, i, i, i, C.POINTER(ll)]),
+        "drone_linear_weight_gradient": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, ll, vp]),
+        "drone_layer_norm": (i, [i, i, i, vp, i, vp, vp, f, i, vp, i, vp, vp, vp]),
+        "drone_layer_norm_backward_scratch": (i, [i, i, i, C.POINTER(ll)]),
+        "drone_layer_norm_backward": (i, [i, i, i, vp, i, vp, i, vp, vp, vp, vp, i, vp, vp, i, vp, vp, vp, ll, vp]),
+        "drone_distillation_loss": (i, [i, i, i, vp, i, i, i, vp, i, vp, i, f, vp, vp, f, f, vp, i, vp, vp, vp]),
         "drone_xplan_create": (i, [C.POINTER(vp), i, i, i, vp, vp, vp, vp, i]),
         "drone_xplan_destroy": (i, [vp]),
         "drone_xplan_enable_p2p": (i, [vp, vp, vp]),

@@ -1,0 +1,71 @@
+// What the dense operators share: element types, activations, reads of several values at once.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace drone {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// 16 bytes of values
+template <typename T>
+struct alignas(16) Vec {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+
+// z -> activation(z) and its derivative.  A NaN stays one, also in the ReLU (max(NaN, 0) would be 0).
+__device__ __forceinline__ float activate(float z, int activation) {
+    switch (activation) {
+        case DRONE_ACT_RELU: return z < 0.f ? 0.f : z;
+        case DRONE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
+        case DRONE_ACT_SILU: return z / (1.f + expf(-z));
+        default: return z;
+    }
+}
+__device__ __forceinline__ float activation_slope(float z, int activation) {
+    switch (activation) {
+        case DRONE_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+        case DRONE_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+        case DRONE_ACT_SILU: {
+            const float p = 1.f / (1.f + expf(-z));
+            return p * (1.f + z * (1.f - p));
+        }
+        default: return 1.f;
+    }
+}
+
+// Whether every row of such a matrix can be read 16 bytes at a time.
+inline bool rows_on_16_bytes(const void *p, long long ld, int size) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * size % 16 == 0;
+}
+
+inline int type_size(int type) { return type == DRONE_F32 ? 4 : 2; }
+
+inline int device_sms(int *sms) {
+    int dev = 0;
+    DRONE_CUDA(cudaGetDevice(&dev));
+    DRONE_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    return DRONE_OK;
+}
+
+// f(tag) with the element type that `type` stands for as decltype(tag)::T
+template <typename E> struct TypeTag { using T = E; };
+template <typename F>
+int with_type(int type, const F &f) {
+    return type == DRONE_F32 ? f(TypeTag<float>()) : type == DRONE_BF16 ? f(TypeTag<__nv_bfloat16>()) : f(TypeTag<__half>());
+}
+
+}  // namespace drone
+
+#define DRONE_TYPE_OK(type) ((type) == DRONE_F32 || (type) == DRONE_BF16 || (type) == DRONE_F16)
+#define DRONE_ALIGNED(p, type) ((reinterpret_cast<uintptr_t>(p) & (drone::type_size(type) - 1)) == 0)

@@ -1,0 +1,395 @@
+// Layer norm of the rows of a matrix and its backward pass: with mean m and r = 1 / sqrt(variance + eps) of a row,
+//     y  = (x - m) r scale + shift                              (and a ReLU of it)
+//     dx = r (h - mean(h) - xhat mean(h xhat)),   h = g scale,  xhat = (x - m) r,  g = dy (0 where the ReLU's output is not positive)
+//     d_scale = sum over rows of g xhat,  d_shift = sum over rows of g.
+//
+// Bound: HBM, one read of every operand and one write of y or dx.  A group of L lanes holds a row in registers (16 bytes a load
+// where rows allow it), so that mean, variance and the two means of the backward pass cost shuffles and no second read; the
+// variance is that of the differences from the mean, in 32 bits.  The sums over rows stay in a thread's registers for all rows it
+// takes, are added within the block in shared memory and over the blocks in double, always in the same order.
+#include "dense_types.cuh"
+
+#include <algorithm>
+
+namespace drone {
+
+// How a row lies in the registers of its lanes: U vectors of V values a lane, or (rows that are not on 16 bytes) U * V single
+// values a lane, L apart.
+template <typename T, int L, int U, bool VEC>
+struct RowShape {
+    static constexpr int V = Vec<T>::N, PER = U * V, THREADS = L > 256 ? L : 256, GROUPS = THREADS / L;
+    __device__ static int column(int gl, int i) { return VEC ? (gl + i / V * L) * V + i % V : gl + i * L; }
+    // values beyond the row are 0
+    __device__ static void load(const T *row, int F, int gl, float (&v)[PER]) {
+        if (VEC) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                Vec<T> x = {};
+                if (column(gl, u * V) < F) x = *reinterpret_cast<const Vec<T> *>(row + column(gl, u * V));
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[u * V + e] = to_float(x.v[e]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = column(gl, i) < F ? to_float(row[column(gl, i)]) : 0.f;
+        }
+    }
+    __device__ static void store(T *row, int F, int gl, const float (&v)[PER]) {
+        if (VEC) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                Vec<T> x;
+#pragma unroll
+                for (int e = 0; e < V; ++e) x.v[e] = from_float<T>(v[u * V + e]);
+                if (column(gl, u * V) < F) *reinterpret_cast<Vec<T> *>(row + column(gl, u * V)) = x;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (column(gl, i) < F) row[column(gl, i)] = from_float<T>(v[i]);
+        }
+    }
+    __device__ static void load_vector(const float *p, int F, int gl, float (&v)[PER]) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = column(gl, i) < F ? __ldg(p + column(gl, i)) : 0.f;
+    }
+};
+
+// Sum of one value per lane over the L lanes of a row (L <= 32: within the warp; above: the block is the row).
+template <int L>
+__device__ __forceinline__ float2 sum_over_row(float2 v) {
+#pragma unroll
+    for (int o = (L < 32 ? L : 32) / 2; o > 0; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if (L > 32) {
+        __shared__ float2 of_warp[2][L / 32 + 1];
+        __syncthreads();      // the sums of the call before have been read
+        if ((threadIdx.x & 31) == 0) of_warp[0][threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = of_warp[0][0];
+        for (int w = 1; w < L / 32; ++w) {
+            v.x += of_warp[0][w].x;
+            v.y += of_warp[0][w].y;
+        }
+    }
+    return v;
+}
+
+template <typename T, int L, int U, bool VEC>
+__global__ void __launch_bounds__(L > 256 ? L : 256)
+layer_norm_kernel(const T *x, long long ldx, const float *__restrict__ scale, const float *__restrict__ shift, int n, int F, float eps, bool relu,
+                  T *y, long long ldy, float *__restrict__ mean, float *__restrict__ rstd) {
+    using S = RowShape<T, L, U, VEC>;
+    const int gl = threadIdx.x % L;
+    float a[S::PER], b[S::PER];
+    S::load_vector(scale, F, gl, a);
+    S::load_vector(shift, F, gl, b);
+    // whole warps stay for the shuffles: a group without a row repeats the last one and writes nothing
+    const long long first = (long long)blockIdx.x * S::GROUPS, group = threadIdx.x / L, step = (long long)gridDim.x * S::GROUPS;
+    for (long long row0 = first; row0 < n; row0 += step) {
+        const bool live = row0 + group < n;
+        const long long row = live ? row0 + group : n - 1;
+        float v[S::PER];
+        S::load(x + row * ldx, F, gl, v);
+        float2 s = make_float2(0, 0);
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i) s.x += v[i];
+        const float m = sum_over_row<L>(s).x / F;
+        s.x = 0;
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i) {
+            v[i] -= m;
+            if (S::column(gl, i) < F) s.x += v[i] * v[i];
+        }
+        const float r = 1.f / sqrtf(sum_over_row<L>(s).x / F + eps);
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i) {
+            v[i] = v[i] * r * a[i] + b[i];
+            if (relu && v[i] < 0.f) v[i] = 0.f;
+        }
+        S::store(y + row * ldy, F, gl, v);
+        if (gl == 0) {
+            if (mean) mean[row] = m;
+            if (rstd) rstd[row] = r;
+        }
+    }
+}
+
+// Rows too wide for the registers of a block: a block a row, read once more for each step (out of L2).
+constexpr int kWideThreads = 512;
+template <typename T>
+__global__ void __launch_bounds__(kWideThreads)
+layer_norm_wide_kernel(const T *x, long long ldx, const float *__restrict__ scale, const float *__restrict__ shift, int n, int F, float eps, bool relu,
+                       T *y, long long ldy, float *__restrict__ mean, float *__restrict__ rstd) {
+    for (long long row = blockIdx.x; row < n; row += gridDim.x) {
+        const T *in = x + row * ldx;
+        T *out = y + row * ldy;
+        float2 s = make_float2(0, 0);
+        for (int c = threadIdx.x; c < F; c += kWideThreads) s.x += to_float(in[c]);
+        const float m = sum_over_row<kWideThreads>(s).x / F;
+        s.x = 0;
+        for (int c = threadIdx.x; c < F; c += kWideThreads) {
+            const float d = to_float(in[c]) - m;
+            s.x += d * d;
+        }
+        const float r = 1.f / sqrtf(sum_over_row<kWideThreads>(s).x / F + eps);
+        for (int c = threadIdx.x; c < F; c += kWideThreads) {
+            const float z = (to_float(in[c]) - m) * r * __ldg(scale + c) + __ldg(shift + c);
+            out[c] = from_float<T>(relu && z < 0.f ? 0.f : z);
+        }
+        if (threadIdx.x == 0) {
+            if (mean) mean[row] = m;
+            if (rstd) rstd[row] = r;
+        }
+    }
+}
+
+// What both forms of the backward pass read and write; sums[block] = {d_scale[F], d_shift[F]} of the block's rows.
+template <typename T>
+struct NormBackward {
+    const T *g, *x, *out;
+    long long ldg, ldx, ldo;
+    const float *scale, *mean, *rstd;
+    const int *mirror2worker;      // rows with an entry other than -1 are left out of the sums
+    T *dx;
+    long long ld;
+    float *sums;
+    int n, F;
+};
+
+template <typename T, int L, int U, bool VEC>
+__global__ void __launch_bounds__(L > 256 ? L : 256) layer_norm_backward_kernel(NormBackward<T> p) {
+    using S = RowShape<T, L, U, VEC>;
+    const int gl = threadIdx.x % L, F = p.F;
+    float a[S::PER], d_scale[S::PER], d_shift[S::PER];
+    S::load_vector(p.scale, F, gl, a);
+#pragma unroll
+    for (int i = 0; i < S::PER; ++i) d_scale[i] = d_shift[i] = 0;
+    const long long first = (long long)blockIdx.x * S::GROUPS, group = threadIdx.x / L, step = (long long)gridDim.x * S::GROUPS;
+    for (long long row0 = first; row0 < p.n; row0 += step) {
+        const bool live = row0 + group < p.n;
+        const long long row = live ? row0 + group : p.n - 1;
+        float g[S::PER], h[S::PER];
+        S::load(p.g + row * p.ldg, F, gl, g);
+        S::load(p.x + row * p.ldx, F, gl, h);
+        if (p.out) {
+            float o[S::PER];
+            S::load(p.out + row * p.ldo, F, gl, o);
+#pragma unroll
+            for (int i = 0; i < S::PER; ++i) g[i] = o[i] > 0.f ? g[i] : 0.f;
+        }
+        const float m = __ldg(p.mean + row), r = __ldg(p.rstd + row);
+        const bool counts = live && (!p.mirror2worker || __ldg(p.mirror2worker + row) == -1);
+        float2 s = make_float2(0, 0);
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i) {
+            h[i] = S::column(gl, i) < F ? (h[i] - m) * r : 0.f;
+            if (counts) {
+                d_scale[i] += g[i] * h[i];
+                d_shift[i] += g[i];
+            }
+            g[i] *= a[i];
+            s.x += g[i];
+            s.y += g[i] * h[i];
+        }
+        s = sum_over_row<L>(s);
+        s.x /= F;
+        s.y /= F;
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i) g[i] = r * (g[i] - s.x - h[i] * s.y);
+        S::store(p.dx + row * p.ld, F, gl, g);
+    }
+    float *of_block = p.sums + (long long)blockIdx.x * 2 * F;
+    if (S::GROUPS == 1) {
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i)
+            if (S::column(gl, i) < F) {
+                of_block[S::column(gl, i)] = d_scale[i];
+                of_block[F + S::column(gl, i)] = d_shift[i];
+            }
+        return;
+    }
+    __shared__ float of_group[S::GROUPS > 1 ? S::THREADS * S::PER : 1];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i) of_group[(threadIdx.x / L * S::PER + i) * L + gl] = which ? d_shift[i] : d_scale[i];
+        __syncthreads();
+        for (int at = threadIdx.x; at < L * S::PER; at += S::THREADS) {
+            const int c = S::column(at % L, at / L);
+            if (c >= F) continue;
+            float sum = 0;
+            for (int w = 0; w < S::GROUPS; ++w) sum += of_group[w * S::PER * L + at];
+            of_block[which * F + c] = sum;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(NormBackward<T> p) {
+    const int F = p.F;
+    float *d_scale = p.sums + (long long)blockIdx.x * 2 * F, *d_shift = d_scale + F;      // a thread always has the same columns
+    for (int c = threadIdx.x; c < F; c += kWideThreads) d_scale[c] = d_shift[c] = 0;
+    for (long long row = blockIdx.x; row < p.n; row += gridDim.x) {
+        const T *in = p.x + row * p.ldx, *dy = p.g + row * p.ldg, *out = p.out ? p.out + row * p.ldo : nullptr;
+        const float m = __ldg(p.mean + row), r = __ldg(p.rstd + row);
+        const bool counts = !p.mirror2worker || __ldg(p.mirror2worker + row) == -1;
+        float2 s = make_float2(0, 0);
+        for (int c = threadIdx.x; c < F; c += kWideThreads) {
+            const float g = out && !(to_float(out[c]) > 0.f) ? 0.f : to_float(dy[c]), h = (to_float(in[c]) - m) * r;
+            if (counts) {
+                d_scale[c] += g * h;
+                d_shift[c] += g;
+            }
+            s.x += g * __ldg(p.scale + c);
+            s.y += g * __ldg(p.scale + c) * h;
+        }
+        s = sum_over_row<kWideThreads>(s);
+        for (int c = threadIdx.x; c < F; c += kWideThreads) {
+            const float g = out && !(to_float(out[c]) > 0.f) ? 0.f : to_float(dy[c]), h = (to_float(in[c]) - m) * r;
+            p.dx[row * p.ld + c] = from_float<T>(r * (g * __ldg(p.scale + c) - s.x / F - h * (s.y / F)));
+        }
+    }
+}
+
+// d_scale, d_shift = the blocks' sums, in order.  A block has 32 of the 2F columns, its warps every eighth of the sums.
+__global__ void __launch_bounds__(256) fold_norm_sums_kernel(const float *__restrict__ sums, int blocks, int F, float *__restrict__ d_scale,
+                                                             float *__restrict__ d_shift) {
+    __shared__ double of_warp[8][32];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+    double sum = 0;
+    if (c < 2 * F) {
+#pragma unroll 4
+        for (int b = w; b < blocks; b += 8) sum += __ldg(sums + (long long)b * 2 * F + c);
+    }
+    of_warp[w][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (w == 0 && c < 2 * F) {
+        for (int i = 1; i < 8; ++i) sum += of_warp[i][threadIdx.x];
+        if (c < F) {
+            if (d_scale) d_scale[c] = (float)sum;
+        } else if (d_shift) {
+            d_shift[c - F] = (float)sum;
+        }
+    }
+}
+
+// f(shape) for the lanes of a row of so many vectors: shape.L lanes with shape.U vectors each; L = 0: too wide for a block's registers.
+template <int LANES, int VECTORS> struct NormShape { static constexpr int L = LANES, U = VECTORS; };
+template <typename F>
+static int with_norm_shape(int vectors, const F &f) {
+    if (vectors <= 8) return f(NormShape<8, 1>());
+    if (vectors <= 16) return f(NormShape<8, 2>());
+    if (vectors <= 32) return f(NormShape<32, 1>());
+    if (vectors <= 64) return f(NormShape<32, 2>());
+    if (vectors <= 128) return f(NormShape<32, 4>());
+    if (vectors <= 512) return f(NormShape<256, 2>());
+    if (vectors <= 1024) return f(NormShape<256, 4>());
+    if (vectors <= 2048) return f(NormShape<512, 4>());
+    return f(NormShape<0, 0>());
+}
+
+struct NormGrid {
+    int groups, blocks;      // rows a block takes at once; blocks
+};
+static NormGrid norm_grid(int type, int n, int F, int sms, int blocks_per_sm) {
+    const int V = type == DRONE_F32 ? 4 : 8, vectors = ceil_div(F, V);
+    NormGrid g;
+    g.groups = vectors <= 16 ? 32 : vectors <= 128 ? 8 : 1;
+    g.blocks = (int)std::min<long long>(((long long)n + g.groups - 1) / g.groups, (long long)sms * blocks_per_sm);
+    return g;
+}
+constexpr int kBackwardBlocksPerSm = 4;
+
+}  // namespace drone
+
+using namespace drone;
+
+extern "C" {
+
+int drone_layer_norm(int type, int n_rows, int F, const void *d_X, int ldx, const float *d_scale, const float *d_shift, float eps, int relu, void *d_Y,
+                     int ldy, float *d_mean, float *d_rstd, void *stream) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type), "drone_layer_norm: type=%d", type);
+    DRONE_REQUIRE(n_rows >= 0 && F >= 1 && F <= DRONE_NORM_MAX_WIDTH && ldx >= F && ldy >= F && eps > 0 && (relu == 0 || relu == 1),
+                  "drone_layer_norm: n_rows=%d F=%d ldx=%d ldy=%d eps=%g relu=%d", n_rows, F, ldx, ldy, eps, relu);
+    if (n_rows == 0) return DRONE_OK;
+    DRONE_REQUIRE(d_X && d_scale && d_shift && d_Y, "drone_layer_norm: NULL argument");
+    DRONE_REQUIRE(DRONE_ALIGNED(d_X, type) && DRONE_ALIGNED(d_Y, type), "drone_layer_norm: an operand is not aligned to its type");
+    cudaStream_t st = (cudaStream_t)stream;
+    int sms = 0, rc = device_sms(&sms);
+    if (rc) return rc;
+    const int blocks = norm_grid(type, n_rows, F, sms, 8).blocks;
+    return with_type(type, [&](auto tag) {
+        using T = typename decltype(tag)::T;
+        constexpr int V = Vec<T>::N;
+        const bool vec = F % V == 0 && rows_on_16_bytes(d_X, ldx, sizeof(T)) && rows_on_16_bytes(d_Y, ldy, sizeof(T));
+        return with_norm_shape(ceil_div(F, V), [&](auto shape) {
+            constexpr int L = decltype(shape)::L, U = decltype(shape)::U;
+            auto launch = [&](auto kernel, int threads) {
+                kernel<<<blocks, threads, 0, st>>>((const T *)d_X, ldx, d_scale, d_shift, n_rows, F, eps, relu != 0, (T *)d_Y, ldy, d_mean, d_rstd);
+            };
+            if constexpr (L == 0) launch(layer_norm_wide_kernel<T>, kWideThreads);
+            else if (vec) launch(layer_norm_kernel<T, L, U, true>, L > 256 ? L : 256);
+            else launch(layer_norm_kernel<T, L, U, false>, L > 256 ? L : 256);
+            DRONE_LAUNCH_CHECK("layer_norm_kernel");
+            return DRONE_OK;
+        });
+    });
+}
+
+int drone_layer_norm_backward_scratch(int type, int n_rows, int F, long long *n_floats) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type) && n_rows >= 0 && F >= 1 && F <= DRONE_NORM_MAX_WIDTH && n_floats,
+                  "drone_layer_norm_backward_scratch: type=%d n_rows=%d F=%d", type, n_rows, F);
+    int sms = 0;
+    const int rc = device_sms(&sms);
+    if (rc) return rc;
+    *n_floats = 2LL * F * norm_grid(type, n_rows, F, sms, kBackwardBlocksPerSm).blocks;
+    return DRONE_OK;
+}
+
+int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int ldg, const void *d_X, int ldx, const float *d_scale,
+                              const float *d_mean, const float *d_rstd, const void *d_out, int ldo, const int *d_mirror2worker, void *d_dX, int ld,
+                              float *d_scale_grad, float *d_shift_grad, float *d_scratch, long long n_scratch, void *stream) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type), "drone_layer_norm_backward: type=%d", type);
+    DRONE_REQUIRE(n_rows >= 0 && F >= 1 && F <= DRONE_NORM_MAX_WIDTH && ldg >= F && ldx >= F && ld >= F && (!d_out || ldo >= F),
+                  "drone_layer_norm_backward: n_rows=%d F=%d ldg=%d ldx=%d ldo=%d ld=%d", n_rows, F, ldg, ldx, ldo, ld);
+    DRONE_REQUIRE(n_rows == 0 || (d_G && d_X && d_scale && d_mean && d_rstd && d_dX), "drone_layer_norm_backward: NULL argument");
+    DRONE_REQUIRE(DRONE_ALIGNED(d_G, type) && DRONE_ALIGNED(d_X, type) && DRONE_ALIGNED(d_out, type) && DRONE_ALIGNED(d_dX, type),
+                  "drone_layer_norm_backward: an operand is not aligned to its type");
+    cudaStream_t st = (cudaStream_t)stream;
+    int sms = 0, rc = device_sms(&sms);
+    if (rc) return rc;
+    const int blocks = norm_grid(type, n_rows, F, sms, kBackwardBlocksPerSm).blocks;
+    const long long need = 2LL * F * blocks;
+    DRONE_REQUIRE(n_scratch >= need && (need == 0 || d_scratch), "drone_layer_norm_backward: %lld floats of scratch, %lld needed", n_scratch, need);
+    if (n_rows > 0) {
+        rc = with_type(type, [&](auto tag) {
+            using T = typename decltype(tag)::T;
+            constexpr int V = Vec<T>::N;
+            const bool vec = F % V == 0 && rows_on_16_bytes(d_G, ldg, sizeof(T)) && rows_on_16_bytes(d_X, ldx, sizeof(T)) &&
+                             rows_on_16_bytes(d_dX, ld, sizeof(T)) && (!d_out || rows_on_16_bytes(d_out, ldo, sizeof(T)));
+            const NormBackward<T> p = {(const T *)d_G, (const T *)d_X, (const T *)d_out, ldg, ldx, ldo, d_scale, d_mean, d_rstd, d_mirror2worker,
+                                       (T *)d_dX, ld, d_scratch, n_rows, F};
+            return with_norm_shape(ceil_div(F, V), [&](auto shape) {
+                constexpr int L = decltype(shape)::L, U = decltype(shape)::U;
+                if constexpr (L == 0) layer_norm_backward_wide_kernel<T><<<blocks, kWideThreads, 0, st>>>(p);
+                else if (vec) layer_norm_backward_kernel<T, L, U, true><<<blocks, L > 256 ? L : 256, 0, st>>>(p);
+                else layer_norm_backward_kernel<T, L, U, false><<<blocks, L > 256 ? L : 256, 0, st>>>(p);
+                DRONE_LAUNCH_CHECK("layer_norm_backward_kernel");
+                return DRONE_OK;
+            });
+        });
+        if (rc) return rc;
+    }
+    if (!d_scale_grad && !d_shift_grad) return DRONE_OK;
+    fold_norm_sums_kernel<<<ceil_div(2LL * F, 32), 256, 0, st>>>(d_scratch, blocks, F, d_scale_grad, d_shift_grad);
+    DRONE_LAUNCH_CHECK("fold_norm_sums_kernel");
+    return DRONE_OK;
+}
+
+}  // extern "C"

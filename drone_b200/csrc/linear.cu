@@ -1,0 +1,255 @@
+// Products of a dense layer, Y = activation(X W + bias) + residual, and its backward pass.
+#include "dense_types.cuh"
+
+#include <algorithm>
+
+namespace drone {
+
+// Where a product's tiles go: through the epilogue to Y (and pre), or as float shares of the sum.
+template <typename T>
+struct LinearOut {
+    const float *bias;
+    int activation;
+    const T *residual;
+    long long ldr;
+    T *y;
+    long long ldy;
+    T *pre;
+    long long ldp;
+    float *shares;      // not NULL: [share][M][N]
+    __device__ void put(int share, long long r, int c, long long M, int N, float acc) const {
+        if (shares) {
+            shares[(share * M + r) * N + c] = acc;
+            return;
+        }
+        const float z = bias ? acc + __ldg(bias + c) : acc;
+        if (pre) pre[r * ldp + c] = from_float<T>(z);
+        float v = activate(z, activation);
+        if (residual) v += to_float(residual[r * ldr + c]);
+        y[r * ldy + c] = from_float<T>(v);
+    }
+};
+
+// C[M, N] = A[M, K] B[K, N] over k in [share * blockIdx.z, ...), operands with any two strides.
+template <typename T>
+__global__ void __launch_bounds__(256)
+product_kernel(const T *__restrict__ A, long long sam, long long sak, const T *__restrict__ B, long long sbk, long long sbn, int M, int N, int K, int share,
+               LinearOut<T> out) {
+    __shared__ float a[16][64 + 4], b[16][64 + 4];
+    const long long m0 = (long long)blockIdx.x * 64;
+    const int n0 = blockIdx.y * 64, k0 = blockIdx.z * share, k1 = min(K, k0 + share);
+    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
+    float acc[4][4] = {};
+    for (int k = k0; k < k1; k += 16) {
+        for (int i = threadIdx.x; i < 16 * 64; i += 256) {
+            const int ka = sak == 1 ? i % 16 : i / 64, ma = sak == 1 ? i / 16 : i % 64;
+            a[ka][ma] = m0 + ma < M && k + ka < k1 ? to_float(A[(m0 + ma) * sam + (long long)(k + ka) * sak]) : 0.f;
+            const int kb = sbk == 1 ? i % 16 : i / 64, nb = sbk == 1 ? i / 16 : i % 64;
+            b[kb][nb] = n0 + nb < N && k + kb < k1 ? to_float(B[(long long)(k + kb) * sbk + (n0 + nb) * sbn]) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < 16; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[kk][tm * 4 + i], b[kk][tn * 4 + j], acc[i][j]);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (m0 + tm * 4 + i < M && n0 + tn * 4 + j < N) out.put(blockIdx.z, m0 + tm * 4 + i, n0 + tn * 4 + j, M, N, acc[i][j]);
+}
+
+// Shares of a product, added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) add_product_shares_kernel(const float *__restrict__ parts, int shares, int M, int N, T *__restrict__ out, long long ld) {
+    const long long count = (long long)M * N;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < count; i += gridDim.x * 256LL) {
+        double sum = 0;
+#pragma unroll 8
+        for (int s = 0; s < shares; ++s) sum += __ldg(parts + s * count + i);
+        out[i / N * ld + i % N] = from_float<T>((float)sum);
+    }
+}
+
+// dZ = G * activation'(pre) and the column sums of a block's rows.  A block has 32 columns and 8 rows at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) activation_gradient_kernel(const T *G, long long ldg, const T *pre, long long ldp, int activation, int n, int N,
+                                                                  int rows_per_block, T *dZ, long long ldz, float *sums) {
+    __shared__ float of_warp[8][32];
+    const int c = blockIdx.y * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+    const long long r0 = (long long)blockIdx.x * rows_per_block, r1 = min((long long)n, r0 + rows_per_block);
+    float sum = 0;
+    if (c < N)
+        for (long long r = r0 + w; r < r1; r += 8) {
+            float d = to_float(G[r * ldg + c]);
+            if (activation != DRONE_ACT_NONE) d *= activation_slope(to_float(pre[r * ldp + c]), activation);
+            if (dZ) dZ[r * ldz + c] = from_float<T>(d);
+            sum += d;
+        }
+    if (!sums) return;
+    of_warp[w][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (w == 0 && c < N) {
+        for (int i = 1; i < 8; ++i) sum += of_warp[i][threadIdx.x];
+        sums[(long long)blockIdx.x * N + c] = sum;
+    }
+}
+__global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ sums, int blocks, int N, float *__restrict__ out) {
+    __shared__ double of_warp[8][32];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+    double sum = 0;
+    if (c < N) {
+#pragma unroll 4
+        for (int b = w; b < blocks; b += 8) sum += __ldg(sums + (long long)b * N + c);
+    }
+    of_warp[w][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (w == 0 && c < N) {
+        for (int i = 1; i < 8; ++i) sum += of_warp[i][threadIdx.x];
+        out[c] = (float)sum;
+    }
+}
+
+struct Shares {
+    int share, count;
+};
+static Shares product_shares(int M, int N, int K, int sms) {
+    const long long tiles = (long long)ceil_div(M, 64) * ceil_div(N, 64);
+    const int most = (int)std::max(1LL, 4LL * sms / tiles);
+    Shares s;
+    s.share = std::max(64, ceil_div(ceil_div(K, most), 16) * 16);
+    s.count = std::max(1, ceil_div(K, s.share));
+    return s;
+}
+
+static int rows_per_gradient_block(int n, int N, int sms, int *blocks) {
+    const int columns = ceil_div(N, 32);
+    const int most = std::max(1, 8 * sms / columns);
+    const int rows = std::max(64, ceil_div(n, most));
+    *blocks = ceil_div(n, rows);
+    return rows;
+}
+
+}  // namespace drone
+
+using namespace drone;
+
+#define DRONE_LINEAR_SIZES(n_rows, K, N) \
+    ((n_rows) >= 0 && (n_rows) <= 1 << 30 && (K) >= 1 && (K) <= 1 << 15 && (N) >= 1 && (N) <= 1 << 15)
+
+extern "C" {
+
+int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_W, int ldw, int transposed, const float *d_bias,
+                 int activation, const void *d_residual, int ldr, void *d_Y, int ldy, void *d_pre, int ldp, void *stream) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type), "drone_linear: type=%d", type);
+    DRONE_REQUIRE(DRONE_LINEAR_SIZES(n_rows, K, N), "drone_linear: n_rows=%d K=%d N=%d", n_rows, K, N);
+    DRONE_REQUIRE(activation >= DRONE_ACT_NONE && activation <= DRONE_ACT_SILU, "drone_linear: activation=%d", activation);
+    DRONE_REQUIRE((transposed == 0 || transposed == 1) && ldx >= K && ldw >= (transposed ? K : N) && ldy >= N && (!d_residual || ldr >= N) &&
+                  (!d_pre || ldp >= N), "drone_linear: ldx=%d ldw=%d transposed=%d ldr=%d ldy=%d ldp=%d", ldx, ldw, transposed, ldr, ldy, ldp);
+    if (n_rows == 0) return DRONE_OK;
+    DRONE_REQUIRE(d_X && d_W && d_Y, "drone_linear: NULL argument");
+    DRONE_REQUIRE(DRONE_ALIGNED(d_X, type) && DRONE_ALIGNED(d_W, type) && DRONE_ALIGNED(d_Y, type) && DRONE_ALIGNED(d_residual, type) &&
+                  DRONE_ALIGNED(d_pre, type), "drone_linear: an operand is not aligned to its type");
+    cudaStream_t st = (cudaStream_t)stream;
+    return with_type(type, [&](auto tag) {
+        using T = typename decltype(tag)::T;
+        const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr};
+        const dim3 grid(ceil_div(n_rows, 64), ceil_div(N, 64), 1);
+        product_kernel<T><<<grid, 256, 0, st>>>((const T *)d_X, ldx, 1, (const T *)d_W, transposed ? 1 : ldw, transposed ? ldw : 1, n_rows, N, K, K, out);
+        DRONE_LAUNCH_CHECK("product_kernel");
+        return DRONE_OK;
+    });
+}
+
+int drone_activation_gradient_scratch(int n_rows, int N, long long *n_floats) {
+    DRONE_REQUIRE(DRONE_LINEAR_SIZES(n_rows, 1, N) && n_floats, "drone_activation_gradient_scratch: n_rows=%d N=%d", n_rows, N);
+    int sms = 0, blocks = 0;
+    const int rc = device_sms(&sms);
+    if (rc) return rc;
+    rows_per_gradient_block(n_rows, N, sms, &blocks);
+    *n_floats = (long long)blocks * N;
+    return DRONE_OK;
+}
+
+int drone_activation_gradient(int type, int n_rows, int N, const void *d_G, int ldg, const void *d_pre, int ldp, int activation, void *d_dZ, int ldz,
+                              float *d_bias_grad, float *d_scratch, long long n_scratch, void *stream) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type), "drone_activation_gradient: type=%d", type);
+    DRONE_REQUIRE(DRONE_LINEAR_SIZES(n_rows, 1, N), "drone_activation_gradient: n_rows=%d N=%d", n_rows, N);
+    DRONE_REQUIRE(activation >= DRONE_ACT_NONE && activation <= DRONE_ACT_SILU, "drone_activation_gradient: activation=%d", activation);
+    const bool reads_pre = activation != DRONE_ACT_NONE;
+    DRONE_REQUIRE(ldg >= N && (!reads_pre || ldp >= N) && (!d_dZ || ldz >= N), "drone_activation_gradient: ldg=%d ldp=%d ldz=%d", ldg, ldp, ldz);
+    DRONE_REQUIRE(n_rows == 0 || (d_G && (d_pre || !reads_pre)), "drone_activation_gradient: NULL argument");
+    DRONE_REQUIRE(DRONE_ALIGNED(d_G, type) && DRONE_ALIGNED(d_pre, type) && DRONE_ALIGNED(d_dZ, type),
+                  "drone_activation_gradient: an operand is not aligned to its type");
+    cudaStream_t st = (cudaStream_t)stream;
+    int sms = 0, blocks = 0;
+    const int rc = device_sms(&sms);
+    if (rc) return rc;
+    const int rows = rows_per_gradient_block(n_rows, N, sms, &blocks);
+    if (d_bias_grad) {
+        const long long need = (long long)blocks * N;
+        DRONE_REQUIRE(n_scratch >= need && (need == 0 || d_scratch), "drone_activation_gradient: %lld floats of scratch, %lld needed", n_scratch, need);
+    }
+    if (n_rows > 0 && (d_dZ || d_bias_grad)) {
+        const int launched = with_type(type, [&](auto tag) {
+            using T = typename decltype(tag)::T;
+            activation_gradient_kernel<T><<<dim3(blocks, ceil_div(N, 32)), 256, 0, st>>>((const T *)d_G, ldg, (const T *)d_pre, ldp, activation, n_rows, N,
+                                                                                          rows, (T *)d_dZ, ldz, d_bias_grad ? d_scratch : nullptr);
+            DRONE_LAUNCH_CHECK("activation_gradient_kernel");
+            return DRONE_OK;
+        });
+        if (launched) return launched;
+    }
+    if (d_bias_grad) {
+        fold_columns_kernel<<<ceil_div(N, 32), 256, 0, st>>>(d_scratch, blocks, N, d_bias_grad);
+        DRONE_LAUNCH_CHECK("fold_columns_kernel");
+    }
+    return DRONE_OK;
+}
+
+int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, int transposed, long long *n_floats) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && (transposed == 0 || transposed == 1) && n_floats,
+                  "drone_linear_weight_gradient_scratch: type=%d n_rows=%d K=%d N=%d transposed=%d", type, n_rows, K, N, transposed);
+    int sms = 0;
+    const int rc = device_sms(&sms);
+    if (rc) return rc;
+    const Shares s = product_shares(transposed ? N : K, transposed ? K : N, n_rows, sms);
+    *n_floats = (long long)s.count * K * N;
+    return DRONE_OK;
+}
+
+int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_dZ, int ldz, int transposed, void *d_dW,
+                                 int ldw, float *d_scratch, long long n_scratch, void *stream) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type), "drone_linear_weight_gradient: type=%d", type);
+    DRONE_REQUIRE(DRONE_LINEAR_SIZES(n_rows, K, N), "drone_linear_weight_gradient: n_rows=%d K=%d N=%d", n_rows, K, N);
+    DRONE_REQUIRE((transposed == 0 || transposed == 1) && ldx >= K && ldz >= N && ldw >= (transposed ? K : N),
+                  "drone_linear_weight_gradient: ldx=%d ldz=%d ldw=%d transposed=%d", ldx, ldz, ldw, transposed);
+    DRONE_REQUIRE(d_dW && (n_rows == 0 || (d_X && d_dZ)), "drone_linear_weight_gradient: NULL argument");
+    DRONE_REQUIRE(DRONE_ALIGNED(d_X, type) && DRONE_ALIGNED(d_dZ, type) && DRONE_ALIGNED(d_dW, type),
+                  "drone_linear_weight_gradient: an operand is not aligned to its type");
+    cudaStream_t st = (cudaStream_t)stream;
+    int sms = 0;
+    const int rc = device_sms(&sms);
+    if (rc) return rc;
+    const int rows = transposed ? N : K, columns = transposed ? K : N;
+    const Shares s = product_shares(rows, columns, n_rows, sms);
+    const long long need = (long long)s.count * K * N;
+    DRONE_REQUIRE(n_scratch >= need && d_scratch, "drone_linear_weight_gradient: %lld floats of scratch, %lld needed", n_scratch, need);
+    return with_type(type, [&](auto tag) {
+        using T = typename decltype(tag)::T;
+        const T *a = (const T *)(transposed ? d_dZ : d_X), *b = (const T *)(transposed ? d_X : d_dZ);
+        const LinearOut<T> out = {nullptr, DRONE_ACT_NONE, nullptr, 0, nullptr, 0, nullptr, 0, d_scratch};
+        product_kernel<T><<<dim3(ceil_div(rows, 64), ceil_div(columns, 64), s.count), 256, 0, st>>>(a, 1, transposed ? ldz : ldx, b, transposed ? ldx : ldz, 1,
+                                                                                                   rows, columns, n_rows, s.share, out);
+        add_product_shares_kernel<T><<<std::min(ceil_div((long long)rows * columns, 256), sms * 8), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
+        DRONE_LAUNCH_CHECK("product_kernel");
+        count_launch();
+        return DRONE_OK;
+    });
+}
+
+}  // extern "C"

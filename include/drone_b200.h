@@ -354,6 +354,82 @@ int drone_weight_gradient_scratch(int K, int M, int N, long long *n_floats);
 int drone_weight_gradient(int K, int M, int N, const float *d_A, int lda, const float *d_B, int ldb, float *d_C, float *d_scratch,
                           long long n_scratch, void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* Dense operators beside the aggregation                                      */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * What a training step or an answer of a residual graph network, or of a model taught by one, needs besides its
+ * aggregations.  The reference has the product alone (CUDAMatmul, cuda_gcn/src/cuda/cuda_module.cu:63-114) and none of
+ * the others.  Matrices are row-major with a leading dimension in values, of one of three element types, at addresses
+ * aligned to the type; vectors (bias, scale, shift, mean, their gradients) are float.  Sums are formed in 32 bits or
+ * more and rounded to the type once; the same bits every time.  Rows <= 2^30.  All are asynchronous on `stream` and run
+ * on the current device.  Scratch is the caller's, as many floats as the _scratch function says (asked with the same
+ * device current) for these sizes, and is in use until the call's work on the stream is done.
+ */
+#define DRONE_F32  0
+#define DRONE_BF16 1
+#define DRONE_F16  2
+
+#define DRONE_ACT_NONE 0
+#define DRONE_ACT_RELU 1
+#define DRONE_ACT_GELU 2   /* z * Phi(z), the exact form */
+#define DRONE_ACT_SILU 3   /* z / (1 + exp(-z)) */
+
+/* Y = activation(X . W + bias) + residual for X [n_rows, K] and W [K, N], or with `transposed` W [N, K].  K, N <= 32768.
+ * d_bias, d_residual, d_pre may be NULL; d_pre receives the values before the activation.  d_residual may be d_Y with the
+ * same leading dimension; no other operand may overlap an output.  Products of floats are as exact as float
+ * multiply-adds. */
+int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_W, int ldw, int transposed,
+                 const float *d_bias, int activation, const void *d_residual, int ldr, void *d_Y, int ldy, void *d_pre, int ldp,
+                 void *stream);
+
+/* The step from the gradient of Y to that before the activation, and to that of the bias: dZ = G * activation'(pre),
+ * bias_grad = column sums of the unrounded dZ.  d_dZ may be d_G with the same leading dimension, or NULL (sums only), d_bias_grad may be
+ * NULL; d_pre is not read without an activation; for the ReLU anything with the same sign will do. */
+int drone_activation_gradient_scratch(int n_rows, int N, long long *n_floats);
+int drone_activation_gradient(int type, int n_rows, int N, const void *d_G, int ldg, const void *d_pre, int ldp, int activation,
+                              void *d_dZ, int ldz, float *d_bias_grad, float *d_scratch, long long n_scratch, void *stream);
+
+/* dW [K, N] = X^T . dZ, or with `transposed` dW [N, K] = dZ^T . X.  (dX is drone_linear of dZ with W and the other value of
+ * `transposed`.) */
+int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, int transposed, long long *n_floats);
+int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_dZ, int ldz, int transposed,
+                                 void *d_dW, int ldw, float *d_scratch, long long n_scratch, void *stream);
+
+/* y = (x - mean) * rstd * scale + shift over the F values of each row, with rstd = 1 / sqrt(variance + eps), and max(y, 0) with
+ * `relu`.  d_mean, d_rstd [n_rows] may be NULL.  d_Y may be d_X with the same leading dimension.  eps > 0. */
+#define DRONE_NORM_MAX_WIDTH 65536
+int drone_layer_norm(int type, int n_rows, int F, const void *d_X, int ldx, const float *d_scale, const float *d_shift, float eps,
+                     int relu, void *d_Y, int ldy, float *d_mean, float *d_rstd, void *stream);
+
+/* dX and the gradients of scale and shift from G, that of y.  d_out: the forward pass's output where it had a ReLU (G counts where
+ * it is positive), else NULL.  d_mirror2worker: rows with an entry other than -1 are left out of the sums over rows (see
+ * drone_clear_mirror_rows); NULL: none.  d_dX may be d_G or d_X with the same leading dimension; d_scale_grad, d_shift_grad may be
+ * NULL. */
+int drone_layer_norm_backward_scratch(int type, int n_rows, int F, long long *n_floats);
+int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int ldg, const void *d_X, int ldx, const float *d_scale,
+                              const float *d_mean, const float *d_rstd, const void *d_out, int ldo, const int *d_mirror2worker,
+                              void *d_dX, int ld, float *d_scale_grad, float *d_shift_grad, float *d_scratch, long long n_scratch,
+                              void *stream);
+
+/* Loss and gradient of [n_rows, classes] logits against a teacher's `top` best logits of each row: values d_teacher [n_rows, top] (of
+ * teacher_type) of the classes d_classes [n_rows, top].  With the temperature t, q = softmax(teacher / t) over the row's entries and
+ * p = softmax(logits / t):
+ *   d_loss[0] = mean over the rows with an entry of t^2 * sum q (log q - log p)
+ *   d_loss[1] = mean over the rows with d_labelled[r] != 0 of the cross-entropy at t = 1 (0 without d_truth, d_labelled)
+ *   d_grad    = soft * t (p - q) + hard * (softmax(logits) - one-hot) * labelled, not divided by the numbers of rows
+ * as drone_softmax_loss has it.  Entries with a negative class or a value of minus infinity are left out, a class that is there
+ * twice has the sum of both; a row without entries has no soft part.  An entry's class of `classes` or more, or a d_truth outside
+ * 0..classes-1 in any row, makes that part of the loss and the row's gradient NaN.  d_scratch: DRONE_DISTILLATION_SCRATCH doubles.  d_grad
+ * may be d_logits with the same leading dimension. */
+#define DRONE_DISTILLATION_MAX_TOP 256
+#define DRONE_DISTILLATION_SCRATCH 4736
+int drone_distillation_loss(int type, int n_rows, int classes, const void *d_logits, int ld, int teacher_type, int top,
+                            const void *d_teacher, int ldt, const long long *d_classes, int ldc, float temperature,
+                            const long long *d_truth, const unsigned char *d_labelled, float soft, float hard, void *d_grad,
+                            int ld_grad, float *d_loss, double *d_scratch, void *stream);
+
 /*
  * Routing plan of one rank, from the reference's routing tables (host arrays,
  * indexed by local vertex id):
