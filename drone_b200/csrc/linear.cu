@@ -1,67 +1,9 @@
 // Products of a dense layer, Y = activation(X W + bias) + residual, and its backward pass.
-#include "dense_types.cuh"
+#include "product_tile.cuh"
 
 #include <algorithm>
 
 namespace drone {
-
-// Where a product's tiles go: through the epilogue to Y (and pre), or as float shares of the sum.
-template <typename T>
-struct LinearOut {
-    const float *bias;
-    int activation;
-    const T *residual;
-    long long ldr;
-    T *y;
-    long long ldy;
-    T *pre;
-    long long ldp;
-    float *shares;      // not NULL: [share][M][N]
-    __device__ void put(int share, long long r, int c, long long M, int N, float acc) const {
-        if (shares) {
-            shares[(share * M + r) * N + c] = acc;
-            return;
-        }
-        const float z = bias ? acc + __ldg(bias + c) : acc;
-        if (pre) pre[r * ldp + c] = from_float<T>(z);
-        float v = activate(z, activation);
-        if (residual) v += to_float(residual[r * ldr + c]);
-        y[r * ldy + c] = from_float<T>(v);
-    }
-};
-
-// C[M, N] = A[M, K] B[K, N] over k in [share * blockIdx.z, ...), operands with any two strides.
-template <typename T>
-__global__ void __launch_bounds__(256)
-product_kernel(const T *__restrict__ A, long long sam, long long sak, const T *__restrict__ B, long long sbk, long long sbn, int M, int N, int K, int share,
-               LinearOut<T> out) {
-    __shared__ float a[16][64 + 4], b[16][64 + 4];
-    const long long m0 = (long long)blockIdx.x * 64;
-    const int n0 = blockIdx.y * 64, k0 = blockIdx.z * share, k1 = min(K, k0 + share);
-    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-    float acc[4][4] = {};
-    for (int k = k0; k < k1; k += 16) {
-        for (int i = threadIdx.x; i < 16 * 64; i += 256) {
-            const int ka = sak == 1 ? i % 16 : i / 64, ma = sak == 1 ? i / 16 : i % 64;
-            a[ka][ma] = m0 + ma < M && k + ka < k1 ? to_float(A[(m0 + ma) * sam + (long long)(k + ka) * sak]) : 0.f;
-            const int kb = sbk == 1 ? i % 16 : i / 64, nb = sbk == 1 ? i / 16 : i % 64;
-            b[kb][nb] = n0 + nb < N && k + kb < k1 ? to_float(B[(long long)(k + kb) * sbk + (n0 + nb) * sbn]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[kk][tm * 4 + i], b[kk][tn * 4 + j], acc[i][j]);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (m0 + tm * 4 + i < M && n0 + tn * 4 + j < N) out.put(blockIdx.z, m0 + tm * 4 + i, n0 + tn * 4 + j, M, N, acc[i][j]);
-}
 
 // Shares of a product, added in order.
 template <typename T>
@@ -114,14 +56,16 @@ __global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restri
     }
 }
 
+// How the rows of a weight gradient, its K, are cut: two blocks an SM, but a share of four steps at least.
 struct Shares {
-    int share, count;
+    int bn, share, count;
 };
-static Shares product_shares(int M, int N, int K, int sms) {
-    const long long tiles = (long long)ceil_div(M, 64) * ceil_div(N, 64);
-    const int most = (int)std::max(1LL, 4LL * sms / tiles);
+static Shares product_shares(int type, int M, int N, int K, int sms) {
+    const int step = type == DRONE_F32 ? TileShape<float>::KS : TileShape<__half>::KS;
     Shares s;
-    s.share = std::max(64, ceil_div(ceil_div(K, most), 16) * 16);
+    s.bn = N <= 64 ? 64 : 128;
+    const int most = std::max(1, 2 * sms / (ceil_div(M, 128) * ceil_div(N, s.bn)));
+    s.share = std::max(4 * step, ceil_div(ceil_div(K, most), step) * step);
     s.count = std::max(1, ceil_div(K, s.share));
     return s;
 }
@@ -157,11 +101,15 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
     cudaStream_t st = (cudaStream_t)stream;
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
-        const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr};
-        const dim3 grid(ceil_div(n_rows, 64), ceil_div(N, 64), 1);
-        product_kernel<T><<<grid, 256, 0, st>>>((const T *)d_X, ldx, 1, (const T *)d_W, transposed ? 1 : ldw, transposed ? ldw : 1, n_rows, N, K, K, out);
-        DRONE_LAUNCH_CHECK("product_kernel");
-        return DRONE_OK;
+        const auto fours = [](const void *p, long long ld) { return !p || ((reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && ld % 4 == 0); };
+        const bool in_fours = N % 4 == 0 && (reinterpret_cast<uintptr_t>(d_bias) & 15) == 0 && fours(d_Y, ldy) && fours(d_residual, ldr) && fours(d_pre, ldp);
+        const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr, in_fours};
+        const Operand<T> x = operand<T>(d_X, ldx), w = operand<T>(d_W, ldw);
+        if (N <= 64)
+            return transposed ? launch_product_tiles<T, 64, true, true>(x, w, n_rows, N, K, K, 1, out, st)
+                              : launch_product_tiles<T, 64, true, false>(x, w, n_rows, N, K, K, 1, out, st);
+        return transposed ? launch_product_tiles<T, 128, true, true>(x, w, n_rows, N, K, K, 1, out, st)
+                          : launch_product_tiles<T, 128, true, false>(x, w, n_rows, N, K, K, 1, out, st);
     });
 }
 
@@ -217,7 +165,7 @@ int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, int
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    const Shares s = product_shares(transposed ? N : K, transposed ? K : N, n_rows, sms);
+    const Shares s = product_shares(type, transposed ? N : K, transposed ? K : N, n_rows, sms);
     *n_floats = (long long)s.count * K * N;
     return DRONE_OK;
 }
@@ -236,18 +184,22 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
     const int rc = device_sms(&sms);
     if (rc) return rc;
     const int rows = transposed ? N : K, columns = transposed ? K : N;
-    const Shares s = product_shares(rows, columns, n_rows, sms);
+    if (n_rows == 0) {
+        DRONE_CUDA(cudaMemset2DAsync(d_dW, (size_t)ldw * type_size(type), 0, (size_t)columns * type_size(type), rows, st));
+        return DRONE_OK;
+    }
+    const Shares s = product_shares(type, rows, columns, n_rows, sms);
     const long long need = (long long)s.count * K * N;
     DRONE_REQUIRE(n_scratch >= need && d_scratch, "drone_linear_weight_gradient: %lld floats of scratch, %lld needed", n_scratch, need);
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
-        const T *a = (const T *)(transposed ? d_dZ : d_X), *b = (const T *)(transposed ? d_X : d_dZ);
-        const LinearOut<T> out = {nullptr, DRONE_ACT_NONE, nullptr, 0, nullptr, 0, nullptr, 0, d_scratch};
-        product_kernel<T><<<dim3(ceil_div(rows, 64), ceil_div(columns, 64), s.count), 256, 0, st>>>(a, 1, transposed ? ldz : ldx, b, transposed ? ldx : ldz, 1,
-                                                                                                   rows, columns, n_rows, s.share, out);
+        const Operand<T> a = transposed ? operand<T>(d_dZ, ldz) : operand<T>(d_X, ldx), b = transposed ? operand<T>(d_X, ldx) : operand<T>(d_dZ, ldz);
+        const LinearOut<T> out = {nullptr, DRONE_ACT_NONE, nullptr, 0, nullptr, 0, nullptr, 0, d_scratch, false};
+        const int launched = s.bn == 64 ? launch_product_tiles<T, 64, false, false>(a, b, rows, columns, n_rows, s.share, s.count, out, st)
+                                        : launch_product_tiles<T, 128, false, false>(a, b, rows, columns, n_rows, s.share, s.count, out, st);
+        if (launched) return launched;
         add_product_shares_kernel<T><<<std::min(ceil_div((long long)rows * columns, 256), sms * 8), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
-        DRONE_LAUNCH_CHECK("product_kernel");
-        count_launch();
+        DRONE_LAUNCH_CHECK("add_product_shares_kernel");
         return DRONE_OK;
     });
 }

@@ -111,8 +111,9 @@ def test_products_of_floats_are_floats(cuda_device):
     want = x.double() * w.double()
     got = dense.linear(x, w)
     # the smallest factors are 2^-60 times a value that may be far below 1, so that products fall below 2^-126, where floats are the
-    # multiples of 2^-149: a rounding there is off by half of that whatever the value's size
-    assert ((got - want).abs() <= 2 * STEP * want.abs() + 2.0 ** -150).all()
+    # multiples of 2^-149: the product is formed of six products of a float's parts, and each of them, cut off there, is off by less than
+    # one of these whatever its size
+    assert ((got - want).abs() <= 2 * STEP * want.abs() + 6 * 2.0 ** -149).all()
     big = torch.tensor([[3.4028235e38], [-3.4028235e38], [3.39e38], [1e-38], [1e-44]], device="cuda")
     got = dense.linear(big, torch.tensor([[1.0, 0.5, -1.0, 1e-30]], device="cuda"))
     want = big.double() * torch.tensor([[1.0, 0.5, -1.0, 1e-30]], device="cuda").double()
