@@ -6,6 +6,8 @@
 
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace drone {
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -16,12 +18,36 @@ template <> __device__ __forceinline__ float from_float<float>(float x) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
-// 16 bytes of values
-template <typename T>
-struct alignas(16) Vec {
-    static constexpr int N = 16 / sizeof(T);
+// N values side by side in memory (all or nothing: 1, 2, 4 ... of them) to floats and back, 16-bit ones in pairs: an instruction for two.
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Values {
     T v[N];
+    __device__ __forceinline__ void get(float *to) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = to_float(v[i]);
+    }
+    __device__ __forceinline__ void set(const float *from) {
+        if constexpr (sizeof(T) == 4 || N == 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = from_float<T>(from[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                unsigned pair;
+                if constexpr (std::is_same_v<T, __half>) {
+                    const __half2 p = __floats2half2_rn(from[i], from[i + 1]);
+                    pair = reinterpret_cast<const unsigned &>(p);
+                } else {
+                    const __nv_bfloat162 p = __floats2bfloat162_rn(from[i], from[i + 1]);
+                    pair = reinterpret_cast<const unsigned &>(p);
+                }
+                reinterpret_cast<unsigned *>(v)[i / 2] = pair;
+            }
+        }
+    }
 };
+
+template <typename T> constexpr int kVector = 16 / sizeof(T);      // values in 16 bytes
 
 // z -> activation(z) and its derivative.  A NaN stays one, also in the ReLU (max(NaN, 0) would be 0).
 __device__ __forceinline__ float activate(float z, int activation) {

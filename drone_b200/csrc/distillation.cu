@@ -10,6 +10,7 @@
 #include "dense_types.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace drone {
 
@@ -33,7 +34,7 @@ struct Distillation {
     int top;
     const long long *truth;
     const unsigned char *labelled;
-    float temperature, soft, hard;
+    float temperature, per_temperature, soft, hard;
     T *grad;
     long long ldg;
     LossSums *sums;
@@ -49,7 +50,7 @@ template <typename T>
 __device__ __forceinline__ int teacher_entry(const Distillation<T> &p, long long row, int j, float *value) {
     const long long c = __ldg(p.classes_of + row * p.ldc + j);
     const float v = load_as(p.teacher, row * p.ldt + j, p.teacher_type);
-    *value = c >= p.classes ? NAN : v / p.temperature;
+    *value = c >= p.classes ? NAN : v * p.per_temperature;
     if (c < 0 || v == -INFINITY) return -1;
     return c >= p.classes ? 0 : (int)c;
 }
@@ -88,199 +89,390 @@ __device__ __forceinline__ void write_sums(LossSums s, LossSums *sums) {
     }
 }
 
-// Rows of at most L * PER classes, L lanes a row.
+// 2^x, of x = (z - the row's maximum) log2(e) / t: three instructions an exponential, one of them of the special function unit.  Off by 2^-22 of
+// the value, as the rounding of x is.  (The difference comes first: a row whose logits are all the type's lowest value is a row of equal ones.)
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.44269504f;
+__device__ __forceinline__ float log_fast(float x) {      // off by 2^-22 and 2^-22 of the value
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y * 0.693147181f;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {      // one unit in the last place
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Below this a logit times log2(e) / t is finite for every t that is allowed, and one multiply-add forms the exponent.
+constexpr float kLargeLogit = 1e30f;
+
+// A sum of floats with what its additions cut off.
+struct LongSum {
+    float sum = 0, lost = 0;
+    __device__ __forceinline__ void add(float x) {
+        x -= lost;
+        const float now = sum + x;
+        lost = fabsf(now) < INFINITY ? (now - sum) - x : 0.f;
+        sum = now;
+    }
+};
+
+// Rows of (PER - 1) * L + 1 to PER * L classes, L lanes a row: logits and exponentials stay in registers, the teacher's shares are added up in
+// shared memory, where the lane of an entry finds its class.
+// 2.4 M rows of 47 classes, 8 entries, labels: 1.18 GB in 341 us (53 % of the copy rate; instructions, and the round trips of a row's reductions); as exponentials by division and expf, computed twice, and every
+// entry shown to every lane 1171 us.
 template <typename T, int L, int PER, bool HARD>
-__global__ void __launch_bounds__(256) distillation_rows_kernel(Distillation<T> p) {
-    const int gl = threadIdx.x & (L - 1), classes = p.classes;
-    const float t = p.temperature;
-    LossSums sums = {0, 0, 0, 0};
+__global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<T> p) {
+    constexpr int ROWS = 32 / L;      // of a warp
+    __shared__ float shares[8][ROWS][L * PER];
+    const int gl = threadIdx.x & (L - 1), classes = p.classes, lane = threadIdx.x & 31;
+    const unsigned group = (L < 32 ? (1u << L) - 1 : 0xffffffffu) << (lane & ~(L - 1));
+    float *const target = shares[threadIdx.x >> 5][lane / L];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) target[gl + u * L] = 0;
+    __syncwarp();
+    const float t = p.temperature, per_t = p.per_temperature, scale = kLog2e / t;
+    LongSum soft_sum, hard_sum;
+    float soft_rows = 0, hard_rows = 0;      // of this group: fewer than 2^24
+    auto inside = [&](int u) { return u < PER - 1 || gl + u * L < classes; };
     const long long step = (long long)gridDim.x * (256 / L), in_block = threadIdx.x / L;
+    // logits, label and the first L entries of a row, read while the row before is worked on
+    float next[PER], next_value = 0;
+    int next_class = -1, next_truth = 0;
+    bool next_labelled = false;
+    auto read = [&](long long row0) {
+        const long long row = row0 + in_block < p.n ? row0 + in_block : p.n - 1;      // whole warps stay for the shuffles
+        next_class = gl < p.top ? teacher_entry(p, row, gl, &next_value) : -1;
+        if (HARD) {
+            const long long c = __ldg(p.truth + row);
+            next_truth = c >= 0 && c < classes ? (int)c : -1;
+            next_labelled = __ldg(p.labelled + row) != 0;
+        }
+#pragma unroll
+        for (int u = 0; u < PER; ++u) next[u] = inside(u) ? to_float(p.logits[row * p.ld + gl + u * L]) : -INFINITY;
+    };
+    if ((long long)blockIdx.x * (256 / L) < p.n) read((long long)blockIdx.x * (256 / L));
     for (long long row0 = (long long)blockIdx.x * (256 / L); row0 < p.n; row0 += step) {
-        const bool live = row0 + in_block < p.n;      // whole warps stay for the shuffles
+        const bool live = row0 + in_block < p.n, labelled = next_labelled;
         const long long row = live ? row0 + in_block : p.n - 1;
         const T *x = p.logits + row * p.ld;
-        float v[PER], m = -INFINITY;
+        const int c0 = next_class, truth = next_truth;      // of the first L entries
+        const float value0 = next_value;
+        float v[PER], e[PER], m = -INFINITY, value;
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
-            v[u] = gl + u * L < classes ? to_float(x[gl + u * L]) : -INFINITY;
+            v[u] = next[u];
             m = fmaxf(m, v[u]);
         }
-        m = max_of_lanes<L>(m);
-        float s = 0, s1 = 0;
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            if (gl + u * L < classes) {
-                s += expf((v[u] - m) / t);
-                if (HARD) s1 += expf(v[u] - m);
-            }
-        }
-        s = sum_of_lanes<L>(s);
-        // the teacher's softmax
-        float tm = -INFINITY, ts = 0, value;
-        int entries = 0;
-        for (int j = gl; j < p.top; j += L)
+        if (row0 + step < p.n) read(row0 + step);
+        bool some = c0 >= 0;
+        float tm = some ? value0 : -INFINITY;
+        for (int j = L + gl; j < p.top; j += L)
             if (teacher_entry(p, row, j, &value) >= 0) {
                 tm = fmaxf(tm, value);
-                ++entries;
+                some = true;
             }
+        some = (__ballot_sync(0xffffffffu, some) & group) != 0;
+        m = max_of_lanes<L>(m);
         tm = max_of_lanes<L>(tm);
-        entries = sum_of_lanes<L>(entries);
-        for (int j = gl; j < p.top; j += L)
-            if (teacher_entry(p, row, j, &value) >= 0) ts += expf(value - tm);
-        ts = sum_of_lanes<L>(ts);
-        const float log_s = logf(s), log_ts = logf(ts);
-        float target[PER], soft = 0;
-#pragma unroll
-        for (int u = 0; u < PER; ++u) target[u] = 0;
-        for (int j0 = 0; j0 < p.top; j0 += L) {
-            int c = -1;
-            float q = 0;
-            if (j0 + gl < p.top) {
-                c = teacher_entry(p, row, j0 + gl, &value);
-                if (c >= 0) {
-                    q = expf(value - tm) / ts;
-                    if (q != 0.f) soft += q * ((value - tm - log_ts) - ((to_float(x[c]) - m) / t - log_s));
-                }
-            }
-#pragma unroll
-            for (int from = 0; from < L; ++from) {
-                if (j0 + from >= p.top) break;
-                const int c_j = __shfl_sync(0xffffffffu, c, from, L);
-                const float q_j = __shfl_sync(0xffffffffu, q, from, L);
-#pragma unroll
-                for (int u = 0; u < PER; ++u)
-                    if (c_j == gl + u * L) target[u] += q_j;
-            }
-        }
-        soft = sum_of_lanes<L>(soft);
-        float at_truth = 0, label = 0;
-        long long truth = 0;
-        if (HARD) {
-            s1 = sum_of_lanes<L>(s1);
-            truth = __ldg(p.truth + row);
-            label = truth < 0 || truth >= classes ? NAN : __ldg(p.labelled + row) ? 1.f : 0.f;
-            at_truth = truth < 0 || truth >= classes ? 0.f : to_float(x[truth]) - m;
-        }
-        __syncwarp();      // the gradient may lie on the logits, and other lanes have read this lane's
-        if (!live) continue;
-        T *g = p.grad + row * p.ldg;
-        const float soft_weight = p.soft * t * (isnan(ts) ? NAN : 1.f);
+        float s = 0, s1 = 0, ts = 0, apart = 0;
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
-            const int c = gl + u * L;
-            if (c >= classes) continue;
-            float d = entries ? soft_weight * (expf((v[u] - m) / t) / s - target[u]) : 0.f;
-            if (HARD && label != 0.f) d += p.hard * label * (expf(v[u] - m) / s1 - (c == truth ? 1.f : 0.f));
-            g[c] = from_float<T>(d);
+            const float z = v[u] - m;
+            e[u] = inside(u) ? exp2_fast(z * scale) : 0.f;
+            s += e[u];
+            if (HARD) {
+                v[u] = inside(u) ? exp2_fast(z * kLog2e) : 0.f;      // from here on
+                s1 += v[u];
+            }
         }
-        if (gl == 0) {
-            if (entries) {
-                sums.soft += (double)(t * t * soft);
-                sums.soft_rows += 1;
+        // the weight of an entry in the teacher's softmax, and its part of the distance
+        auto weigh = [&](int c, float of) {
+            if (c < 0) return 0.f;
+            const float w = exp2_fast((of - tm) * kLog2e);
+            ts += w;
+            if (w != 0.f) apart += w * ((of - tm) - (to_float(x[c]) - m) * per_t);
+            return w;
+        };
+        const float weight0 = weigh(c0, value0);
+        for (int j = L + gl; j < p.top; j += L) {
+            const int c = teacher_entry(p, row, j, &value);
+            weigh(c, value);
+        }
+        s = sum_of_lanes<L>(s);
+        ts = sum_of_lanes<L>(ts);
+        apart = sum_of_lanes<L>(apart);
+        float at_truth = 0, label = 0, per_s1 = 0;
+        if (HARD) {
+            s1 = sum_of_lanes<L>(s1);
+            per_s1 = reciprocal_fast(s1);
+            label = truth < 0 ? NAN : labelled ? 1.f : 0.f;
+            at_truth = truth < 0 ? 0.f : to_float(x[truth]) - m;
+        }
+        const float per_ts = reciprocal_fast(ts), soft_weight = some ? p.soft * t * (isnan(ts) ? NAN : 1.f) : 0.f, hard_weight = label != 0.f ? p.hard * label : 0.f;
+        // What the gradient loses at the classes of entries, and of the label.  A lane puts its entry's share at its class, where its number says
+        // first whether another lane has the same class: then each adds up the shares of all of them.
+        auto share = [&](int c, float w) {
+            float q = soft_weight * (w * per_ts);
+            const float before = c >= 0 ? target[c] : 0.f;
+            __syncwarp();
+            if (c >= 0) target[c] = __int_as_float(lane);
+            __syncwarp();
+            if (__any_sync(0xffffffffu, c >= 0 && __float_as_int(target[c]) != lane)) {
+                float sum = 0;
+#pragma unroll 1
+                for (int from = 0; from < L; ++from) {
+                    const int other_c = __shfl_sync(0xffffffffu, c, from, L);
+                    const float other_q = __shfl_sync(0xffffffffu, q, from, L);
+                    if (other_c == c) sum += other_q;
+                }
+                q = sum;
+            }
+            __syncwarp();
+            if (c >= 0) target[c] = before + q;
+            __syncwarp();
+        };
+        share(c0, weight0);
+        for (int j0 = L; j0 < p.top; j0 += L) {
+            const int c = j0 + gl < p.top ? teacher_entry(p, row, j0 + gl, &value) : -1;
+            share(c, c >= 0 ? exp2_fast((value - tm) * kLog2e) : 0.f);
+        }
+        if (HARD && gl == 0 && truth >= 0) target[truth] += hard_weight;
+        __syncwarp();      // and from here on the gradient may lie on the logits
+        T *g = p.grad + row * p.ldg;
+        const float of_e = some ? soft_weight * reciprocal_fast(s) : 0.f, of_v = hard_weight * per_s1;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            float d = fmaf(e[u], of_e, -target[gl + u * L]);
+            if (HARD) d = fmaf(v[u], of_v, d);
+            if (inside(u) && live) g[gl + u * L] = from_float<T>(d);
+        }
+        __syncwarp();
+        if (c0 >= 0) target[c0] = 0;
+        for (int j = L + gl; j < p.top; j += L) {
+            const int c = teacher_entry(p, row, j, &value);
+            if (c >= 0) target[c] = 0;
+        }
+        if (HARD && gl == 0 && truth >= 0) target[truth] = 0;
+        __syncwarp();
+        if (live) {      // the same in every lane of the row
+            if (some) {
+                soft_sum.add(t * t * (apart * per_ts - log_fast(ts) + log_fast(s)));
+                soft_rows += 1;
             }
             if (HARD && label != 0.f) {
-                sums.hard += (double)((logf(s1) - at_truth) * label);
-                sums.hard_rows += label;
+                hard_sum.add((log_fast(s1) - at_truth) * label);
+                hard_rows += label;
             }
         }
     }
+    LossSums sums = {0, 0, 0, 0};
+    if (gl == 0) sums = {(double)soft_sum.sum, (double)soft_rows, (double)hard_sum.sum, (double)hard_rows};
     write_sums<256>(sums, p.sums);
 }
 
-// Maximum or sums of a block, the same in every thread.
-constexpr int kBlock = 512;
-__device__ __forceinline__ float block_max(float v, float *of_warp) {
-    v = max_of_lanes<32>(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return max_of_lanes<32>(of_warp[threadIdx.x & (kBlock / 32 - 1)]);
-}
-__device__ __forceinline__ float block_sum(float v, float *of_warp) {
-    v = sum_of_lanes<32>(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return sum_of_lanes<kBlock / 32>(of_warp[threadIdx.x & (kBlock / 32 - 1)]);
-}
-
-// Rows of any number of classes, a block a row.
-template <typename T, bool HARD>
-__global__ void __launch_bounds__(kBlock) distillation_block_kernel(Distillation<T> p) {
-    __shared__ float of_warp[kBlock / 32], entry_q[kMaxTop];
+// Rows of any number of classes, a block a row: one pass for maximum and sums (every thread its own maximum, so that the sums are scaled when
+// it grows), one for the gradient that finds the row in L2.  16 bytes at a time behind the first values up to a multiple of 16, where logits
+// and gradient lie alike; VEC = false: single values.
+// 8,192 rows of 32,000 bfloat16 classes, 64 entries: 1.05 GB in 246 us (66 % of the copy rate; two exponentials a value); in three passes of single values
+// 845 us, with blocks of 512 threads 316.
+template <typename T, int THREADS, bool HARD, bool VEC>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_kernel(Distillation<T> p) {
+    constexpr int V = VEC ? kVector<T> : 1, WARPS = THREADS / 32, AT_ONCE = VEC ? 4 : 8;      // vectors in flight a thread
+    using Vector = Values<T, V>;
+    __shared__ float2 max_of_warp[WARPS];
+    __shared__ float4 sums_of_warp[WARPS];
+    __shared__ float entry_weight[kMaxTop];
     __shared__ int entry_class[kMaxTop];
-    static_assert(kMaxTop <= kBlock, "an entry a thread");
+    static_assert(kMaxTop <= THREADS, "an entry a thread");
     const int tid = threadIdx.x, classes = p.classes;
-    const float t = p.temperature;
+    const float t = p.temperature, scale = kLog2e / t;
     LossSums sums = {0, 0, 0, 0};
     for (long long row = blockIdx.x; row < p.n; row += gridDim.x) {
         const T *x = p.logits + row * p.ld;
         T *g = p.grad + row * p.ldg;
-        float m = -INFINITY;
-        for (int c = tid; c < classes; c += kBlock) m = fmaxf(m, to_float(x[c]));
-        m = block_max(m, of_warp);
-        float s = 0, s1 = 0;
-        for (int c = tid; c < classes; c += kBlock) {
-            const float z = to_float(x[c]) - m;
-            s += expf(z / t);
-            if (HARD) s1 += expf(z);
-        }
-        s = block_sum(s, of_warp);
-        if (HARD) s1 = block_sum(s1, of_warp);
-        float value = -INFINITY, q = 0, soft = 0, z_c = 0;
+        float value = -INFINITY;
         const int c_mine = tid < p.top ? teacher_entry(p, row, tid, &value) : -1;
-        const float tm = block_max(c_mine >= 0 ? value : -INFINITY, of_warp);
-        const float e = c_mine >= 0 ? expf(value - tm) : 0.f, ts = block_sum(e, of_warp);
-        const bool any = __syncthreads_or(c_mine >= 0);
-        if (c_mine >= 0) {
-            q = e / ts;
-            z_c = to_float(x[c_mine]) - m;
-            if (q != 0.f) soft = q * ((value - tm - logf(ts)) - (z_c / t - logf(s)));
-        }
-        soft = block_sum(soft, of_warp);
-        if (tid < p.top) {
-            entry_class[tid] = c_mine;
-            entry_q[tid] = q;
-        }
-        float label = 0, at_truth = 0;
-        long long truth = -1;
-        if (HARD) {
-            truth = __ldg(p.truth + row);
-            label = truth < 0 || truth >= classes ? NAN : __ldg(p.labelled + row) ? 1.f : 0.f;
-            at_truth = truth < 0 || truth >= classes ? 0.f : to_float(x[truth]) - m;
-        }
-        const float soft_weight = p.soft * t * (isnan(ts) ? NAN : 1.f);
-        // the gradient of a class whose logit is m + z and whose share of the teacher is q
-        auto gradient = [&](float z, float q_c, bool is_truth) {
-            float d = any ? soft_weight * (expf(z / t) / s - q_c) : 0.f;
-            if (HARD && label != 0.f) d += p.hard * label * (expf(z) / s1 - (is_truth ? 1.f : 0.f));
-            return from_float<T>(d);
-        };
-        // the entries of a class that is there more than once are added by the first; before the gradient, which may lie on the logits
-        __syncthreads();
-        bool first = c_mine >= 0;
-        float q_class = 0;
-        if (first)
-            for (int j = 0; j < p.top; ++j)
-                if (entry_class[j] == c_mine) {
-                    if (j < tid) first = false;
-                    q_class += entry_q[j];
+        if (tid < p.top) entry_class[tid] = c_mine;
+        const int head = VEC ? min(classes, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T))) : 0, vectors = (classes - head) / V,
+                  tail = head + vectors * V;
+        float m = -INFINITY, s = 0, s1 = 0;
+        // adds values of which `to` is the largest
+        auto add = [&](const float *z, int count, float to) {
+            if (to > m) {
+                if (m != -INFINITY) {
+                    s *= exp2_fast((m - to) * scale);
+                    if (HARD) s1 *= exp2_fast((m - to) * kLog2e);
                 }
-        for (int c = tid; c < classes; c += kBlock) g[c] = gradient(to_float(x[c]) - m, 0.f, c == truth);
+                m = to;
+            }
+            if (fabsf(m) < kLargeLogit) {
+                const float shift = m * scale, shift1 = m * kLog2e;
+#pragma unroll
+                for (int k = 0; k < count; ++k) {
+                    s += exp2_fast(fmaf(z[k], scale, -shift));
+                    if (HARD) s1 += exp2_fast(fmaf(z[k], kLog2e, -shift1));
+                }
+            } else {      // minus infinity adds 0, also where the thread has seen nothing else
+#pragma unroll
+                for (int k = 0; k < count; ++k) {
+                    const float d = m == -INFINITY && z[k] == -INFINITY ? -INFINITY : z[k] - m;
+                    s += exp2_fast(d * scale);
+                    if (HARD) s1 += exp2_fast(d * kLog2e);
+                }
+            }
+        };
+        int i = tid;
+        for (; i + (AT_ONCE - 1) * THREADS < vectors; i += THREADS * AT_ONCE) {
+            Vector w[AT_ONCE];
+            float z[AT_ONCE * V], most = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < AT_ONCE; ++b) w[b] = *reinterpret_cast<const Vector *>(x + head + (long long)(i + b * THREADS) * V);
+#pragma unroll
+            for (int b = 0; b < AT_ONCE; ++b) w[b].get(z + b * V);
+#pragma unroll
+            for (int k = 0; k < AT_ONCE * V; ++k) most = fmaxf(most, z[k]);
+            add(z, AT_ONCE * V, most);
+        }
+        for (; i < vectors; i += THREADS) {
+            const Vector w = *reinterpret_cast<const Vector *>(x + head + (long long)i * V);
+            float z[V], most = -INFINITY;
+            w.get(z);
+#pragma unroll
+            for (int k = 0; k < V; ++k) most = fmaxf(most, z[k]);
+            add(z, V, most);
+        }
+        if (VEC) {      // fewer than 16 bytes at either end
+            const int c = tid < head ? tid : tail + tid - head;
+            if (tid < head || (tid >= head && c < classes)) {
+                const float z = to_float(x[c]);
+                add(&z, 1, isnan(z) ? -INFINITY : z);
+            }
+        }
+        const float2 most = make_float2(max_of_lanes<32>(m), max_of_lanes<32>(c_mine >= 0 ? value : -INFINITY));
+        if ((tid & 31) == 0) max_of_warp[tid >> 5] = most;
+        const bool any = __syncthreads_or(c_mine >= 0);
+        float2 of_warp = max_of_warp[(tid & 31) % WARPS];
+        const float row_max = max_of_lanes<32>(of_warp.x), tm = max_of_lanes<32>(of_warp.y);
+        // sums of the row (those of a thread that has seen nothing but minus infinity are 0), and the teacher's
+        float weight = 0, z_mine = 0;
+        float4 sum = make_float4(m == -INFINITY ? s : s * exp2_fast((m - row_max) * scale), m == -INFINITY ? s1 : s1 * exp2_fast((m - row_max) * kLog2e), 0, 0);
+        bool first = c_mine >= 0, again = false;
+        if (c_mine >= 0) {
+            weight = expf(value - tm);
+            z_mine = to_float(x[c_mine]);
+            sum.z = weight;
+            if (weight != 0.f) sum.w = weight * ((value - tm) - (z_mine - row_max) / t);
+            entry_weight[tid] = weight;
+#pragma unroll 4
+            for (int j = 0; j < p.top; ++j) {
+                const bool same = j != tid && entry_class[j] == c_mine;
+                again = again || same;
+                first = first && !(same && j < tid);
+            }
+        }
+        sum.x = sum_of_lanes<32>(sum.x);
+        if (HARD) sum.y = sum_of_lanes<32>(sum.y);
+        sum.z = sum_of_lanes<32>(sum.z);
+        sum.w = sum_of_lanes<32>(sum.w);
+        if ((tid & 31) == 0) sums_of_warp[tid >> 5] = sum;
+        float label = 0, at_truth = 0;
+        int truth = -1;
+        if (HARD) {
+            const long long wanted = __ldg(p.truth + row);
+            const bool exists = wanted >= 0 && wanted < classes;
+            label = !exists ? NAN : __ldg(p.labelled + row) ? 1.f : 0.f;
+            truth = exists ? (int)wanted : -1;
+            at_truth = exists ? to_float(x[truth]) : 0.f;
+        }
+        __syncthreads();      // and from here on the gradient may lie on the logits
+        sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float4 o = sums_of_warp[w];
+            sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
+        }
+        const float per_ts = 1.f / sum.z, soft_weight = any ? p.soft * t * (isnan(sum.z) ? NAN : 1.f) : 0.f, per_s = soft_weight / sum.x;
+        const float hard_weight = label != 0.f ? p.hard * label : 0.f, per_s1 = hard_weight / sum.y;
+        const bool ordinary = fabsf(row_max) < kLargeLogit;
+        const float shift = row_max * scale, shift1 = row_max * kLog2e;
+        // the gradient of a class whose logit is z, without the teacher's share and the label
+        auto gradient = [&](float z, bool fast) {
+            float d = exp2_fast(fast ? fmaf(z, scale, -shift) : (z - row_max) * scale) * per_s;
+            if (HARD) d = fmaf(exp2_fast(fast ? fmaf(z, kLog2e, -shift1) : (z - row_max) * kLog2e), per_s1, d);
+            return d;
+        };
+        auto write = [&](auto fast) {
+            constexpr bool FAST = decltype(fast)::value;
+            int i = tid;
+            for (; i + (AT_ONCE - 1) * THREADS < vectors; i += THREADS * AT_ONCE) {
+                Vector w[AT_ONCE];
+#pragma unroll
+                for (int b = 0; b < AT_ONCE; ++b) w[b] = *reinterpret_cast<const Vector *>(x + head + (long long)(i + b * THREADS) * V);
+#pragma unroll
+                for (int b = 0; b < AT_ONCE; ++b) {
+                    float z[V];
+                    w[b].get(z);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) z[k] = gradient(z[k], FAST);
+                    w[b].set(z);
+                    *reinterpret_cast<Vector *>(g + head + (long long)(i + b * THREADS) * V) = w[b];
+                }
+            }
+            for (; i < vectors; i += THREADS) {
+                Vector w = *reinterpret_cast<const Vector *>(x + head + (long long)i * V);
+                float z[V];
+                w.get(z);
+#pragma unroll
+                for (int k = 0; k < V; ++k) z[k] = gradient(z[k], FAST);
+                w.set(z);
+                *reinterpret_cast<Vector *>(g + head + (long long)i * V) = w;
+            }
+            if (VEC) {
+                const int c = tid < head ? tid : tail + tid - head;
+                if (tid < head || (tid >= head && c < classes)) g[c] = from_float<T>(gradient(to_float(x[c]), FAST));
+            }
+        };
+        if (!any && label == 0.f) {
+            for (int c = tid; c < classes; c += THREADS) g[c] = from_float<T>(0.f);
+        } else if (ordinary) {
+            write(std::true_type());
+        } else {
+            write(std::false_type());
+        }
         __syncthreads();
-        if (first) g[c_mine] = gradient(z_c, q_class, c_mine == truth);
+        if (first) {      // the first entry of a class has the share of all of them
+            float all = weight;
+            if (again)
+                for (int j = tid + 1; j < p.top; ++j)
+                    if (entry_class[j] == c_mine) all += entry_weight[j];
+            float d = gradient(z_mine, ordinary) - soft_weight * (all * per_ts);
+            if (HARD && c_mine == truth) d -= hard_weight;
+            g[c_mine] = from_float<T>(d);
+        }
+        if (HARD) {      // a labelled class that is no entry
+            bool entry = false;
+            if (tid < p.top) entry = c_mine == truth;
+            entry = __syncthreads_or(entry);
+            if (!entry && tid == 0 && truth >= 0 && label != 0.f) g[truth] = from_float<T>(gradient(at_truth, ordinary) - hard_weight);
+        }
         if (tid == 0) {
             if (any) {
-                sums.soft += (double)(t * t * soft);
+                sums.soft += (double)(t * t * (sum.w * per_ts - logf(sum.z) + logf(sum.x)));
                 sums.soft_rows += 1;
             }
             if (HARD && label != 0.f) {
-                sums.hard += (double)((logf(s1) - at_truth) * label);
+                sums.hard += (double)((logf(sum.y) - (at_truth - row_max)) * label);
                 sums.hard_rows += label;
             }
         }
+        __syncthreads();      // the entries have been read
     }
-    write_sums<kBlock>(sums, p.sums);
+    write_sums<THREADS>(sums, p.sums);
 }
 
 // loss[0], loss[1] = the means of the soft and of the hard losses over the rows that have one (0 where there are none)
@@ -306,12 +498,17 @@ static int launch_distillation(const Distillation<T> &p, float *loss, cudaStream
     const int lanes = p.classes <= 64 ? 8 : p.classes <= 256 ? 32 : 0, rows = lanes ? 256 / lanes : 1;
     const int blocks = (int)std::min<long long>(kRowBlocks, ((long long)p.n + rows - 1) / rows);
     if (p.n > 0) {
-        if (p.classes <= 8) distillation_rows_kernel<T, 8, 1, HARD><<<blocks, 256, 0, st>>>(p);
-        else if (p.classes <= 16) distillation_rows_kernel<T, 8, 2, HARD><<<blocks, 256, 0, st>>>(p);
-        else if (p.classes <= 32) distillation_rows_kernel<T, 8, 4, HARD><<<blocks, 256, 0, st>>>(p);
-        else if (p.classes <= 64) distillation_rows_kernel<T, 8, 8, HARD><<<blocks, 256, 0, st>>>(p);
-        else if (p.classes <= 256) distillation_rows_kernel<T, 32, 8, HARD><<<blocks, 256, 0, st>>>(p);
-        else distillation_block_kernel<T, HARD><<<blocks, kBlock, 0, st>>>(p);
+        const bool alike = ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad)) & 15) == 0 && (p.ld - p.ldg) * (long long)sizeof(T) % 16 == 0;
+        const int per = lanes ? (p.classes + lanes - 1) / lanes : 0;
+        switch (lanes + per) {
+#define DRONE_ROWS(L, PER) case L + PER: distillation_rows_kernel<T, L, PER, HARD><<<blocks, 256, 0, st>>>(p); break
+            DRONE_ROWS(8, 1); DRONE_ROWS(8, 2); DRONE_ROWS(8, 3); DRONE_ROWS(8, 4); DRONE_ROWS(8, 5); DRONE_ROWS(8, 6); DRONE_ROWS(8, 7); DRONE_ROWS(8, 8);
+            DRONE_ROWS(32, 3); DRONE_ROWS(32, 4); DRONE_ROWS(32, 5); DRONE_ROWS(32, 6); DRONE_ROWS(32, 7); DRONE_ROWS(32, 8);
+#undef DRONE_ROWS
+            default:
+                alike ? distillation_block_kernel<T, 256, HARD, true><<<blocks, 256, 0, st>>>(p)
+                      : distillation_block_kernel<T, 256, HARD, false><<<blocks, 256, 0, st>>>(p);
+        }
         DRONE_LAUNCH_CHECK("distillation_kernel");
     }
     fold_distillation_kernel<<<1, 256, 0, st>>>(p.sums, p.n > 0 ? blocks : 0, loss);
@@ -332,7 +529,7 @@ int drone_distillation_loss(int type, int n_rows, int classes, const void *d_log
     DRONE_REQUIRE(n_rows >= 0 && classes >= 1 && ld >= classes && ld_grad >= classes, "drone_distillation_loss: n_rows=%d classes=%d ld=%d ld_grad=%d",
                   n_rows, classes, ld, ld_grad);
     DRONE_REQUIRE(top >= 1 && top <= kMaxTop && ldt >= top && ldc >= top, "drone_distillation_loss: top=%d (1..%d) ldt=%d ldc=%d", top, kMaxTop, ldt, ldc);
-    DRONE_REQUIRE(temperature > 0 && temperature <= 1e30f, "drone_distillation_loss: temperature=%g", temperature);
+    DRONE_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, "drone_distillation_loss: temperature=%g", temperature);
     DRONE_REQUIRE(d_loss && d_scratch && (n_rows == 0 || (d_logits && d_teacher && d_classes && d_grad)), "drone_distillation_loss: NULL argument");
     DRONE_REQUIRE((d_truth == nullptr) == (d_labelled == nullptr), "drone_distillation_loss: d_truth and d_labelled come together");
     DRONE_REQUIRE(DRONE_ALIGNED(d_logits, type) && DRONE_ALIGNED(d_grad, type) && DRONE_ALIGNED(d_teacher, teacher_type),
@@ -341,7 +538,7 @@ int drone_distillation_loss(int type, int n_rows, int classes, const void *d_log
     cudaStream_t st = (cudaStream_t)stream;
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
-        const Distillation<T> p = {(const T *)d_logits, ld, d_teacher, ldt, teacher_type, d_classes, ldc, top, d_truth, d_labelled, temperature, soft,
+        const Distillation<T> p = {(const T *)d_logits, ld, d_teacher, ldt, teacher_type, d_classes, ldc, top, d_truth, d_labelled, temperature, 1 / temperature, soft,
                                    hard, (T *)d_grad, ld_grad, (LossSums *)d_scratch, n_rows, classes};
         return d_truth ? launch_distillation<T, true>(p, d_loss, st) : launch_distillation<T, false>(p, d_loss, st);
     });

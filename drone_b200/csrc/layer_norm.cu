@@ -17,17 +17,16 @@ namespace drone {
 // values a lane, L apart.
 template <typename T, int L, int U, bool VEC>
 struct RowShape {
-    static constexpr int V = Vec<T>::N, PER = U * V, THREADS = L > 256 ? L : 256, GROUPS = THREADS / L;
+    static constexpr int V = kVector<T>, PER = U * V, THREADS = L > 256 ? L : 256, GROUPS = THREADS / L;
     __device__ static int column(int gl, int i) { return VEC ? (gl + i / V * L) * V + i % V : gl + i * L; }
     // values beyond the row are 0
     __device__ static void load(const T *row, int F, int gl, float (&v)[PER]) {
         if (VEC) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                Vec<T> x = {};
-                if (column(gl, u * V) < F) x = *reinterpret_cast<const Vec<T> *>(row + column(gl, u * V));
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[u * V + e] = to_float(x.v[e]);
+                Values<T, V> x = {};
+                if (column(gl, u * V) < F) x = *reinterpret_cast<const Values<T, V> *>(row + column(gl, u * V));
+                x.get(v + u * V);
             }
         } else {
 #pragma unroll
@@ -38,10 +37,9 @@ struct RowShape {
         if (VEC) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                Vec<T> x;
-#pragma unroll
-                for (int e = 0; e < V; ++e) x.v[e] = from_float<T>(v[u * V + e]);
-                if (column(gl, u * V) < F) *reinterpret_cast<Vec<T> *>(row + column(gl, u * V)) = x;
+                Values<T, V> x;
+                x.set(v + u * V);
+                if (column(gl, u * V) < F) *reinterpret_cast<Values<T, V> *>(row + column(gl, u * V)) = x;
             }
         } else {
 #pragma unroll
@@ -326,7 +324,7 @@ int drone_layer_norm(int type, int n_rows, int F, const void *d_X, int ldx, cons
     const int blocks = norm_grid(type, n_rows, F, sms, 8).blocks;
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
-        constexpr int V = Vec<T>::N;
+        constexpr int V = kVector<T>;
         const bool vec = F % V == 0 && rows_on_16_bytes(d_X, ldx, sizeof(T)) && rows_on_16_bytes(d_Y, ldy, sizeof(T));
         return with_norm_shape(ceil_div(F, V), [&](auto shape) {
             constexpr int L = decltype(shape)::L, U = decltype(shape)::U;
@@ -370,7 +368,7 @@ int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int 
     if (n_rows > 0) {
         rc = with_type(type, [&](auto tag) {
             using T = typename decltype(tag)::T;
-            constexpr int V = Vec<T>::N;
+            constexpr int V = kVector<T>;
             const bool vec = F % V == 0 && rows_on_16_bytes(d_G, ldg, sizeof(T)) && rows_on_16_bytes(d_X, ldx, sizeof(T)) &&
                              rows_on_16_bytes(d_dX, ld, sizeof(T)) && (!d_out || rows_on_16_bytes(d_out, ldo, sizeof(T)));
             const NormBackward<T> p = {(const T *)d_G, (const T *)d_X, (const T *)d_out, ldg, ldx, ldo, d_scale, d_mean, d_rstd, d_mirror2worker,

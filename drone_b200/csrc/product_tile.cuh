@@ -361,17 +361,20 @@ product_tile_kernel(Operand<T> A, Operand<T> B, int M, int N, int K, int share, 
             b[0] = x.x, b[1] = x.y, b[2] = x.z, b[3] = x.w;
         }
         for (int r = threadIdx.x / LANES; r < rows; r += AT_ONCE) {
-            struct alignas(4 * sizeof(T)) Four { T v[4]; } x, y, z;
+            using Four = Values<T, 4>;
+            Four x = {}, y, z;
+            float before[4], after[4], added[4];
             const long long row = m0 + r;
             if (out.residual) x = *reinterpret_cast<const Four *>(out.residual + row * out.ldr + n0 + c);
+            x.get(added);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float acc = value(r, c + i) + b[i];
-                z.v[i] = from_float<T>(acc);
-                float v = activate(acc, out.activation);
-                if (out.residual) v += to_float(x.v[i]);
-                y.v[i] = from_float<T>(v);
+                before[i] = value(r, c + i) + b[i];
+                after[i] = activate(before[i], out.activation);
+                if (out.residual) after[i] += added[i];
             }
+            z.set(before);
+            y.set(after);
             if (out.pre) *reinterpret_cast<Four *>(out.pre + row * out.ldp + n0 + c) = z;
             *reinterpret_cast<Four *>(out.y + row * out.ldy + n0 + c) = y;
         }

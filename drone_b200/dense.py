@@ -219,7 +219,7 @@ def distillation_loss(logits, teacher, classes, temperature=1.0, truth=None, lab
     top = teacher.shape[1]
     _require(top <= DISTILLATION_MAX_TOP, "%d entries of the teacher: at most %d", top, DISTILLATION_MAX_TOP)
     ldc = _matrix("classes", classes, n, top, torch.int64, device)
-    _require(temperature > 0 and temperature <= 1e30, "temperature=%r", temperature)
+    _require(1e-6 <= temperature <= 1e6, "temperature=%r", temperature)
     _require((truth is None) == (labelled is None), "truth and labelled come together")
     if truth is not None:
         _vector("truth", truth, n, torch.int64, device)

@@ -414,7 +414,7 @@ int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int 
                               void *stream);
 
 /* Loss and gradient of [n_rows, classes] logits against a teacher's `top` best logits of each row: values d_teacher [n_rows, top] (of
- * teacher_type) of the classes d_classes [n_rows, top].  With the temperature t, q = softmax(teacher / t) over the row's entries and
+ * teacher_type) of the classes d_classes [n_rows, top].  With the temperature t (1e-6 to 1e6), q = softmax(teacher / t) over the row's entries and
  * p = softmax(logits / t):
  *   d_loss[0] = mean over the rows with an entry of t^2 * sum q (log q - log p)
  *   d_loss[1] = mean over the rows with d_labelled[r] != 0 of the cross-entropy at t = 1 (0 without d_truth, d_labelled)

@@ -389,3 +389,16 @@ def test_distillation_gradient_against_differences(cuda_device):
         want = (value(logits + h * d) - value(logits - h * d)) / (2 * h)
         # a loss of size n * 10, good to 32 steps, over h, and h^2
         assert abs((grad.double() * d.double()).sum().item() - want) <= 32 * STEP * n * 10 / h + h * h
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distillation_of_masked_logits(cuda_device, dtype):
+    """Logits and entries of the type's lowest value: no share beside others, equal shares where there is nothing else."""
+    gen = torch.Generator(cuda_device).manual_seed(11)
+    low = torch.finfo(dtype).min
+    for c in (7, 47, 100, 500, 9000):
+        logits, teacher = rows_of(gen, 6, c, dtype), rows_of(gen, 6, 4, dtype)
+        classes = torch.arange(4, device="cuda").expand(6, 4).contiguous()
+        logits[1, 5:], logits[2], teacher[3, 1:], teacher[4] = low, low, low, low
+        check_distillation(logits, teacher, classes, 1.0)
+        check_distillation(logits, teacher, classes, 4.0)
