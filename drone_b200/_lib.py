@@ -105,7 +105,7 @@ def _declare(lib):
         "drone_weight_gradient_scratch": (i, [i, i, i, C.POINTER(ll)]),
         "drone_weight_gradient": (i, [i, i, i, vp, i, vp, i, vp, vp, ll, vp]),
         "drone_linear": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, i, vp, i, vp, i, vp]),
-        "drone_activation_gradient_scratch": (i, [i, i, C.POINTER(ll)]),
+        "drone_activation_gradient_scratch": (i, [i, i, i, C.POINTER(ll)]),
         "drone_activation_gradient": (i, [i, i, i, vp, i, vp, i, i, vp, i, vp, vp, ll, vp]),
         "drone_linear_weight_gradient_scratch": (i, [i, i, i, i, i, C.POINTER(ll)]),
         "drone_linear_weight_gradient": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, ll, vp]),

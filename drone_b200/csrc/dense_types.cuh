@@ -49,24 +49,66 @@ struct alignas(N * sizeof(T)) Values {
 
 template <typename T> constexpr int kVector = 16 / sizeof(T);      // values in 16 bytes
 
-// z -> activation(z) and its derivative.  A NaN stays one, also in the ReLU (max(NaN, 0) would be 0).
-__device__ __forceinline__ float activate(float z, int activation) {
+// f(std::integral_constant) of an activation
+template <typename F>
+__host__ __device__ __forceinline__ void with_activation(int activation, const F &f) {
     switch (activation) {
-        case DRONE_ACT_RELU: return z < 0.f ? 0.f : z;
-        case DRONE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
-        case DRONE_ACT_SILU: return z / (1.f + expf(-z));
-        default: return z;
+        case DRONE_ACT_RELU: f(std::integral_constant<int, DRONE_ACT_RELU>()); break;
+        case DRONE_ACT_GELU: f(std::integral_constant<int, DRONE_ACT_GELU>()); break;
+        case DRONE_ACT_SILU: f(std::integral_constant<int, DRONE_ACT_SILU>()); break;
+        default: f(std::integral_constant<int, DRONE_ACT_NONE>());
     }
 }
-__device__ __forceinline__ float activation_slope(float z, int activation) {
-    switch (activation) {
-        case DRONE_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case DRONE_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
-        case DRONE_ACT_SILU: {
-            const float p = 1.f / (1.f + expf(-z));
-            return p * (1.f + z * (1.f - p));
-        }
-        default: return 1.f;
+
+__device__ __forceinline__ float exp2_fast(float x) {      // off by 2^-22 of the value
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {      // one unit in the last place
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Phi(z), the normal distribution's, and exp(-z^2 / 2), for results of 16 bits: Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7 of 1 against
+// the 2^-11 or 2^-8 of a value that the rounding leaves; a dozen instructions where erff and expf take fifty.
+__device__ __forceinline__ float normal_fast(float z, float *bell) {
+    const float x = fabsf(z) * 0.70710678f, t = reciprocal_fast(fmaf(0.3275911f, x, 1.f));
+    *bell = exp2_fast(x * x * -1.44269504f);
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * poly * *bell;      // Phi(-|z|)
+    return z < 0.f ? tail : 1.f - tail;
+}
+
+// z -> activation(z) and its derivative, for values of type T.  A NaN stays one, also in the ReLU (max(NaN, 0) would be 0).
+template <typename T, int ACTIVATION>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACTIVATION == DRONE_ACT_RELU) {
+        return z < 0.f ? 0.f : z;
+    } else if constexpr (ACTIVATION == DRONE_ACT_GELU) {
+        float bell;
+        return sizeof(T) == 4 ? 0.5f * z * (1.f + erff(z * 0.70710678f)) : z * normal_fast(z, &bell);
+    } else if constexpr (ACTIVATION == DRONE_ACT_SILU) {
+        return sizeof(T) == 4 ? z / (1.f + expf(-z)) : z * reciprocal_fast(1.f + exp2_fast(z * -1.44269504f));
+    } else {
+        return z;
+    }
+}
+template <typename T, int ACTIVATION>
+__device__ __forceinline__ float activation_slope(float z) {
+    if constexpr (ACTIVATION == DRONE_ACT_RELU) {
+        return z > 0.f ? 1.f : 0.f;
+    } else if constexpr (ACTIVATION == DRONE_ACT_GELU) {
+        if (sizeof(T) == 4) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+        float bell;
+        const float phi = normal_fast(z, &bell);
+        return fmaf(z * 0.39894228f, bell, phi);
+    } else if constexpr (ACTIVATION == DRONE_ACT_SILU) {
+        const float p = sizeof(T) == 4 ? 1.f / (1.f + expf(-z)) : reciprocal_fast(1.f + exp2_fast(z * -1.44269504f));
+        return p * (1.f + z * (1.f - p));
+    } else {
+        return 1.f;
     }
 }
 

@@ -89,23 +89,13 @@ __device__ __forceinline__ void write_sums(LossSums s, LossSums *sums) {
     }
 }
 
-// 2^x, of x = (z - the row's maximum) log2(e) / t: three instructions an exponential, one of them of the special function unit.  Off by 2^-22 of
-// the value, as the rounding of x is.  (The difference comes first: a row whose logits are all the type's lowest value is a row of equal ones.)
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
+// Exponentials are exp2_fast of (z - the row's maximum) log2(e) / t, whose rounding is off by as much.  (The difference comes first: a row whose
+// logits are all the type's lowest value is a row of equal ones.)
 constexpr float kLog2e = 1.44269504f;
 __device__ __forceinline__ float log_fast(float x) {      // off by 2^-22 and 2^-22 of the value
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y * 0.693147181f;
-}
-__device__ __forceinline__ float reciprocal_fast(float x) {      // one unit in the last place
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // Below this a logit times log2(e) / t is finite for every t that is allowed, and one multiply-add forms the exponent.
 constexpr float kLargeLogit = 1e30f;

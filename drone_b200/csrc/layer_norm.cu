@@ -7,51 +7,11 @@
 // where rows allow it), so that mean, variance and the two means of the backward pass cost shuffles and no second read; the
 // variance is that of the differences from the mean, in 32 bits.  The sums over rows stay in a thread's registers for all rows it
 // takes, are added within the block in shared memory and over the blocks in double, always in the same order.
-#include "dense_types.cuh"
+#include "row_shape.cuh"
 
 #include <algorithm>
 
 namespace drone {
-
-// How a row lies in the registers of its lanes: U vectors of V values a lane, or (rows that are not on 16 bytes) U * V single
-// values a lane, L apart.
-template <typename T, int L, int U, bool VEC>
-struct RowShape {
-    static constexpr int V = kVector<T>, PER = U * V, THREADS = L > 256 ? L : 256, GROUPS = THREADS / L;
-    __device__ static int column(int gl, int i) { return VEC ? (gl + i / V * L) * V + i % V : gl + i * L; }
-    // values beyond the row are 0
-    __device__ static void load(const T *row, int F, int gl, float (&v)[PER]) {
-        if (VEC) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                Values<T, V> x = {};
-                if (column(gl, u * V) < F) x = *reinterpret_cast<const Values<T, V> *>(row + column(gl, u * V));
-                x.get(v + u * V);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) v[i] = column(gl, i) < F ? to_float(row[column(gl, i)]) : 0.f;
-        }
-    }
-    __device__ static void store(T *row, int F, int gl, const float (&v)[PER]) {
-        if (VEC) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                Values<T, V> x;
-                x.set(v + u * V);
-                if (column(gl, u * V) < F) *reinterpret_cast<Values<T, V> *>(row + column(gl, u * V)) = x;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (column(gl, i) < F) row[column(gl, i)] = from_float<T>(v[i]);
-        }
-    }
-    __device__ static void load_vector(const float *p, int F, int gl, float (&v)[PER]) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = column(gl, i) < F ? __ldg(p + column(gl, i)) : 0.f;
-    }
-};
 
 // Sum of one value per lane over the L lanes of a row (L <= 32: within the warp; above: the block is the row).
 template <int L>
@@ -202,30 +162,8 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) layer_norm_backward_kernel(
         S::store(p.dx + row * p.ld, F, gl, g);
     }
     float *of_block = p.sums + (long long)blockIdx.x * 2 * F;
-    if (S::GROUPS == 1) {
-#pragma unroll
-        for (int i = 0; i < S::PER; ++i)
-            if (S::column(gl, i) < F) {
-                of_block[S::column(gl, i)] = d_scale[i];
-                of_block[F + S::column(gl, i)] = d_shift[i];
-            }
-        return;
-    }
-    __shared__ float of_group[S::GROUPS > 1 ? S::THREADS * S::PER : 1];
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < S::PER; ++i) of_group[(threadIdx.x / L * S::PER + i) * L + gl] = which ? d_shift[i] : d_scale[i];
-        __syncthreads();
-        for (int at = threadIdx.x; at < L * S::PER; at += S::THREADS) {
-            const int c = S::column(at % L, at / L);
-            if (c >= F) continue;
-            float sum = 0;
-            for (int w = 0; w < S::GROUPS; ++w) sum += of_group[w * S::PER * L + at];
-            of_block[which * F + c] = sum;
-        }
-    }
+    S::add_groups(d_scale, F, gl, of_block);
+    S::add_groups(d_shift, F, gl, of_block + F);
 }
 
 template <typename T>
@@ -253,43 +191,6 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(
             p.dx[row * p.ld + c] = from_float<T>(r * (g * __ldg(p.scale + c) - s.x / F - h * (s.y / F)));
         }
     }
-}
-
-// d_scale, d_shift = the blocks' sums, in order.  A block has 32 of the 2F columns, its warps every eighth of the sums.
-__global__ void __launch_bounds__(256) fold_norm_sums_kernel(const float *__restrict__ sums, int blocks, int F, float *__restrict__ d_scale,
-                                                             float *__restrict__ d_shift) {
-    __shared__ double of_warp[8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
-    double sum = 0;
-    if (c < 2 * F) {
-#pragma unroll 4
-        for (int b = w; b < blocks; b += 8) sum += __ldg(sums + (long long)b * 2 * F + c);
-    }
-    of_warp[w][threadIdx.x & 31] = sum;
-    __syncthreads();
-    if (w == 0 && c < 2 * F) {
-        for (int i = 1; i < 8; ++i) sum += of_warp[i][threadIdx.x];
-        if (c < F) {
-            if (d_scale) d_scale[c] = (float)sum;
-        } else if (d_shift) {
-            d_shift[c - F] = (float)sum;
-        }
-    }
-}
-
-// f(shape) for the lanes of a row of so many vectors: shape.L lanes with shape.U vectors each; L = 0: too wide for a block's registers.
-template <int LANES, int VECTORS> struct NormShape { static constexpr int L = LANES, U = VECTORS; };
-template <typename F>
-static int with_norm_shape(int vectors, const F &f) {
-    if (vectors <= 8) return f(NormShape<8, 1>());
-    if (vectors <= 16) return f(NormShape<8, 2>());
-    if (vectors <= 32) return f(NormShape<32, 1>());
-    if (vectors <= 64) return f(NormShape<32, 2>());
-    if (vectors <= 128) return f(NormShape<32, 4>());
-    if (vectors <= 512) return f(NormShape<256, 2>());
-    if (vectors <= 1024) return f(NormShape<256, 4>());
-    if (vectors <= 2048) return f(NormShape<512, 4>());
-    return f(NormShape<0, 0>());
 }
 
 struct NormGrid {
@@ -326,7 +227,7 @@ int drone_layer_norm(int type, int n_rows, int F, const void *d_X, int ldx, cons
         using T = typename decltype(tag)::T;
         constexpr int V = kVector<T>;
         const bool vec = F % V == 0 && rows_on_16_bytes(d_X, ldx, sizeof(T)) && rows_on_16_bytes(d_Y, ldy, sizeof(T));
-        return with_norm_shape(ceil_div(F, V), [&](auto shape) {
+        return with_row_shape(ceil_div(F, V), [&](auto shape) {
             constexpr int L = decltype(shape)::L, U = decltype(shape)::U;
             auto launch = [&](auto kernel, int threads) {
                 kernel<<<blocks, threads, 0, st>>>((const T *)d_X, ldx, d_scale, d_shift, n_rows, F, eps, relu != 0, (T *)d_Y, ldy, d_mean, d_rstd);
@@ -373,7 +274,7 @@ int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int 
                              rows_on_16_bytes(d_dX, ld, sizeof(T)) && (!d_out || rows_on_16_bytes(d_out, ldo, sizeof(T)));
             const NormBackward<T> p = {(const T *)d_G, (const T *)d_X, (const T *)d_out, ldg, ldx, ldo, d_scale, d_mean, d_rstd, d_mirror2worker,
                                        (T *)d_dX, ld, d_scratch, n_rows, F};
-            return with_norm_shape(ceil_div(F, V), [&](auto shape) {
+            return with_row_shape(ceil_div(F, V), [&](auto shape) {
                 constexpr int L = decltype(shape)::L, U = decltype(shape)::U;
                 if constexpr (L == 0) layer_norm_backward_wide_kernel<T><<<blocks, kWideThreads, 0, st>>>(p);
                 else if (vec) layer_norm_backward_kernel<T, L, U, true><<<blocks, L > 256 ? L : 256, 0, st>>>(p);
@@ -385,9 +286,7 @@ int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int 
         if (rc) return rc;
     }
     if (!d_scale_grad && !d_shift_grad) return DRONE_OK;
-    fold_norm_sums_kernel<<<ceil_div(2LL * F, 32), 256, 0, st>>>(d_scratch, blocks, F, d_scale_grad, d_shift_grad);
-    DRONE_LAUNCH_CHECK("fold_norm_sums_kernel");
-    return DRONE_OK;
+    return fold_columns(d_scratch, blocks, 2 * F, d_scale_grad, F, d_shift_grad, st);
 }
 
 }  // extern "C"

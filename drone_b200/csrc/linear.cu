@@ -1,5 +1,6 @@
 // Products of a dense layer, Y = activation(X W + bias) + residual, and its backward pass.
 #include "product_tile.cuh"
+#include "row_shape.cuh"
 
 #include <algorithm>
 
@@ -17,43 +18,59 @@ __global__ void __launch_bounds__(256) add_product_shares_kernel(const float *__
     }
 }
 
-// dZ = G * activation'(pre) and the column sums of a block's rows.  A block has 32 columns and 8 rows at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) activation_gradient_kernel(const T *G, long long ldg, const T *pre, long long ldp, int activation, int n, int N,
-                                                                  int rows_per_block, T *dZ, long long ldz, float *sums) {
-    __shared__ float of_warp[8][32];
-    const int c = blockIdx.y * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
-    const long long r0 = (long long)blockIdx.x * rows_per_block, r1 = min((long long)n, r0 + rows_per_block);
-    float sum = 0;
-    if (c < N)
-        for (long long r = r0 + w; r < r1; r += 8) {
-            float d = to_float(G[r * ldg + c]);
-            if (activation != DRONE_ACT_NONE) d *= activation_slope(to_float(pre[r * ldp + c]), activation);
-            if (dZ) dZ[r * ldz + c] = from_float<T>(d);
-            sum += d;
+// dZ = G * activation'(pre) and the sums of its columns, of those from blockIdx.y * width on; sums[blockIdx.x] = those of the block's rows.
+// Bound: HBM, two reads and a write.
+template <typename T, int L, int U, bool VEC, int ACTIVATION>
+__global__ void __launch_bounds__(256)
+activation_gradient_kernel(const T *G, long long ldg, const T *pre, long long ldp, int n, int N, int width, T *dZ, long long ldz, float *sums) {
+    using S = RowShape<T, L, U, VEC>;
+    const int gl = threadIdx.x % L, c0 = blockIdx.y * width, F = min(width, N - c0);
+    float sum[S::PER];
+#pragma unroll
+    for (int i = 0; i < S::PER; ++i) sum[i] = 0;
+    for (long long row = (long long)blockIdx.x * S::GROUPS + threadIdx.x / L; row < n; row += (long long)gridDim.x * S::GROUPS) {
+        float d[S::PER];
+        S::load(G + row * ldg + c0, F, gl, d);
+        if (ACTIVATION != DRONE_ACT_NONE) {
+            float z[S::PER];
+            S::load(pre + row * ldp + c0, F, gl, z);
+#pragma unroll
+            for (int i = 0; i < S::PER; ++i) d[i] *= activation_slope<T, ACTIVATION>(z[i]);
+            if (dZ) S::store(dZ + row * ldz + c0, F, gl, d);
+        } else if (dZ) {
+            S::store(dZ + row * ldz + c0, F, gl, d);
         }
-    if (!sums) return;
-    of_warp[w][threadIdx.x & 31] = sum;
-    __syncthreads();
-    if (w == 0 && c < N) {
-        for (int i = 1; i < 8; ++i) sum += of_warp[i][threadIdx.x];
-        sums[(long long)blockIdx.x * N + c] = sum;
+#pragma unroll
+        for (int i = 0; i < S::PER; ++i) sum[i] += d[i];
     }
+    if (sums) S::add_groups(sum, F, gl, sums + (long long)blockIdx.x * N + c0);
 }
-__global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ sums, int blocks, int N, float *__restrict__ out) {
+
+// A block has 32 of the columns, its warps every eighth of the sums.
+__global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ sums, int blocks, int columns, float *a, int split, float *b) {
     __shared__ double of_warp[8][32];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
     double sum = 0;
-    if (c < N) {
+    if (c < columns) {
 #pragma unroll 4
-        for (int b = w; b < blocks; b += 8) sum += __ldg(sums + (long long)b * N + c);
+        for (int i = w; i < blocks; i += 8) sum += __ldg(sums + (long long)i * columns + c);
     }
     of_warp[w][threadIdx.x & 31] = sum;
     __syncthreads();
-    if (w == 0 && c < N) {
+    if (w == 0 && c < columns) {
         for (int i = 1; i < 8; ++i) sum += of_warp[i][threadIdx.x];
-        out[c] = (float)sum;
+        if (c < split) {
+            if (a) a[c] = (float)sum;
+        } else if (b) {
+            b[c - split] = (float)sum;
+        }
     }
+}
+
+int fold_columns(const float *sums, int blocks, int columns, float *a, int split, float *b, cudaStream_t st) {
+    fold_columns_kernel<<<ceil_div(columns, 32), 256, 0, st>>>(sums, blocks, columns, a, split, b);
+    DRONE_LAUNCH_CHECK("fold_columns_kernel");
+    return DRONE_OK;
 }
 
 // How the rows of a weight gradient, its K, are cut: two blocks an SM, but a share of four steps at least.
@@ -70,12 +87,18 @@ static Shares product_shares(int type, int M, int N, int K, int sms) {
     return s;
 }
 
-static int rows_per_gradient_block(int n, int N, int sms, int *blocks) {
-    const int columns = ceil_div(N, 32);
-    const int most = std::max(1, 8 * sms / columns);
-    const int rows = std::max(64, ceil_div(n, most));
-    *blocks = ceil_div(n, rows);
-    return rows;
+// Blocks of the activations' gradient: as many as the SMs hold, of at most 128 vectors a row.
+struct GradientBlocks {
+    int width, columns, rows;      // of a block; blocks along the columns and the rows
+};
+static GradientBlocks gradient_blocks(int type, int n, int N, int sms) {
+    const int V = 16 / type_size(type);
+    GradientBlocks b;
+    b.width = std::min(N, 128 * V);
+    b.columns = ceil_div(N, b.width);
+    const int groups = ceil_div(b.width, V) <= 16 ? 32 : 8;
+    b.rows = (int)std::min<long long>(((long long)n + groups - 1) / groups, std::max(1, 6 * sms / b.columns));
+    return b;
 }
 
 }  // namespace drone
@@ -113,13 +136,13 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
     });
 }
 
-int drone_activation_gradient_scratch(int n_rows, int N, long long *n_floats) {
-    DRONE_REQUIRE(DRONE_LINEAR_SIZES(n_rows, 1, N) && n_floats, "drone_activation_gradient_scratch: n_rows=%d N=%d", n_rows, N);
-    int sms = 0, blocks = 0;
+int drone_activation_gradient_scratch(int type, int n_rows, int N, long long *n_floats) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, 1, N) && n_floats, "drone_activation_gradient_scratch: type=%d n_rows=%d N=%d", type, n_rows,
+                  N);
+    int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    rows_per_gradient_block(n_rows, N, sms, &blocks);
-    *n_floats = (long long)blocks * N;
+    *n_floats = (long long)gradient_blocks(type, n_rows, N, sms).rows * N;
     return DRONE_OK;
 }
 
@@ -134,29 +157,37 @@ int drone_activation_gradient(int type, int n_rows, int N, const void *d_G, int 
     DRONE_REQUIRE(DRONE_ALIGNED(d_G, type) && DRONE_ALIGNED(d_pre, type) && DRONE_ALIGNED(d_dZ, type),
                   "drone_activation_gradient: an operand is not aligned to its type");
     cudaStream_t st = (cudaStream_t)stream;
-    int sms = 0, blocks = 0;
+    int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    const int rows = rows_per_gradient_block(n_rows, N, sms, &blocks);
+    const GradientBlocks b = gradient_blocks(type, n_rows, N, sms);
     if (d_bias_grad) {
-        const long long need = (long long)blocks * N;
+        const long long need = (long long)b.rows * N;
         DRONE_REQUIRE(n_scratch >= need && (need == 0 || d_scratch), "drone_activation_gradient: %lld floats of scratch, %lld needed", n_scratch, need);
     }
     if (n_rows > 0 && (d_dZ || d_bias_grad)) {
         const int launched = with_type(type, [&](auto tag) {
             using T = typename decltype(tag)::T;
-            activation_gradient_kernel<T><<<dim3(blocks, ceil_div(N, 32)), 256, 0, st>>>((const T *)d_G, ldg, (const T *)d_pre, ldp, activation, n_rows, N,
-                                                                                          rows, (T *)d_dZ, ldz, d_bias_grad ? d_scratch : nullptr);
-            DRONE_LAUNCH_CHECK("activation_gradient_kernel");
-            return DRONE_OK;
+            constexpr int V = kVector<T>;
+            const bool vec = N % V == 0 && rows_on_16_bytes(d_G, ldg, sizeof(T)) && (!reads_pre || rows_on_16_bytes(d_pre, ldp, sizeof(T))) &&
+                             (!d_dZ || rows_on_16_bytes(d_dZ, ldz, sizeof(T)));
+            return with_row_shape(ceil_div(b.width, V), [&](auto shape) {
+                constexpr int L = decltype(shape)::L, U = decltype(shape)::U;
+                if constexpr (L == 8 || L == 32) {
+                    with_activation(activation, [&](auto act) {
+                        constexpr int A = decltype(act)::value;
+                        auto *const kernel = vec ? activation_gradient_kernel<T, L, U, true, A> : activation_gradient_kernel<T, L, U, false, A>;
+                        kernel<<<dim3(b.rows, b.columns), 256, 0, st>>>((const T *)d_G, ldg, (const T *)d_pre, ldp, n_rows, N, b.width, (T *)d_dZ, ldz,
+                                                                        d_bias_grad ? d_scratch : nullptr);
+                    });
+                }
+                DRONE_LAUNCH_CHECK("activation_gradient_kernel");
+                return DRONE_OK;
+            });
         });
         if (launched) return launched;
     }
-    if (d_bias_grad) {
-        fold_columns_kernel<<<ceil_div(N, 32), 256, 0, st>>>(d_scratch, blocks, N, d_bias_grad);
-        DRONE_LAUNCH_CHECK("fold_columns_kernel");
-    }
-    return DRONE_OK;
+    return d_bias_grad ? fold_columns(d_scratch, b.rows, N, d_bias_grad, N, nullptr, st) : DRONE_OK;
 }
 
 int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, int transposed, long long *n_floats) {

@@ -327,6 +327,9 @@ product_tile_kernel(Operand<T> A, Operand<T> B, int M, int N, int K, int share, 
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] += w[i];
             }
+            if (!ended)      // a wait was given up: nothing plausible comes out
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = NAN;
 #pragma unroll
             for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(tile + row * PITCH + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
@@ -339,57 +342,59 @@ product_tile_kernel(Operand<T> A, Operand<T> B, int M, int N, int K, int share, 
         return;
     }
     const int rows = (int)min((long long)S::ROWS, M - m0), width = min(BN, N - n0);
-    auto value = [&](int r, int c) {
-        float acc = tile[r * PITCH + c];
-        if (!ended) return NAN;      // a wait was given up: nothing plausible comes out
-        if (S::PLANES > 1 && !isfinite(acc)) acc = plain_product<T, A_ALONG_K, B_ALONG_K>(A, B, m0 + r, n0 + c, k0, k1);
+    auto mended = [&](float acc, int r, int c) {      // what the split does not give
+        if (S::PLANES > 1 && !(fabsf(acc) < INFINITY)) acc = ended ? plain_product<T, A_ALONG_K, B_ALONG_K>(A, B, m0 + r, n0 + c, k0, k1) : NAN;
         return acc;
     };
     if (out.shares) {
         float *const to = out.shares + ((long long)blockIdx.y * M + m0) * N + n0;
         for (int r = warp; r < rows; r += 8)
-            for (int c = threadIdx.x & 31; c < width; c += 32) to[(long long)r * N + c] = value(r, c);
+            for (int c = threadIdx.x & 31; c < width; c += 32) to[(long long)r * N + c] = mended(tile[r * PITCH + c], r, c);
         return;
     }
-    if (out.fours) {
-        constexpr int LANES = BN / 4, AT_ONCE = 256 / LANES;      // of a row; rows
-        const int c = (int)(threadIdx.x % LANES) * 4;
-        if (c >= width) return;
-        float b[4] = {0, 0, 0, 0};
-        if (out.bias) {
-            const float4 x = __ldg((const float4 *)(out.bias + n0 + c));
-            b[0] = x.x, b[1] = x.y, b[2] = x.z, b[3] = x.w;
-        }
-        for (int r = threadIdx.x / LANES; r < rows; r += AT_ONCE) {
+    with_activation(out.activation, [&](auto act) {
+        constexpr int ACTIVATION = decltype(act)::value;
+        if (out.fours) {
+            constexpr int LANES = BN / 4, AT_ONCE = 256 / LANES;      // of a row; rows
             using Four = Values<T, 4>;
-            Four x = {}, y, z;
-            float before[4], after[4], added[4];
-            const long long row = m0 + r;
-            if (out.residual) x = *reinterpret_cast<const Four *>(out.residual + row * out.ldr + n0 + c);
-            x.get(added);
+            const int c = (int)(threadIdx.x % LANES) * 4;
+            if (c >= width) return;
+            float4 b = make_float4(0, 0, 0, 0);
+            if (out.bias) b = __ldg((const float4 *)(out.bias + n0 + c));
+#pragma unroll 2
+            for (int r = threadIdx.x / LANES; r < rows; r += AT_ONCE) {
+                const long long row = m0 + r;
+                Four x = {}, y;
+                if (out.residual) x = *reinterpret_cast<const Four *>(out.residual + row * out.ldr + n0 + c);
+                const float4 acc = *reinterpret_cast<const float4 *>(tile + r * PITCH + c);
+                float z[4] = {mended(acc.x, r, c) + b.x, mended(acc.y, r, c + 1) + b.y, mended(acc.z, r, c + 2) + b.z, mended(acc.w, r, c + 3) + b.w}, v[4], added[4];
+                x.get(added);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                before[i] = value(r, c + i) + b[i];
-                after[i] = activate(before[i], out.activation);
-                if (out.residual) after[i] += added[i];
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = activate<T, ACTIVATION>(z[i]);
+                    if (out.residual) v[i] += added[i];
+                }
+                if (out.pre) {
+                    Four p;
+                    p.set(z);
+                    *reinterpret_cast<Four *>(out.pre + row * out.ldp + n0 + c) = p;
+                }
+                y.set(v);
+                *reinterpret_cast<Four *>(out.y + row * out.ldy + n0 + c) = y;
             }
-            z.set(before);
-            y.set(after);
-            if (out.pre) *reinterpret_cast<Four *>(out.pre + row * out.ldp + n0 + c) = z;
-            *reinterpret_cast<Four *>(out.y + row * out.ldy + n0 + c) = y;
+            return;
         }
-        return;
-    }
-    for (int r = warp; r < rows; r += 8)
-        for (int c = threadIdx.x & 31; c < width; c += 32) {
-            const long long row = m0 + r;
-            float acc = value(r, c);
-            if (out.bias) acc += __ldg(out.bias + n0 + c);
-            if (out.pre) out.pre[row * out.ldp + n0 + c] = from_float<T>(acc);
-            float v = activate(acc, out.activation);
-            if (out.residual) v += to_float(out.residual[row * out.ldr + n0 + c]);
-            out.y[row * out.ldy + n0 + c] = from_float<T>(v);
-        }
+        for (int r = warp; r < rows; r += 8)
+            for (int c = threadIdx.x & 31; c < width; c += 32) {
+                const long long row = m0 + r;
+                float acc = mended(tile[r * PITCH + c], r, c);
+                if (out.bias) acc += __ldg(out.bias + n0 + c);
+                if (out.pre) out.pre[row * out.ldp + n0 + c] = from_float<T>(acc);
+                float v = activate<T, ACTIVATION>(acc);
+                if (out.residual) v += to_float(out.residual[row * out.ldr + n0 + c]);
+                out.y[row * out.ldy + n0 + c] = from_float<T>(v);
+            }
+    });
 }
 
 // How many bytes of an operand's rows can be read at once.

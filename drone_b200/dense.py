@@ -152,7 +152,7 @@ def linear_backward(grad, x, w, pre=None, activation=None, transposed=False, bia
         if act != ACT_NONE:
             dz, ldz = torch.empty((n, outputs), dtype=dtype, device=device), outputs
         if act != ACT_NONE or bias:
-            size = call.scratch("drone_activation_gradient_scratch", n, outputs) if bias else (None, 0)
+            size = call.scratch("drone_activation_gradient_scratch", kind, n, outputs) if bias else (None, 0)
             call("drone_activation_gradient", kind, n, outputs, grad.data_ptr(), ldg, _pointer(pre) if act != ACT_NONE else None,
                  ldp if act != ACT_NONE else 0, act, dz.data_ptr() if act != ACT_NONE else None, ldz, _pointer(grad_b), _pointer(size[0]), size[1])
         if input_gradient:

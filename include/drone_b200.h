@@ -387,7 +387,7 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
 /* The step from the gradient of Y to that before the activation, and to that of the bias: dZ = G * activation'(pre),
  * bias_grad = column sums of the unrounded dZ.  d_dZ may be d_G with the same leading dimension, or NULL (sums only), d_bias_grad may be
  * NULL; d_pre is not read without an activation; for the ReLU anything with the same sign will do. */
-int drone_activation_gradient_scratch(int n_rows, int N, long long *n_floats);
+int drone_activation_gradient_scratch(int type, int n_rows, int N, long long *n_floats);
 int drone_activation_gradient(int type, int n_rows, int N, const void *d_G, int ldg, const void *d_pre, int ldp, int activation,
                               void *d_dZ, int ldz, float *d_bias_grad, float *d_scratch, long long n_scratch, void *stream);
 
