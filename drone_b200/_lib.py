@@ -104,7 +104,8 @@ def _declare(lib):
         "drone_relu_mask": (i, [i, i, vp, i, vp, i, vp]),
         "drone_weight_gradient_scratch": (i, [i, i, i, C.POINTER(ll)]),
         "drone_weight_gradient": (i, [i, i, i, vp, i, vp, i, vp, vp, ll, vp]),
-        "drone_linear": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, i, vp, i, vp, i, vp]),
+        "drone_linear_scratch": (i, [i, i, i, i, C.POINTER(ll)]),
+        "drone_linear": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, i, vp, i, vp, i, vp, ll, vp]),
         "drone_activation_gradient_scratch": (i, [i, i, i, C.POINTER(ll)]),
         "drone_activation_gradient": (i, [i, i, i, vp, i, vp, i, i, vp, i, vp, vp, ll, vp]),
         "drone_linear_weight_gradient_scratch": (i, [i, i, i, i, i, C.POINTER(ll)]),

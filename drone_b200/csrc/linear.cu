@@ -6,16 +6,38 @@
 
 namespace drone {
 
-// Shares of a product, added in order.
+// Shares of a product, added in order.  A block has 32 values, its warps every eighth share.
 template <typename T>
 __global__ void __launch_bounds__(256) add_product_shares_kernel(const float *__restrict__ parts, int shares, int M, int N, T *__restrict__ out, long long ld) {
-    const long long count = (long long)M * N;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < count; i += gridDim.x * 256LL) {
-        double sum = 0;
-#pragma unroll 8
-        for (int s = 0; s < shares; ++s) sum += __ldg(parts + s * count + i);
+    __shared__ double of_warp[8][32];
+    const long long count = (long long)M * N, i = blockIdx.x * 32LL + (threadIdx.x & 31);
+    const int w = threadIdx.x >> 5;
+    double sum = 0;
+    if (i < count) {
+#pragma unroll 4
+        for (int s = w; s < shares; s += 8) sum += __ldg(parts + s * count + i);
+    }
+    of_warp[w][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (w == 0 && i < count) {
+        for (int o = 1; o < 8; ++o) sum += of_warp[o][threadIdx.x];
         out[i / N * ld + i % N] = from_float<T>((float)sum);
     }
+}
+
+int tile_map(CUtensorMap *map, bool bf16, const void *p, long long width, long long rows, long long ld, int box) {
+    using Encode = decltype(&cuTensorMapEncodeTiled);
+    static const Encode encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        return cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) == cudaSuccess ? (Encode)f : nullptr;
+    }();
+    if (!encode) return set_error(DRONE_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t sizes[2] = {(cuuint64_t)width, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, steps[2] = {1, 1};
+    const CUresult rc = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(p), sizes, stride, boxes, steps,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? DRONE_OK : set_error(DRONE_E_CUDA, "cuTensorMapEncodeTiled failed: %d (%lld x %lld, %lld apart)", (int)rc, rows, width, ld);
 }
 
 // dZ = G * activation'(pre) and the sums of its columns, of those from blockIdx.y * width on; sums[blockIdx.x] = those of the block's rows.
@@ -73,18 +95,28 @@ int fold_columns(const float *sums, int blocks, int columns, float *a, int split
     return DRONE_OK;
 }
 
-// How the rows of a weight gradient, its K, are cut: two blocks an SM, but a share of four steps at least.
+// How the rows of a weight gradient, its K, are cut: a block an SM, but a share of four steps at least.
 struct Shares {
-    int bn, share, count;
+    int share, count;
 };
-static Shares product_shares(int type, int M, int N, int K, int sms) {
-    const int step = type == DRONE_F32 ? TileShape<float>::KS : TileShape<__half>::KS;
+template <typename T>
+static Shares product_shares(int M, int N, int K, int sms) {
+    using S = TileShape<T>;
+    const int most = std::max(1, sms / (ceil_div(M, S::ROWS) * ceil_div(N, S::BN)));
     Shares s;
-    s.bn = N <= 64 ? 64 : 128;
-    const int most = std::max(1, 2 * sms / (ceil_div(M, 128) * ceil_div(N, s.bn)));
-    s.share = std::max(4 * step, ceil_div(ceil_div(K, most), step) * step);
+    s.share = std::max(4 * S::KS, ceil_div(ceil_div(K, most), S::KS) * S::KS);
     s.count = std::max(1, ceil_div(K, s.share));
     return s;
+}
+static Shares product_shares(int type, int M, int N, int K, int sms) {
+    return type == DRONE_F32 ? product_shares<float>(M, N, K, sms) : product_shares<__half>(M, N, K, sms);
+}
+
+// Floats of the image of a product's weights.
+template <typename T>
+static long long image_floats(int K, int N) {
+    using S = TileShape<T>;
+    return (long long)ceil_div(N, S::BN) * ceil_div(K, S::KS) * (S::B_BYTES / 4);
 }
 
 // Blocks of the activations' gradient: as many as the SMs hold, of at most 128 vectors a row.
@@ -110,8 +142,14 @@ using namespace drone;
 
 extern "C" {
 
+int drone_linear_scratch(int type, int n_rows, int K, int N, long long *n_floats) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && n_floats, "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d", type, n_rows, K, N);
+    *n_floats = n_rows == 0 ? 0 : type == DRONE_F32 ? image_floats<float>(K, N) : image_floats<__half>(K, N);
+    return DRONE_OK;
+}
+
 int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_W, int ldw, int transposed, const float *d_bias,
-                 int activation, const void *d_residual, int ldr, void *d_Y, int ldy, void *d_pre, int ldp, void *stream) {
+                 int activation, const void *d_residual, int ldr, void *d_Y, int ldy, void *d_pre, int ldp, float *d_scratch, long long n_scratch, void *stream) {
     DRONE_REQUIRE(DRONE_TYPE_OK(type), "drone_linear: type=%d", type);
     DRONE_REQUIRE(DRONE_LINEAR_SIZES(n_rows, K, N), "drone_linear: n_rows=%d K=%d N=%d", n_rows, K, N);
     DRONE_REQUIRE(activation >= DRONE_ACT_NONE && activation <= DRONE_ACT_SILU, "drone_linear: activation=%d", activation);
@@ -120,7 +158,14 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
     if (n_rows == 0) return DRONE_OK;
     DRONE_REQUIRE(d_X && d_W && d_Y, "drone_linear: NULL argument");
     DRONE_REQUIRE(DRONE_ALIGNED(d_X, type) && DRONE_ALIGNED(d_W, type) && DRONE_ALIGNED(d_Y, type) && DRONE_ALIGNED(d_residual, type) &&
-                  DRONE_ALIGNED(d_pre, type), "drone_linear: an operand is not aligned to its type");
+                  DRONE_ALIGNED(d_pre, type) && (reinterpret_cast<uintptr_t>(d_bias) & 3) == 0, "drone_linear: an operand is not aligned to its type");
+    long long need = 0;
+    int sms = 0, rc = drone_linear_scratch(type, n_rows, K, N, &need);
+    if (rc) return rc;
+    DRONE_REQUIRE(n_scratch >= need && d_scratch && (reinterpret_cast<uintptr_t>(d_scratch) & 15) == 0,
+                  "drone_linear: %lld floats of scratch on 16 bytes needed, %lld at %p given", need, n_scratch, (void *)d_scratch);
+    rc = device_sms(&sms);
+    if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
@@ -128,11 +173,12 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
         const bool in_fours = N % 4 == 0 && (reinterpret_cast<uintptr_t>(d_bias) & 15) == 0 && fours(d_Y, ldy) && fours(d_residual, ldr) && fours(d_pre, ldp);
         const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr, in_fours};
         const Operand<T> x = operand<T>(d_X, ldx), w = operand<T>(d_W, ldw);
-        if (N <= 64)
-            return transposed ? launch_product_tiles<T, 64, true, true>(x, w, n_rows, N, K, K, 1, out, st)
-                              : launch_product_tiles<T, 64, true, false>(x, w, n_rows, N, K, K, 1, out, st);
-        return transposed ? launch_product_tiles<T, 128, true, true>(x, w, n_rows, N, K, K, 1, out, st)
-                          : launch_product_tiles<T, 128, true, false>(x, w, n_rows, N, K, K, 1, out, st);
+        if constexpr (sizeof(T) == 2)
+            if (x.bytes == 16 && w.bytes == 16)
+                return transposed ? launch_product_tiles<T, kCopied, true, true>(x, w, n_rows, N, K, K, 1, nullptr, out, sms, st)
+                                  : launch_product_tiles<T, kCopied, true, false>(x, w, n_rows, N, K, K, 1, nullptr, out, sms, st);
+        return transposed ? launch_product_tiles<T, kImage, true, true>(x, w, n_rows, N, K, K, 1, d_scratch, out, sms, st)
+                          : launch_product_tiles<T, kImage, true, false>(x, w, n_rows, N, K, K, 1, d_scratch, out, sms, st);
     });
 }
 
@@ -226,10 +272,13 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
         using T = typename decltype(tag)::T;
         const Operand<T> a = transposed ? operand<T>(d_dZ, ldz) : operand<T>(d_X, ldx), b = transposed ? operand<T>(d_X, ldx) : operand<T>(d_dZ, ldz);
         const LinearOut<T> out = {nullptr, DRONE_ACT_NONE, nullptr, 0, nullptr, 0, nullptr, 0, d_scratch, false};
-        const int launched = s.bn == 64 ? launch_product_tiles<T, 64, false, false>(a, b, rows, columns, n_rows, s.share, s.count, out, st)
-                                        : launch_product_tiles<T, 128, false, false>(a, b, rows, columns, n_rows, s.share, s.count, out, st);
+        const int launched = [&] {
+            if constexpr (sizeof(T) == 2)
+                if (a.bytes == 16 && b.bytes == 16) return launch_product_tiles<T, kCopied, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
+            return launch_product_tiles<T, kThrough, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
+        }();
         if (launched) return launched;
-        add_product_shares_kernel<T><<<std::min(ceil_div((long long)rows * columns, 256), sms * 8), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
+        add_product_shares_kernel<T><<<ceil_div((long long)rows * columns, 32), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
         DRONE_LAUNCH_CHECK("add_product_shares_kernel");
         return DRONE_OK;
     });

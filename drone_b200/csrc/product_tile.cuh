@@ -1,17 +1,27 @@
-// C[M, N] = A[M, K] B[K, N] on the tensor cores: a block has a tile of 128 rows and BN columns, its accumulators in tensor memory.
+// C[M, N] = A[M, K] B[K, N] on the tensor cores: one block an SM walks tiles of 128 rows and BN columns, with two sets of accumulators in
+// tensor memory, so that a tile's way to global memory and the next one's products overlap.
 //
-// Eight warps bring the operands: they read a step of K from global memory into registers, whatever the rows' alignment (features of
-// 602 or 47 values start anywhere, which no tensor map takes), and store it in the swizzled order that the matrix instructions read; one
-// thread issues these.  The values of A and B lie along K or along the other dimension in shared memory as they do in global memory.
+// Its warps: 8 take finished tiles out (bias, activation, residual), one issues the matrix instructions, one the asynchronous copies, and
+// where an operand needs registers on its way 8 more bring it.  Operands come in one of three ways:
+//   kCopied    both 16-bit and on 16-byte boundaries: tensor copies, tiles lie in shared memory as they do in global memory (along K or not)
+//   kImage     A through registers, from any address (features of 602 or 47 values start anywhere, which no tensor map takes), floats split on
+//              the way; B from an image of it that image_kernel has written, a copy a step
+//   kThrough   both through registers
 //
 // Floats are split into three bfloat16 of 8 bits each, x = h + m + l exactly (but for values below 2^-110), and six of the nine products are added:
 // h h' in one accumulator, h m' + m h' + m m' + h l' + l h' in a second one that is 2^-8 of it, so that neither loses bits of the other.
-// The rest is below 2^-25 of |x y|.  An output that is not finite (infinities split into NaN, values within 2^-9 of the largest float round
-// to infinity) is computed again from the operands.
+// The rest is below 2^-25 of |x y|.  The accumulators cut off what they cannot hold, half a unit an addition in the mean and always towards
+// 0: after every 256 of K they are added up in shared memory, rounding to nearest, and begin anew.  An output that is not finite (infinities split into NaN, values within
+// 2^-9 of the largest float round to infinity) is computed again from the operands.
+//
+// All waits end after two seconds; a block whose wait did leaves NaN in its outputs.
 #pragma once
 
 #include "dense_types.cuh"
 
+#include <cuda.h>
+
+#include <algorithm>
 #include <type_traits>
 
 namespace drone {
@@ -39,16 +49,21 @@ struct Operand {
     int bytes;
 };
 
+enum Bring { kCopied, kImage, kThrough };
+
 template <typename T> struct TileShape {
     static constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+    static constexpr int ROWS = 128, BN = sizeof(T) == 4 ? 128 : 256;
     static constexpr int KS = sizeof(T) == 4 ? 32 : 64;          // of K in a step
-    static constexpr int STAGES = sizeof(T) == 4 ? 2 : 3;
-    static constexpr int ROWS = 128, THREADS = 256 + 32;
-    static constexpr int operand_bytes(int rows) { return PLANES * rows * KS * 2; }
-    static constexpr int stage_bytes(int bn) { return operand_bytes(ROWS) + operand_bytes(bn); }
-    static constexpr int accumulators = sizeof(T) == 4 ? 2 : 1;
-    static constexpr int shared_bytes(int bn) { return STAGES * stage_bytes(bn) + 1024; }
+    static constexpr int STAGES = 3;
+    static constexpr int CHUNK = sizeof(T) == 4 ? 256 / KS : 1 << 30;      // steps until the accumulators are added up
+    static constexpr int A_PLANE = ROWS * KS * 2, B_PLANE = BN * KS * 2, A_BYTES = PLANES * A_PLANE, B_BYTES = PLANES * B_PLANE, STAGE = A_BYTES + B_BYTES;
+    static constexpr int SET = (sizeof(T) == 4 ? 2 : 1) * BN;    // columns of tensor memory of a set of accumulators, of which there are two
+    // floats between the rows on their way out: of a whole tile whose sums are kept there, or of a warp's piece of 32 x 32
+    static constexpr int PITCH = sizeof(T) == 4 ? BN + 4 : 36;
+    static constexpr int SHARED = 1024 + STAGES * STAGE + (sizeof(T) == 4 ? ROWS : 8 * 32) * PITCH * 4;
 };
+constexpr int kOutWarps = 8, kBringThreads = 256, kBringFrom = (kOutWarps + 2) * 32;
 
 __device__ __forceinline__ unsigned shared_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrier_init(unsigned bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); }
@@ -137,7 +152,7 @@ __device__ __forceinline__ unsigned bf16_pair(float low, float high) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(low, high);
     return reinterpret_cast<const unsigned &>(p);
 }
-__device__ __forceinline__ void store_eight(unsigned at, unsigned plane_bytes, const float (&v)[8]) {
+__device__ __forceinline__ void split_eight(const float (&v)[8], uint4 (&planes)[3]) {
     unsigned h[4], m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -148,46 +163,51 @@ __device__ __forceinline__ void store_eight(unsigned at, unsigned plane_bytes, c
         a -= __uint_as_float(m[i] << 16), b -= __uint_as_float(m[i] & 0xffff0000u);
         l[i] = bf16_pair(a, b);
     }
-    store_shared(at, h[0], h[1], h[2], h[3]);
-    store_shared(at + plane_bytes, m[0], m[1], m[2], m[3]);
-    store_shared(at + 2 * plane_bytes, l[0], l[1], l[2], l[3]);
+    planes[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    planes[1] = make_uint4(m[0], m[1], m[2], m[3]);
+    planes[2] = make_uint4(l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ void store_eight(unsigned at, unsigned plane_bytes, const float (&v)[8]) {
+    uint4 planes[3];
+    split_eight(v, planes);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) store_shared(at + q * plane_bytes, planes[q].x, planes[q].y, planes[q].z, planes[q].w);
 }
 __device__ __forceinline__ void store_eight(unsigned at, unsigned, const unsigned (&v)[4]) { store_shared(at, v[0], v[1], v[2], v[3]); }
 
-// What a thread brings of an operand in each step: UNITS times eight values.
+// What a thread brings of an operand's tile in each step: UNITS times eight values.
 template <typename T, int R, bool ALONG_K>
 struct Share {
     using S = TileShape<T>;
     using L = SharedLayout<S::KS, ALONG_K>;
-    static constexpr int ACROSS = (ALONG_K ? S::KS : R) / 8;                 // units of a row
-    static constexpr int UNITS = R * S::KS / 8 / 256, STEP = 256 / ACROSS;   // rows between a thread's units
+    static constexpr int ACROSS = (ALONG_K ? S::KS : R) / 8;                                   // units of a row
+    static constexpr int UNITS = R * S::KS / 8 / kBringThreads, STEP = kBringThreads / ACROSS;   // rows between a thread's units
     static constexpr unsigned PLANE = R * S::KS * 2;
     using Eight = std::conditional_t<sizeof(T) == 4, float[8], unsigned[4]>;
-    const T *at;
-    long long ld;
-    // limit: rows or columns of the tile that exist; needed: that the instructions read; k: of K until the share's end
-    int row, unit, bytes, limit, needed, k;
+    struct Eights { Eight v[UNITS]; };
+    Operand<T> from;
+    int row, unit;
+    const T *at = nullptr;
+    int limit = 0, k = 0;      // rows or columns of the tile that exist; of K until the share's end
 
-    __device__ Share(const Operand<T> &o, long long start, int size, int read, int k0, int k1) : ld(o.ld), bytes(o.bytes), limit(size), needed(read), k(k1 - k0) {
-        row = threadIdx.x / ACROSS, unit = threadIdx.x % ACROSS;
-        at = ALONG_K ? o.at + (start + row) * ld + k0 + unit * 8 : o.at + (long long)(k0 + row) * ld + start + unit * 8;
+    __device__ Share(const Operand<T> &o, int thread) : from(o), row(thread / ACROSS), unit(thread % ACROSS) {}
+    __device__ void begin(long long start, int size, int k0, int k1) {
+        at = ALONG_K ? from.at + (start + row) * from.ld + k0 + unit * 8 : from.at + (long long)(k0 + row) * from.ld + start + unit * 8;
+        limit = size, k = k1 - k0;
     }
-    __device__ void load(Eight (&v)[UNITS]) {
+    __device__ void load(Eights &to) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const int r = row + u * STEP;
             const bool in_row = ALONG_K ? r < limit : r < k;
-            load_eight(at + (long long)(u * STEP) * ld, in_row ? (ALONG_K ? k : limit) - unit * 8 : 0, bytes, v[u]);
+            load_eight(at + (long long)(u * STEP) * from.ld, in_row ? (ALONG_K ? k : limit) - unit * 8 : 0, from.bytes, to.v[u]);
         }
         k -= S::KS;
-        at += ALONG_K ? S::KS : S::KS * ld;
+        at += ALONG_K ? S::KS : S::KS * from.ld;
     }
-    __device__ void store(unsigned to, const Eight (&v)[UNITS]) const {
+    __device__ void store(unsigned to, const Eights &v) const {
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const int r = row + u * STEP;
-            if ((ALONG_K ? r : unit * 8) < needed) store_eight(to + L::offset(r, unit), PLANE, v[u]);
-        }
+        for (int u = 0; u < UNITS; ++u) store_eight(to + L::offset(row + u * STEP, unit), PLANE, v.v[u]);
     }
 };
 
@@ -198,7 +218,7 @@ __device__ __forceinline__ void mma(unsigned accumulator, unsigned long long a, 
 __device__ __forceinline__ void mma_commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
 }
-__device__ __forceinline__ void load_accumulators(unsigned at, float (&v)[32]) {
+__device__ __forceinline__ void load_accumulators(unsigned at, float *v) {
     unsigned r[32];
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
                  "%23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
@@ -211,6 +231,17 @@ __device__ __forceinline__ void load_accumulators(unsigned at, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ void load_accumulators16(unsigned at, float *v) {
+    unsigned r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // One output from the operands, for those that the split does not give.
 template <typename T, bool A_ALONG_K, bool B_ALONG_K>
 __device__ __noinline__ float plain_product(Operand<T> A, Operand<T> B, long long m, int n, int k0, int k1) {
@@ -220,181 +251,388 @@ __device__ __noinline__ float plain_product(Operand<T> A, Operand<T> B, long lon
     return acc;
 }
 
-template <typename T, int BN, bool A_ALONG_K, bool B_ALONG_K>
-__global__ void __launch_bounds__(TileShape<T>::THREADS, 2)
-product_tile_kernel(Operand<T> A, Operand<T> B, int M, int N, int K, int share, LinearOut<T> out) {
+__device__ __forceinline__ void expect_bytes(unsigned bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_tile(unsigned to, const CUtensorMap *map, int x, int y, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 :: "r"(to), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void copy_bytes(unsigned to, const void *from, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" :: "r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+
+// The tiles of a block, in turn: columns first, so that blocks at work at the same time share their rows, then rows, then shares of K.
+struct TileWalk {
+    int tiles_n, tiles_m, M, N, K, share, bn, ks;
+    long long tile, count;
+    long long m0;
+    int n0, k0, k1, steps, index;      // index: of the share
+    __device__ TileWalk(int M_, int N_, int K_, int share_, int shares, int bn_, int ks_)
+        : tiles_n((N_ + bn_ - 1) / bn_), tiles_m((M_ + 127) / 128), M(M_), N(N_), K(K_), share(share_), bn(bn_), ks(ks_), tile(blockIdx.x) {
+        count = (long long)tiles_n * tiles_m * shares;
+        place();
+    }
+    __device__ bool valid() const { return tile < count; }
+    __device__ void next() {
+        tile += gridDim.x;
+        place();
+    }
+    __device__ void place() {
+        if (tile >= count) return;
+        const long long a_share = (long long)tiles_n * tiles_m, in_share = tile % a_share;
+        index = (int)(tile / a_share);
+        m0 = in_share / tiles_n * 128;
+        n0 = (int)(in_share % tiles_n) * bn;
+        k0 = index * share;
+        k1 = min(K, k0 + share);
+        steps = (k1 - k0 + ks - 1) / ks;
+    }
+    __device__ int rows() const { return (int)min(128LL, M - m0); }
+    __device__ int width() const { return min(bn, N - n0); }
+    __device__ int columns() const { return (width() + 15) / 16 * 16; }      // that the instructions compute
+};
+
+template <typename T, Bring BRING, bool A_ALONG_K, bool B_ALONG_K>
+struct ProductArgs {
+    Operand<T> A, B;
+    CUtensorMap map_a, map_b;      // kCopied
+    const char *image;             // kImage
+    int M, N, K, share, shares;
+    LinearOut<T> out;
+};
+
+// 32 x 32 values of a finished tile, of which the warp has written a row a lane to shared memory, to the outputs with neighbouring columns in
+// neighbouring lanes.
+template <typename T, int PITCH, int ACTIVATION>
+__device__ __forceinline__ void put_piece(const LinearOut<T> &out, const float *piece, long long row0, int rows, int col0, int width) {
+    const int lane = threadIdx.x & 31;
+    if (out.fours) {
+        using Four = Values<T, 4>;
+        const int c = (lane & 7) * 4;
+        if (c >= width) return;
+        float4 b = make_float4(0, 0, 0, 0);
+        if (out.bias) b = __ldg((const float4 *)(out.bias + col0 + c));
+#pragma unroll 4
+        for (int r = lane >> 3; r < rows; r += 4) {
+            const long long row = row0 + r;
+            Four x = {}, y;
+            if (out.residual) x = *reinterpret_cast<const Four *>(out.residual + row * out.ldr + col0 + c);
+            const float4 acc = *reinterpret_cast<const float4 *>(piece + r * PITCH + c);
+            float z[4] = {acc.x + b.x, acc.y + b.y, acc.z + b.z, acc.w + b.w}, w[4], added[4];
+            x.get(added);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = activate<T, ACTIVATION>(z[i]);
+                if (out.residual) w[i] += added[i];
+            }
+            if (out.pre) {
+                Four p;
+                p.set(z);
+                *reinterpret_cast<Four *>(out.pre + row * out.ldp + col0 + c) = p;
+            }
+            y.set(w);
+            *reinterpret_cast<Four *>(out.y + row * out.ldy + col0 + c) = y;
+        }
+    } else if (lane < width) {
+        const float b = out.bias ? __ldg(out.bias + col0 + lane) : 0.f;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+            const long long row = row0 + r;
+            const float z = piece[r * PITCH + lane] + b;
+            float w = activate<T, ACTIVATION>(z);
+            if (out.residual) w += to_float(out.residual[row * out.ldr + col0 + lane]);
+            if (out.pre) out.pre[row * out.ldp + col0 + lane] = from_float<T>(z);
+            out.y[row * out.ldy + col0 + lane] = from_float<T>(w);
+        }
+    }
+}
+
+template <typename T, Bring BRING, bool A_ALONG_K, bool B_ALONG_K>
+__global__ void __launch_bounds__(kBringFrom + (BRING == kCopied ? 0 : kBringThreads), 1)
+product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_ALONG_K> p) {
     using S = TileShape<T>;
+    constexpr bool B_SHARED_ALONG_K = BRING == kImage || B_ALONG_K;
     using LA = SharedLayout<S::KS, A_ALONG_K>;
-    using LB = SharedLayout<S::KS, B_ALONG_K>;
-    constexpr int COLUMNS = S::accumulators * BN, A_PLANE = S::ROWS * S::KS * 2, B_PLANE = BN * S::KS * 2, A_BYTES = S::operand_bytes(S::ROWS);
+    using LB = SharedLayout<S::KS, B_SHARED_ALONG_K>;
     extern __shared__ char bytes[];
-    __shared__ __align__(8) unsigned long long bars[2 * S::STAGES + 1];
+    __shared__ __align__(8) unsigned long long bars[2 * S::STAGES + 5];
     __shared__ unsigned tensor_memory;
     char *const shared = bytes + ((1024 - (shared_address(bytes) & 1023)) & 1023);
-    const unsigned stages = shared_address(shared), full = shared_address(bars), empty = full + 8 * S::STAGES, all_done = full + 16 * S::STAGES;
-    const int tiles_n = (N + BN - 1) / BN, warp = threadIdx.x >> 5;
-    const long long m0 = (long long)(blockIdx.x / tiles_n) * S::ROWS;
-    const int n0 = (int)(blockIdx.x % tiles_n) * BN, k0 = (int)blockIdx.y * share, k1 = min(K, k0 + share), steps = (k1 - k0 + S::KS - 1) / S::KS;
-    const int columns = min(BN, (N - n0 + 15) / 16 * 16);      // of the tile that the instructions compute
+    const unsigned stages = shared_address(shared), full = shared_address(bars), empty = full + 8 * S::STAGES, done = full + 16 * S::STAGES, taken = done + 16,
+                   last = taken + 16;
+    const int warp = threadIdx.x >> 5;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
-            barrier_init(full + 8 * s, 256);
+            barrier_init(full + 8 * s, (BRING == kCopied ? 0 : kBringThreads) + (BRING == kThrough ? 0 : 1));
             barrier_init(empty + 8 * s, 1);
         }
-        barrier_init(all_done, 1);
+        for (int b = 0; b < 2; ++b) {
+            barrier_init(done + 8 * b, 1);
+            barrier_init(taken + 8 * b, kOutWarps);
+        }
+        barrier_init(last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(shared_address(&tensor_memory)), "n"(COLUMNS) : "memory");
+    if (warp == kOutWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(shared_address(&tensor_memory)), "n"(2 * S::SET) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned accumulators = tensor_memory;
+    TileWalk walk(p.M, p.N, p.K, p.share, p.shares, S::BN, S::KS);
 
-    bool ended = true;      // no wait was given up
-    if (warp < 8) {
-        Share<T, S::ROWS, A_ALONG_K> a(A, m0, (int)min((long long)S::ROWS, M - m0), S::ROWS, k0, k1);
-        Share<T, BN, B_ALONG_K> b(B, n0, min(BN, N - n0), columns, k0, k1);
-        typename decltype(a)::Eight va[decltype(a)::UNITS];
-        typename decltype(b)::Eight vb[decltype(b)::UNITS];
-        a.load(va);
-        b.load(vb);
-        for (int s = 0; s < steps && ended; ++s) {
-            const int stage = s % S::STAGES;
-            if (s >= S::STAGES) ended = barrier_wait(empty + 8 * stage, (s / S::STAGES - 1) & 1);
-            const unsigned to = stages + stage * S::stage_bytes(BN);
-            a.store(to, va);
-            b.store(to + A_BYTES, vb);
+    if (warp < kOutWarps) {
+        // Takes tiles out: a quarter of the rows (the lanes of tensor memory that the warp can read), half of the columns.
+        constexpr int HALF = S::BN / 2;
+        const int lane_row = (warp & 3) * 32, half = (warp >> 2) * HALF;
+        float *const piece = reinterpret_cast<float *>(shared + S::STAGES * S::STAGE) + (S::PLANES > 1 ? lane_row * S::PITCH + half : warp * 32 * S::PITCH);
+        float *const row = piece + (threadIdx.x & 31) * S::PITCH;      // this lane's
+        bool ended = true;      // no wait was given up
+        unsigned chunk = 0;     // of the block, over all tiles
+        with_activation(p.out.activation, [&](auto act) {
+            constexpr int ACTIVATION = decltype(act)::value;
+            for (; walk.valid(); walk.next()) {
+                const int rows = min(32, walk.rows() - lane_row), width = walk.width() - half;
+                auto put = [&](const float *from, int c) {      // 32 columns from c on
+                    if (rows <= 0 || width - c <= 0) return;
+                    if (p.out.shares) {
+                        LinearOut<float> to = {};
+                        to.y = p.out.shares + (long long)walk.index * p.M * p.N;
+                        to.ldy = p.N;
+                        to.fours = p.N % 4 == 0;
+                        put_piece<float, S::PITCH, DRONE_ACT_NONE>(to, from, walk.m0 + lane_row, rows, walk.n0 + half + c, min(32, width - c));
+                    } else {
+                        put_piece<T, S::PITCH, ACTIVATION>(p.out, from, walk.m0 + lane_row, rows, walk.n0 + half + c, min(32, width - c));
+                    }
+                };
+                if constexpr (S::PLANES > 1) {
+                    for (int s = 0; s < walk.steps; s += S::CHUNK, ++chunk) {
+                        const unsigned set = chunk & 1, at = accumulators + ((unsigned)lane_row << 16) + set * S::SET + half;
+                        ended = ended && barrier_wait(done + 8 * set, (chunk >> 1) & 1);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        bool fine = true;
+#pragma unroll 1
+                        for (int c = 0; c < HALF && c < width; c += 16) {
+                            float a[16], b[16];
+                            load_accumulators16(at + c, a);
+                            load_accumulators16(at + S::BN + c, b);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) {
+                                float4 *const to = reinterpret_cast<float4 *>(row + c + i);
+                                float4 v = make_float4(a[i] + b[i], a[i + 1] + b[i + 1], a[i + 2] + b[i + 2], a[i + 3] + b[i + 3]);
+                                if (s > 0) {
+                                    const float4 before = *to;
+                                    v = make_float4(before.x + v.x, before.y + v.y, before.z + v.z, before.w + v.w);
+                                }
+                                if (!ended) v = make_float4(NAN, NAN, NAN, NAN);      // a wait was given up: nothing plausible comes out
+                                fine = fine && fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
+                                *to = v;
+                            }
+                        }
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if ((threadIdx.x & 31) == 0) barrier_arrive(taken + 8 * set);
+                        if (s + S::CHUNK >= walk.steps && !fine && ended && (int)(threadIdx.x & 31) < rows) {      // what the split does not give
+#pragma unroll 1
+                            for (int c = 0; c < HALF && c < width; ++c)
+                                if (!(fabsf(row[c]) < INFINITY))
+                                    row[c] = plain_product<T, A_ALONG_K, B_ALONG_K>(p.A, p.B, walk.m0 + lane_row + (threadIdx.x & 31), walk.n0 + half + c, walk.k0, walk.k1);
+                        }
+                        __syncwarp();
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < HALF; c += 32) put(piece + c, c);
+                    __syncwarp();      // the tile has been read
+                } else {
+                    const unsigned set = chunk & 1, at = accumulators + ((unsigned)lane_row << 16) + set * S::SET + half;
+                    ended = ended && barrier_wait(done + 8 * set, (chunk >> 1) & 1);
+                    ++chunk;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int c = 0; c < HALF && c < width; c += 32) {
+                        float v[32];
+                        load_accumulators(at + c, v);
+                        __syncwarp();      // the piece before has been read
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            if (!ended) w = make_float4(NAN, NAN, NAN, NAN);
+                            *reinterpret_cast<float4 *>(row + i) = w;
+                        }
+                        __syncwarp();
+                        put(piece, c);
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if ((threadIdx.x & 31) == 0) barrier_arrive(taken + 8 * set);
+                }
+            }
+        });
+    } else if (threadIdx.x == kOutWarps * 32) {
+        // Issues the matrix instructions.
+        constexpr unsigned TYPE = std::is_same_v<T, __half> ? 0 : 1;
+        bool ended = true;
+        unsigned step = 0, chunk = 0;      // of the block, over all tiles
+        for (; walk.valid() && ended; walk.next()) {
+            // float accumulators, both operands of this type, lying along K (0) or not (1), columns / 8, rows / 16
+            const unsigned instruction = 1u << 4 | TYPE << 7 | TYPE << 10 | (A_ALONG_K ? 0u : 1u) << 15 | (B_SHARED_ALONG_K ? 0u : 1u) << 16 |
+                                         (unsigned)(walk.columns() / 8) << 17 | (unsigned)(S::ROWS / 16) << 24;
+            for (int s = 0; s < walk.steps && ended; ++s, ++step) {
+                const bool begins = s % S::CHUNK == 0;
+                const unsigned set = chunk & 1, to = accumulators + set * S::SET;
+                if (begins && chunk >= 2) ended = barrier_wait(taken + 8 * set, ((chunk >> 1) - 1) & 1);
+                const int stage = step % S::STAGES;
+                ended = ended && barrier_wait(full + 8 * stage, (step / S::STAGES) & 1);
+                if (!ended) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned a = stages + stage * S::STAGE, b = a + S::A_BYTES;
+#pragma unroll
+                for (int k = 0; k < S::KS; k += 16) {
+                    const bool add = !begins || k > 0;
+                    if (S::PLANES == 1) {
+                        mma(to, LA::descriptor(a, k), LB::descriptor(b, k), instruction, add);
+                    } else {
+                        const unsigned long long ah = LA::descriptor(a, k), am = LA::descriptor(a + S::A_PLANE, k), al = LA::descriptor(a + 2 * S::A_PLANE, k);
+                        const unsigned long long bh = LB::descriptor(b, k), bm = LB::descriptor(b + S::B_PLANE, k), bl = LB::descriptor(b + 2 * S::B_PLANE, k);
+                        mma(to, ah, bh, instruction, add);
+                        mma(to + S::BN, ah, bl, instruction, add);
+                        mma(to + S::BN, al, bh, instruction, true);
+                        mma(to + S::BN, am, bm, instruction, true);
+                        mma(to + S::BN, ah, bm, instruction, true);
+                        mma(to + S::BN, am, bh, instruction, true);
+                    }
+                }
+                mma_commit(empty + 8 * stage);
+                if (s + 1 == walk.steps || (s + 1) % S::CHUNK == 0) {
+                    mma_commit(done + 8 * set);
+                    ++chunk;
+                }
+            }
+        }
+        mma_commit(last);
+    } else if (threadIdx.x == (kOutWarps + 1) * 32) {
+        // Issues the copies.
+        bool ended = true;
+        unsigned step = 0;
+        if (BRING != kThrough)
+            for (; walk.valid() && ended; walk.next()) {
+                const int pieces = (walk.columns() + 63) / 64;      // of 64 columns, of B along N
+                const unsigned a_bytes = BRING == kCopied ? S::A_BYTES : 0, b_bytes = BRING == kCopied && !B_ALONG_K ? pieces * (S::KS * 128) : S::B_BYTES;
+                for (int s = 0; s < walk.steps; ++s, ++step) {
+                    const int stage = step % S::STAGES, k = walk.k0 + s * S::KS;
+                    if (step >= S::STAGES) ended = barrier_wait(empty + 8 * stage, (step / S::STAGES - 1) & 1);
+                    if (!ended) break;
+                    const unsigned bar = full + 8 * stage, a = stages + stage * S::STAGE, b = a + S::A_BYTES;
+                    expect_bytes(bar, a_bytes + b_bytes);
+                    if constexpr (BRING == kCopied) {
+                        if (A_ALONG_K) {
+                            copy_tile(a, &p.map_a, k, (int)walk.m0, bar);
+                        } else {
+                            for (int i = 0; i < S::ROWS / 64; ++i) copy_tile(a + i * (S::KS * 128), &p.map_a, (int)walk.m0 + i * 64, k, bar);
+                        }
+                        if (B_ALONG_K) {
+                            copy_tile(b, &p.map_b, k, walk.n0, bar);
+                        } else {
+                            for (int i = 0; i < pieces; ++i) copy_tile(b + i * (S::KS * 128), &p.map_b, walk.n0 + i * 64, k, bar);
+                        }
+                    } else {
+                        copy_bytes(b, p.image + ((long long)(walk.n0 / S::BN) * walk.steps + s) * S::B_BYTES, S::B_BYTES, bar);
+                    }
+                }
+            }
+        if (!ended)      // copies in flight land before the block goes
+            for (unsigned back = 1; back <= (unsigned)S::STAGES && back <= step; ++back) barrier_wait(full + 8 * ((step - back) % S::STAGES), ((step - back) / S::STAGES) & 1);
+    } else if (BRING != kCopied && warp >= kOutWarps + 2) {
+        // Bring what goes through registers, DEPTH steps ahead.
+        constexpr int DEPTH = BRING == kImage ? 3 : sizeof(T) == 4 ? 2 : 1;      // by the registers that a step takes: 16, 32, 48
+        const int thread = threadIdx.x - kBringFrom;
+        Share<T, S::ROWS, A_ALONG_K> a(p.A, thread);
+        Share<T, S::BN, B_ALONG_K> b(p.B, thread);
+        typename decltype(a)::Eights va[DEPTH];
+        typename decltype(b)::Eights vb[BRING == kThrough ? DEPTH : 1];
+        int s = 0;
+        unsigned asked = 0, step = 0;
+        auto begin = [&] {
+            if (!walk.valid()) return;
+            a.begin(walk.m0, walk.rows(), walk.k0, walk.k1);
+            if (BRING == kThrough) b.begin(walk.n0, walk.width(), walk.k0, walk.k1);
+        };
+        auto load = [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            if (!walk.valid()) return;
+            a.load(va[D]);
+            if constexpr (BRING == kThrough) b.load(vb[D]);
+            ++asked;
+            if (++s == walk.steps) {
+                s = 0;
+                walk.next();
+                begin();
+            }
+        };
+        bool ended = true;
+        auto store = [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            if (step == asked || !ended) return false;
+            const int stage = step % S::STAGES;
+            if (step >= S::STAGES) ended = barrier_wait(empty + 8 * stage, (step / S::STAGES - 1) & 1);
+            if (!ended) return false;
+            const unsigned to = stages + stage * S::STAGE;
+            a.store(to, va[D]);
+            if constexpr (BRING == kThrough) b.store(to + S::A_BYTES, vb[D]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             barrier_arrive(full + 8 * stage);
-            if (s + 1 < steps) {
-                a.load(va);
-                b.load(vb);
-            }
+            ++step;
+            load(d);
+            return true;
+        };
+        begin();
+        load(std::integral_constant<int, 0>());
+        if constexpr (DEPTH == 3) {
+            load(std::integral_constant<int, 1>());
+            load(std::integral_constant<int, 2>());
+            while (store(std::integral_constant<int, 0>()) && store(std::integral_constant<int, 1>()) && store(std::integral_constant<int, 2>())) {}
+        } else if constexpr (DEPTH == 2) {
+            load(std::integral_constant<int, 1>());
+            while (store(std::integral_constant<int, 0>()) && store(std::integral_constant<int, 1>())) {}
+        } else {
+            while (store(std::integral_constant<int, 0>())) {}
         }
-    } else if (threadIdx.x == 256) {
-        // float accumulators, both operands of this type, rows along K (0) or not (1), columns / 8, rows / 16
-        constexpr unsigned TYPE = std::is_same_v<T, __half> ? 0 : 1;
-        const unsigned instruction = 1u << 4 | TYPE << 7 | TYPE << 10 | (A_ALONG_K ? 0u : 1u) << 15 | (B_ALONG_K ? 0u : 1u) << 16 | (unsigned)(columns / 8) << 17 |
-                                     (unsigned)(S::ROWS / 16) << 24;
-        for (int s = 0; s < steps && ended; ++s) {
-            const int stage = s % S::STAGES;
-            ended = barrier_wait(full + 8 * stage, (s / S::STAGES) & 1);
-            if (!ended) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned a = stages + stage * S::stage_bytes(BN), b = a + A_BYTES;
-#pragma unroll
-            for (int k = 0; k < S::KS; k += 16) {
-                const bool add = s > 0 || k > 0;
-                if (S::PLANES == 1) {
-                    mma(accumulators, LA::descriptor(a, k), LB::descriptor(b, k), instruction, add);
-                } else {
-                    const unsigned long long ah = LA::descriptor(a, k), am = LA::descriptor(a + A_PLANE, k), al = LA::descriptor(a + 2 * A_PLANE, k);
-                    const unsigned long long bh = LB::descriptor(b, k), bm = LB::descriptor(b + B_PLANE, k), bl = LB::descriptor(b + 2 * B_PLANE, k);
-                    mma(accumulators, ah, bh, instruction, add);
-                    mma(accumulators + BN, ah, bl, instruction, add);
-                    mma(accumulators + BN, al, bh, instruction, true);
-                    mma(accumulators + BN, am, bm, instruction, true);
-                    mma(accumulators + BN, ah, bm, instruction, true);
-                    mma(accumulators + BN, am, bh, instruction, true);
-                }
-            }
-            mma_commit(empty + 8 * stage);
-        }
-        mma_commit(all_done);
     }
     __syncwarp();
-    ended = barrier_wait(all_done, 0) && ended;
-    ended = __syncthreads_and(ended);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-
-    // Accumulators to shared memory (a row a lane), from there to the outputs with neighbouring columns in neighbouring lanes.
-    constexpr int PITCH = BN + 4;
-    static_assert(S::ROWS * PITCH * 4 <= S::STAGES * S::stage_bytes(BN), "the tile fits the stages");
-    float *const tile = reinterpret_cast<float *>(shared);
-    if (warp < 8) {
-        const int row = (warp & 3) * 32 + (threadIdx.x & 31);
-        for (int c = (warp >> 2) * 32; c < columns; c += 64) {
-            float v[32];
-            const unsigned at = accumulators + ((unsigned)((warp & 3) * 32) << 16) + c;
-            load_accumulators(at, v);
-            if (S::PLANES > 1) {
-                float w[32];
-                load_accumulators(at + BN, w);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] += w[i];
-            }
-            if (!ended)      // a wait was given up: nothing plausible comes out
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = NAN;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(tile + row * PITCH + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    }
+    barrier_wait(last, 0);      // no matrix instruction is in flight
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kOutWarps) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(accumulators), "n"(COLUMNS));
-        return;
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(accumulators), "n"(2 * S::SET));
     }
-    const int rows = (int)min((long long)S::ROWS, M - m0), width = min(BN, N - n0);
-    auto mended = [&](float acc, int r, int c) {      // what the split does not give
-        if (S::PLANES > 1 && !(fabsf(acc) < INFINITY)) acc = ended ? plain_product<T, A_ALONG_K, B_ALONG_K>(A, B, m0 + r, n0 + c, k0, k1) : NAN;
-        return acc;
-    };
-    if (out.shares) {
-        float *const to = out.shares + ((long long)blockIdx.y * M + m0) * N + n0;
-        for (int r = warp; r < rows; r += 8)
-            for (int c = threadIdx.x & 31; c < width; c += 32) to[(long long)r * N + c] = mended(tile[r * PITCH + c], r, c);
-        return;
-    }
-    with_activation(out.activation, [&](auto act) {
-        constexpr int ACTIVATION = decltype(act)::value;
-        if (out.fours) {
-            constexpr int LANES = BN / 4, AT_ONCE = 256 / LANES;      // of a row; rows
-            using Four = Values<T, 4>;
-            const int c = (int)(threadIdx.x % LANES) * 4;
-            if (c >= width) return;
-            float4 b = make_float4(0, 0, 0, 0);
-            if (out.bias) b = __ldg((const float4 *)(out.bias + n0 + c));
-#pragma unroll 2
-            for (int r = threadIdx.x / LANES; r < rows; r += AT_ONCE) {
-                const long long row = m0 + r;
-                Four x = {}, y;
-                if (out.residual) x = *reinterpret_cast<const Four *>(out.residual + row * out.ldr + n0 + c);
-                const float4 acc = *reinterpret_cast<const float4 *>(tile + r * PITCH + c);
-                float z[4] = {mended(acc.x, r, c) + b.x, mended(acc.y, r, c + 1) + b.y, mended(acc.z, r, c + 2) + b.z, mended(acc.w, r, c + 3) + b.w}, v[4], added[4];
-                x.get(added);
+}
+
+// The image of B that kImage copies: for every tile of columns and step of K its values as they lie in shared memory (along K, split if floats).
+template <typename T, bool B_ALONG_K>
+__global__ void __launch_bounds__(256) image_kernel(Operand<T> B, int N, int K, char *image) {
+    using S = TileShape<T>;
+    using L = SharedLayout<S::KS, true>;
+    const int steps = (K + S::KS - 1) / S::KS, n0 = (int)blockIdx.x / steps * S::BN, k0 = (int)blockIdx.x % steps * S::KS;
+    char *const to = image + (long long)blockIdx.x * S::B_BYTES;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < S::BN * S::KS / 8; i += gridDim.y * 256) {
+        const int row = B_ALONG_K ? i / (S::KS / 8) : i % S::BN, unit = B_ALONG_K ? i % (S::KS / 8) : i / S::BN, n = n0 + row, k = k0 + unit * 8;
+        T v[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[i] = activate<T, ACTIVATION>(z[i]);
-                    if (out.residual) v[i] += added[i];
-                }
-                if (out.pre) {
-                    Four p;
-                    p.set(z);
-                    *reinterpret_cast<Four *>(out.pre + row * out.ldp + n0 + c) = p;
-                }
-                y.set(v);
-                *reinterpret_cast<Four *>(out.y + row * out.ldy + n0 + c) = y;
-            }
-            return;
+        for (int e = 0; e < 8; ++e) v[e] = n < N && k + e < K ? B.at[B_ALONG_K ? (long long)n * B.ld + k + e : (long long)(k + e) * B.ld + n] : from_float<T>(0.f);
+        uint4 planes[S::PLANES];
+        if constexpr (S::PLANES == 3) {
+            split_eight(v, planes);
+        } else {
+            memcpy(planes, v, 16);
         }
-        for (int r = warp; r < rows; r += 8)
-            for (int c = threadIdx.x & 31; c < width; c += 32) {
-                const long long row = m0 + r;
-                float acc = mended(tile[r * PITCH + c], r, c);
-                if (out.bias) acc += __ldg(out.bias + n0 + c);
-                if (out.pre) out.pre[row * out.ldp + n0 + c] = from_float<T>(acc);
-                float v = activate<T, ACTIVATION>(acc);
-                if (out.residual) v += to_float(out.residual[row * out.ldr + n0 + c]);
-                out.y[row * out.ldy + n0 + c] = from_float<T>(v);
-            }
-    });
+#pragma unroll
+        for (int q = 0; q < S::PLANES; ++q) *reinterpret_cast<uint4 *>(to + q * S::B_PLANE + L::offset(row, unit)) = planes[q];
+    }
 }
 
 // How many bytes of an operand's rows can be read at once.
@@ -404,13 +642,29 @@ Operand<T> operand(const void *p, long long ld) {
     return {(const T *)p, ld, (int)(bits & (~bits + 1))};
 }
 
-template <typename T, int BN, bool A_ALONG_K, bool B_ALONG_K>
-int launch_product_tiles(const Operand<T> &A, const Operand<T> &B, int M, int N, int K, int share, int shares, const LinearOut<T> &out, cudaStream_t st) {
-    constexpr int bytes = TileShape<T>::shared_bytes(BN);
-    auto *const kernel = product_tile_kernel<T, BN, A_ALONG_K, B_ALONG_K>;
-    DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    const long long tiles = (long long)ceil_div(M, 128) * ceil_div(N, BN);
-    kernel<<<dim3((unsigned)tiles, shares), TileShape<T>::THREADS, bytes, st>>>(A, B, M, N, K, share, out);
+// A tensor map of 16-bit values: boxes of 64 values (128 bytes, in the order of the 128-byte swizzle) of `box` rows.
+int tile_map(CUtensorMap *map, bool bf16, const void *p, long long width, long long rows, long long ld, int box);
+
+template <typename T, Bring BRING, bool A_ALONG_K, bool B_ALONG_K>
+int launch_product_tiles(const Operand<T> &A, const Operand<T> &B, int M, int N, int K, int share, int shares, void *image, const LinearOut<T> &out, int sms,
+                         cudaStream_t st) {
+    using S = TileShape<T>;
+    ProductArgs<T, BRING, A_ALONG_K, B_ALONG_K> p = {};
+    p.A = A, p.B = B, p.image = (const char *)image, p.M = M, p.N = N, p.K = K, p.share = share, p.shares = shares, p.out = out;
+    if (BRING == kCopied) {
+        constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+        int rc = A_ALONG_K ? tile_map(&p.map_a, bf16, A.at, K, M, A.ld, S::ROWS) : tile_map(&p.map_a, bf16, A.at, M, K, A.ld, S::KS);
+        if (!rc) rc = B_ALONG_K ? tile_map(&p.map_b, bf16, B.at, K, N, B.ld, S::BN) : tile_map(&p.map_b, bf16, B.at, N, K, B.ld, S::KS);
+        if (rc) return rc;
+    } else if (BRING == kImage) {
+        const int blocks = ceil_div(N, S::BN) * ceil_div(K, S::KS);
+        image_kernel<T, B_ALONG_K><<<dim3(blocks, S::BN * S::KS / 8 / 256), 256, 0, st>>>(B, N, K, (char *)image);
+        DRONE_LAUNCH_CHECK("image_kernel");
+    }
+    auto *const kernel = product_tile_kernel<T, BRING, A_ALONG_K, B_ALONG_K>;
+    DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
+    const long long tiles = (long long)ceil_div(M, S::ROWS) * ceil_div(N, S::BN) * shares;
+    kernel<<<(unsigned)std::min<long long>(tiles, sms), kBringFrom + (BRING == kCopied ? 0 : kBringThreads), S::SHARED, st>>>(p);
     DRONE_LAUNCH_CHECK("product_tile_kernel");
     return DRONE_OK;
 }

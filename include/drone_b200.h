@@ -380,9 +380,10 @@ int drone_weight_gradient(int K, int M, int N, const float *d_A, int lda, const 
  * d_bias, d_residual, d_pre may be NULL; d_pre receives the values before the activation.  d_residual may be d_Y with the
  * same leading dimension; no other operand may overlap an output.  Products of floats are as exact as float
  * multiply-adds. */
+int drone_linear_scratch(int type, int n_rows, int K, int N, long long *n_floats);
 int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_W, int ldw, int transposed,
                  const float *d_bias, int activation, const void *d_residual, int ldr, void *d_Y, int ldy, void *d_pre, int ldp,
-                 void *stream);
+                 float *d_scratch, long long n_scratch, void *stream);
 
 /* The step from the gradient of Y to that before the activation, and to that of the bias: dZ = G * activation'(pre),
  * bias_grad = column sums of the unrounded dZ.  d_dZ may be d_G with the same leading dimension, or NULL (sums only), d_bias_grad may be
