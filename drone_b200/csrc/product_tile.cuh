@@ -1,7 +1,7 @@
 // C[M, N] = A[M, K] B[K, N] on the tensor cores: one block an SM walks tiles of 128 rows and BN columns, with two sets of accumulators in
 // tensor memory, so that a tile's way to global memory and the next one's products overlap.
 //
-// Its warps: 8 take finished tiles out (bias, activation, residual), one issues the matrix instructions, one the asynchronous copies, and
+// Its warps: 8 or 16 take finished tiles out (bias, activation, residual), one issues the matrix instructions, one the asynchronous copies, and
 // where an operand needs registers on its way 8 more bring it.  Operands come in one of three ways:
 //   kCopied    both 16-bit and on 16-byte boundaries: tensor copies, tiles lie in shared memory as they do in global memory (along K or not)
 //   kImage     A through registers, from any address (features of 602 or 47 values start anywhere, which no tensor map takes), floats split on
@@ -61,9 +61,13 @@ template <typename T> struct TileShape {
     static constexpr int SET = (sizeof(T) == 4 ? 2 : 1) * BN;    // columns of tensor memory of a set of accumulators, of which there are two
     // floats between the rows on their way out: of a whole tile whose sums are kept there, or of a warp's piece of 32 x 32
     static constexpr int PITCH = sizeof(T) == 4 ? BN + 4 : 36;
-    static constexpr int SHARED = 1024 + STAGES * STAGE + (sizeof(T) == 4 ? ROWS : 8 * 32) * PITCH * 4;
+    static constexpr int shared(int out_warps) { return 1024 + STAGES * STAGE + (sizeof(T) == 4 ? ROWS : out_warps * 32) * PITCH * 4; }
 };
-constexpr int kOutWarps = 8, kBringThreads = 256, kBringFrom = (kOutWarps + 2) * 32;
+// Warps that take tiles out, threads that bring operands.  (17 warps and more leave 96 registers a thread.)
+template <Bring BRING> constexpr int kOutWarps = BRING == kCopied ? 16 : 8;
+constexpr int kBringThreads = 256;
+template <Bring BRING> constexpr int kBringFrom = (kOutWarps<BRING> + 2) * 32;
+template <Bring BRING> constexpr int kProductThreads = kBringFrom<BRING> + (BRING == kCopied ? 0 : kBringThreads);
 
 __device__ __forceinline__ unsigned shared_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrier_init(unsigned bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); }
@@ -349,9 +353,10 @@ __device__ __forceinline__ void put_piece(const LinearOut<T> &out, const float *
 }
 
 template <typename T, Bring BRING, bool A_ALONG_K, bool B_ALONG_K>
-__global__ void __launch_bounds__(kBringFrom + (BRING == kCopied ? 0 : kBringThreads), 1)
+__global__ void __launch_bounds__(kProductThreads<BRING>, 1)
 product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_ALONG_K> p) {
     using S = TileShape<T>;
+    constexpr int OUT = kOutWarps<BRING>;
     constexpr bool B_SHARED_ALONG_K = BRING == kImage || B_ALONG_K;
     using LA = SharedLayout<S::KS, A_ALONG_K>;
     using LB = SharedLayout<S::KS, B_SHARED_ALONG_K>;
@@ -370,12 +375,12 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         }
         for (int b = 0; b < 2; ++b) {
             barrier_init(done + 8 * b, 1);
-            barrier_init(taken + 8 * b, kOutWarps);
+            barrier_init(taken + 8 * b, OUT);
         }
         barrier_init(last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kOutWarps) {
+    if (warp == OUT) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(shared_address(&tensor_memory)), "n"(2 * S::SET) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -385,38 +390,51 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
     const unsigned accumulators = tensor_memory;
     TileWalk walk(p.M, p.N, p.K, p.share, p.shares, S::BN, S::KS);
 
-    if (warp < kOutWarps) {
-        // Takes tiles out: a quarter of the rows (the lanes of tensor memory that the warp can read), half of the columns.
-        constexpr int HALF = S::BN / 2;
-        const int lane_row = (warp & 3) * 32, half = (warp >> 2) * HALF;
-        float *const piece = reinterpret_cast<float *>(shared + S::STAGES * S::STAGE) + (S::PLANES > 1 ? lane_row * S::PITCH + half : warp * 32 * S::PITCH);
+    if (warp < OUT) {
+        // Takes tiles out: a quarter of the rows (the lanes of tensor memory that the warp can read) and some of the columns.
+        constexpr int COLUMNS = S::BN / (OUT / 4);
+        const int lane_row = (warp & 3) * 32, first = (warp >> 2) * COLUMNS;
+        float *const piece = reinterpret_cast<float *>(shared + S::STAGES * S::STAGE) + (S::PLANES > 1 ? lane_row * S::PITCH + first : warp * 32 * S::PITCH);
         float *const row = piece + (threadIdx.x & 31) * S::PITCH;      // this lane's
         bool ended = true;      // no wait was given up
         unsigned chunk = 0;     // of the block, over all tiles
         with_activation(p.out.activation, [&](auto act) {
             constexpr int ACTIVATION = decltype(act)::value;
+            // The residual of the tile after the one at work, on its way to L2.
+            auto prefetch = [&](const TileWalk &of) {
+                const int r = threadIdx.x & 31;
+                if (!p.out.residual || !of.valid() || lane_row + r >= of.rows()) return;
+                const T *at = p.out.residual + (of.m0 + lane_row + r) * p.out.ldr + of.n0 + first;
+                for (int c = 0; c < min(COLUMNS, of.width() - first); c += 128 / (int)sizeof(T)) asm volatile("prefetch.global.L2 [%0];" :: "l"(at + c));
+            };
+            TileWalk upcoming = walk;
+            prefetch(upcoming);
             for (; walk.valid(); walk.next()) {
-                const int rows = min(32, walk.rows() - lane_row), width = walk.width() - half;
+                const int rows = min(32, walk.rows() - lane_row), width = walk.width() - first;
+                upcoming.next();
+                prefetch(upcoming);
                 auto put = [&](const float *from, int c) {      // 32 columns from c on
                     if (rows <= 0 || width - c <= 0) return;
+                    const long long row0 = walk.m0 + lane_row;
+                    const int col0 = walk.n0 + first + c, live = min(32, width - c);
                     if (p.out.shares) {
                         LinearOut<float> to = {};
                         to.y = p.out.shares + (long long)walk.index * p.M * p.N;
                         to.ldy = p.N;
                         to.fours = p.N % 4 == 0;
-                        put_piece<float, S::PITCH, DRONE_ACT_NONE>(to, from, walk.m0 + lane_row, rows, walk.n0 + half + c, min(32, width - c));
+                        put_piece<float, S::PITCH, DRONE_ACT_NONE>(to, from, row0, rows, col0, live);
                     } else {
-                        put_piece<T, S::PITCH, ACTIVATION>(p.out, from, walk.m0 + lane_row, rows, walk.n0 + half + c, min(32, width - c));
+                        put_piece<T, S::PITCH, ACTIVATION>(p.out, from, row0, rows, col0, live);
                     }
                 };
                 if constexpr (S::PLANES > 1) {
                     for (int s = 0; s < walk.steps; s += S::CHUNK, ++chunk) {
-                        const unsigned set = chunk & 1, at = accumulators + ((unsigned)lane_row << 16) + set * S::SET + half;
+                        const unsigned set = chunk & 1, at = accumulators + ((unsigned)lane_row << 16) + set * S::SET + first;
                         ended = ended && barrier_wait(done + 8 * set, (chunk >> 1) & 1);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         bool fine = true;
 #pragma unroll 1
-                        for (int c = 0; c < HALF && c < width; c += 16) {
+                        for (int c = 0; c < COLUMNS && c < width; c += 16) {
                             float a[16], b[16];
                             load_accumulators16(at + c, a);
                             load_accumulators16(at + S::BN + c, b);
@@ -438,33 +456,35 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                         if ((threadIdx.x & 31) == 0) barrier_arrive(taken + 8 * set);
                         if (s + S::CHUNK >= walk.steps && !fine && ended && (int)(threadIdx.x & 31) < rows) {      // what the split does not give
 #pragma unroll 1
-                            for (int c = 0; c < HALF && c < width; ++c)
+                            for (int c = 0; c < COLUMNS && c < width; ++c)
                                 if (!(fabsf(row[c]) < INFINITY))
-                                    row[c] = plain_product<T, A_ALONG_K, B_ALONG_K>(p.A, p.B, walk.m0 + lane_row + (threadIdx.x & 31), walk.n0 + half + c, walk.k0, walk.k1);
+                                    row[c] = plain_product<T, A_ALONG_K, B_ALONG_K>(p.A, p.B, walk.m0 + lane_row + (threadIdx.x & 31), walk.n0 + first + c, walk.k0, walk.k1);
                         }
                         __syncwarp();
                     }
 #pragma unroll 1
-                    for (int c = 0; c < HALF; c += 32) put(piece + c, c);
+                    for (int c = 0; c < COLUMNS; c += 32) put(piece + c, c);
                     __syncwarp();      // the tile has been read
                 } else {
-                    const unsigned set = chunk & 1, at = accumulators + ((unsigned)lane_row << 16) + set * S::SET + half;
+                    const unsigned set = chunk & 1, at = accumulators + ((unsigned)lane_row << 16) + set * S::SET + first;
                     ended = ended && barrier_wait(done + 8 * set, (chunk >> 1) & 1);
                     ++chunk;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                    for (int c = 0; c < HALF && c < width; c += 32) {
-                        float v[32];
-                        load_accumulators(at + c, v);
-                        __syncwarp();      // the piece before has been read
+                    for (int c = 0; c < COLUMNS; c += 32) {
+                        if (c < width) {
+                            float v[32];
+                            load_accumulators(at + c, v);
+                            __syncwarp();      // the piece before has been read
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                            if (!ended) w = make_float4(NAN, NAN, NAN, NAN);
-                            *reinterpret_cast<float4 *>(row + i) = w;
+                            for (int i = 0; i < 32; i += 4) {
+                                float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                                if (!ended) w = make_float4(NAN, NAN, NAN, NAN);
+                                *reinterpret_cast<float4 *>(row + i) = w;
+                            }
+                            __syncwarp();
+                            put(piece, c);
                         }
-                        __syncwarp();
-                        put(piece, c);
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
@@ -472,7 +492,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                 }
             }
         });
-    } else if (threadIdx.x == kOutWarps * 32) {
+    } else if (threadIdx.x == OUT * 32) {
         // Issues the matrix instructions.
         constexpr unsigned TYPE = std::is_same_v<T, __half> ? 0 : 1;
         bool ended = true;
@@ -514,7 +534,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             }
         }
         mma_commit(last);
-    } else if (threadIdx.x == (kOutWarps + 1) * 32) {
+    } else if (threadIdx.x == (OUT + 1) * 32) {
         // Issues the copies.
         bool ended = true;
         unsigned step = 0;
@@ -546,10 +566,10 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             }
         if (!ended)      // copies in flight land before the block goes
             for (unsigned back = 1; back <= (unsigned)S::STAGES && back <= step; ++back) barrier_wait(full + 8 * ((step - back) % S::STAGES), ((step - back) / S::STAGES) & 1);
-    } else if (BRING != kCopied && warp >= kOutWarps + 2) {
+    } else if (BRING != kCopied && warp >= OUT + 2) {
         // Bring what goes through registers, DEPTH steps ahead.
         constexpr int DEPTH = BRING == kImage ? 3 : sizeof(T) == 4 ? 2 : 1;      // by the registers that a step takes: 16, 32, 48
-        const int thread = threadIdx.x - kBringFrom;
+        const int thread = threadIdx.x - kBringFrom<BRING>;
         Share<T, S::ROWS, A_ALONG_K> a(p.A, thread);
         Share<T, S::BN, B_ALONG_K> b(p.B, thread);
         typename decltype(a)::Eights va[DEPTH];
@@ -606,7 +626,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
     barrier_wait(last, 0);      // no matrix instruction is in flight
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == kOutWarps) {
+    if (warp == OUT) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(accumulators), "n"(2 * S::SET));
     }
@@ -661,10 +681,11 @@ int launch_product_tiles(const Operand<T> &A, const Operand<T> &B, int M, int N,
         image_kernel<T, B_ALONG_K><<<dim3(blocks, S::BN * S::KS / 8 / 256), 256, 0, st>>>(B, N, K, (char *)image);
         DRONE_LAUNCH_CHECK("image_kernel");
     }
+    constexpr int bytes = S::shared(kOutWarps<BRING>);
     auto *const kernel = product_tile_kernel<T, BRING, A_ALONG_K, B_ALONG_K>;
-    DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SHARED));
+    DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     const long long tiles = (long long)ceil_div(M, S::ROWS) * ceil_div(N, S::BN) * shares;
-    kernel<<<(unsigned)std::min<long long>(tiles, sms), kBringFrom + (BRING == kCopied ? 0 : kBringThreads), S::SHARED, st>>>(p);
+    kernel<<<(unsigned)std::min<long long>(tiles, sms), kProductThreads<BRING>, bytes, st>>>(p);
     DRONE_LAUNCH_CHECK("product_tile_kernel");
     return DRONE_OK;
 }
