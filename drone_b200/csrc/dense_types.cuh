@@ -71,14 +71,12 @@ __device__ __forceinline__ float reciprocal_fast(float x) {      // one unit in 
     return y;
 }
 
-// Phi(z), the normal distribution's, and exp(-z^2 / 2), for results of 16 bits: Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7 of 1 against
+// 1 - Phi(|z|), of the normal distribution, and exp(-z^2 / 2), for results of 16 bits: Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7 of 1 against
 // the 2^-11 or 2^-8 of a value that the rounding leaves; a dozen instructions where erff and expf take fifty.
-__device__ __forceinline__ float normal_fast(float z, float *bell) {
-    const float x = fabsf(z) * 0.70710678f, t = reciprocal_fast(fmaf(0.3275911f, x, 1.f));
-    *bell = exp2_fast(x * x * -1.44269504f);
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * poly * *bell;      // Phi(-|z|)
-    return z < 0.f ? tail : 1.f - tail;
+__device__ __forceinline__ float normal_tail(float z, float *bell) {
+    const float t = reciprocal_fast(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+    *bell = exp2_fast(z * -0.72134752f * z);
+    return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f) * *bell;
 }
 
 // z -> activation(z) and its derivative, for values of type T.  A NaN stays one, also in the ReLU (max(NaN, 0) would be 0).
@@ -87,8 +85,10 @@ __device__ __forceinline__ float activate(float z) {
     if constexpr (ACTIVATION == DRONE_ACT_RELU) {
         return z < 0.f ? 0.f : z;
     } else if constexpr (ACTIVATION == DRONE_ACT_GELU) {
+        if (sizeof(T) == 4) return 0.5f * z * (1.f + erff(z * 0.70710678f));
         float bell;
-        return sizeof(T) == 4 ? 0.5f * z * (1.f + erff(z * 0.70710678f)) : z * normal_fast(z, &bell);
+        const float tail = normal_tail(z, &bell);
+        return fmaf(-fabsf(z), tail, z < 0.f ? 0.f : z);      // z Phi(z), of either sign; a NaN is the tail's
     } else if constexpr (ACTIVATION == DRONE_ACT_SILU) {
         return sizeof(T) == 4 ? z / (1.f + expf(-z)) : z * reciprocal_fast(1.f + exp2_fast(z * -1.44269504f));
     } else {
@@ -102,8 +102,8 @@ __device__ __forceinline__ float activation_slope(float z) {
     } else if constexpr (ACTIVATION == DRONE_ACT_GELU) {
         if (sizeof(T) == 4) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
         float bell;
-        const float phi = normal_fast(z, &bell);
-        return fmaf(z * 0.39894228f, bell, phi);
+        const float tail = normal_tail(z, &bell);
+        return fmaf(z * 0.39894228f, bell, z < 0.f ? tail : 1.f - tail);
     } else if constexpr (ACTIVATION == DRONE_ACT_SILU) {
         const float p = sizeof(T) == 4 ? 1.f / (1.f + expf(-z)) : reciprocal_fast(1.f + exp2_fast(z * -1.44269504f));
         return p * (1.f + z * (1.f - p));

@@ -6,21 +6,24 @@
 
 namespace drone {
 
-// Shares of a product, added in order.  A block has 32 values, its warps every eighth share.
-template <typename T>
+// Shares of a product, added in order.  A block has 256 / WAYS values, its parts every WAYS-th share: all of them for a thread where they are few.
+template <typename T, int WAYS>
 __global__ void __launch_bounds__(256) add_product_shares_kernel(const float *__restrict__ parts, int shares, int M, int N, T *__restrict__ out, long long ld) {
-    __shared__ double of_warp[8][32];
-    const long long count = (long long)M * N, i = blockIdx.x * 32LL + (threadIdx.x & 31);
-    const int w = threadIdx.x >> 5;
+    constexpr int VALUES = 256 / WAYS;
+    __shared__ double of_part[WAYS][VALUES];
+    const long long count = (long long)M * N, i = (long long)blockIdx.x * VALUES + threadIdx.x % VALUES;
+    const int w = threadIdx.x / VALUES;
     double sum = 0;
     if (i < count) {
-#pragma unroll 4
-        for (int s = w; s < shares; s += 8) sum += __ldg(parts + s * count + i);
+#pragma unroll 8
+        for (int s = w; s < shares; s += WAYS) sum += __ldg(parts + s * count + i);
     }
-    of_warp[w][threadIdx.x & 31] = sum;
-    __syncthreads();
+    if (WAYS > 1) {
+        of_part[w][threadIdx.x % VALUES] = sum;
+        __syncthreads();
+    }
     if (w == 0 && i < count) {
-        for (int o = 1; o < 8; ++o) sum += of_warp[o][threadIdx.x];
+        for (int o = 1; o < WAYS; ++o) sum += of_part[o][threadIdx.x];
         out[i / N * ld + i % N] = from_float<T>((float)sum);
     }
 }
@@ -278,7 +281,9 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
             return launch_product_tiles<T, kThrough, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
         }();
         if (launched) return launched;
-        add_product_shares_kernel<T><<<ceil_div((long long)rows * columns, 32), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
+        const long long values = (long long)rows * columns;
+        if (s.count <= 32) add_product_shares_kernel<T, 1><<<ceil_div(values, 256), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
+        else add_product_shares_kernel<T, 8><<<ceil_div(values, 32), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
         DRONE_LAUNCH_CHECK("add_product_shares_kernel");
         return DRONE_OK;
     });

@@ -104,114 +104,129 @@ struct SharedLayout {
     }
 };
 
-// Eight values side by side, of which `live` exist (the others are 0).
-__device__ __forceinline__ void load_eight(const float *p, int live, int bytes, float (&v)[8]) {
-    if (live >= 8) {
-        if (bytes == 16) {
-            const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else if (bytes == 8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 a = __ldg((const float2 *)p + i);
-                v[2 * i] = a.x, v[2 * i + 1] = a.y;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __ldg(p + i);
+// V values side by side, of which `live` exist (the others are 0); `bytes` can be read at once.
+template <int V>
+__device__ __forceinline__ void load_values(const float *p, int live, int bytes, float *v) {
+    if constexpr (V == 4) {
+        float4 a = make_float4(0, 0, 0, 0);
+        if (live >= 4) {
+            a = __ldg((const float4 *)p);
+        } else if (live > 0) {
+            a.x = __ldg(p);
+            if (live > 1) a.y = __ldg(p + 1);
+            if (live > 2) a.z = __ldg(p + 2);
         }
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < live ? __ldg(p + i) : 0.f;
+        float2 a = make_float2(0, 0);
+        if (live >= 2 && bytes >= 8) {
+            a = __ldg((const float2 *)p);
+        } else {
+            if (live > 0) a.x = __ldg(p);
+            if (live > 1) a.y = __ldg(p + 1);
+        }
+        v[0] = a.x, v[1] = a.y;
     }
 }
 // 16-bit values in pairs
-template <typename T>
-__device__ __forceinline__ void load_eight(const T *p, int live, int bytes, unsigned (&v)[4]) {
-    if (live >= 8 && bytes >= 4) {
-        if (bytes == 16) {
-            const uint4 a = __ldg((const uint4 *)p);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        } else if (bytes == 8) {
-            const uint2 a = __ldg((const uint2 *)p), b = __ldg((const uint2 *)p + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __ldg((const unsigned *)p + i);
-        }
+template <int V, typename T>
+__device__ __forceinline__ void load_values(const T *p, int live, int bytes, unsigned *v) {
+    const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+    if (V == 8 && live >= 8) {
+        const uint4 a = __ldg((const uint4 *)p);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    } else if (V == 2 && live >= 2 && bytes >= 4) {
+        v[0] = __ldg((const unsigned *)p);
     } else {
-        const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned lo = 2 * i < live ? __ldg(q + 2 * i) : 0, hi = 2 * i + 1 < live ? __ldg(q + 2 * i + 1) : 0;
-            v[i] = lo | hi << 16;
+        for (int i = 0; i < V / 2; ++i) {
+            const unsigned low = 2 * i < live ? __ldg(q + 2 * i) : 0, high = 2 * i + 1 < live ? __ldg(q + 2 * i + 1) : 0;
+            v[i] = low | high << 16;
         }
     }
 }
 
-__device__ __forceinline__ void store_shared(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+template <int WORDS>
+__device__ __forceinline__ void store_shared(unsigned at, const unsigned *v) {
+    if constexpr (WORDS == 1) asm volatile("st.shared.b32 [%0], %1;" :: "r"(at), "r"(v[0]) : "memory");
+    else if constexpr (WORDS == 2) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" :: "r"(at), "r"(v[0]), "r"(v[1]) : "memory");
+    else asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 __device__ __forceinline__ unsigned bf16_pair(float low, float high) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(low, high);
     return reinterpret_cast<const unsigned &>(p);
 }
-__device__ __forceinline__ void split_eight(const float (&v)[8], uint4 (&planes)[3]) {
-    unsigned h[4], m[4], l[4];
+// Pairs of floats in three pairs of bfloat16.
+template <int V>
+__device__ __forceinline__ void split_values(const float *v, unsigned (&planes)[3][V / 2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < V / 2; ++i) {
         float a = v[2 * i], b = v[2 * i + 1];
-        h[i] = bf16_pair(a, b);
-        a -= __uint_as_float(h[i] << 16), b -= __uint_as_float(h[i] & 0xffff0000u);
-        m[i] = bf16_pair(a, b);
-        a -= __uint_as_float(m[i] << 16), b -= __uint_as_float(m[i] & 0xffff0000u);
-        l[i] = bf16_pair(a, b);
-    }
-    planes[0] = make_uint4(h[0], h[1], h[2], h[3]);
-    planes[1] = make_uint4(m[0], m[1], m[2], m[3]);
-    planes[2] = make_uint4(l[0], l[1], l[2], l[3]);
-}
-__device__ __forceinline__ void store_eight(unsigned at, unsigned plane_bytes, const float (&v)[8]) {
-    uint4 planes[3];
-    split_eight(v, planes);
 #pragma unroll
-    for (int q = 0; q < 3; ++q) store_shared(at + q * plane_bytes, planes[q].x, planes[q].y, planes[q].z, planes[q].w);
+        for (int q = 0; q < 3; ++q) {
+            const unsigned pair = planes[q][i] = bf16_pair(a, b);
+            a -= __uint_as_float(pair << 16), b -= __uint_as_float(pair & 0xffff0000u);
+        }
+    }
 }
-__device__ __forceinline__ void store_eight(unsigned at, unsigned, const unsigned (&v)[4]) { store_shared(at, v[0], v[1], v[2], v[3]); }
+template <int V>
+__device__ __forceinline__ void store_values(unsigned at, unsigned plane_bytes, const float *v) {
+    unsigned planes[3][V / 2];
+    split_values<V>(v, planes);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) store_shared<V / 2>(at + q * plane_bytes, planes[q]);
+}
+template <int V>
+__device__ __forceinline__ void store_values(unsigned at, unsigned, const unsigned *v) { store_shared<V / 2>(at, v); }
 
-// What a thread brings of an operand's tile in each step: UNITS times eight values.
+// What a thread brings of an operand's tile in each step.  Neighbouring threads have neighbouring values: 16 bytes each where rows allow it,
+// else pairs (lanes with 32 bytes each of rows that are not on 16 bytes touch four times the lines with every load).
 template <typename T, int R, bool ALONG_K>
 struct Share {
     using S = TileShape<T>;
     using L = SharedLayout<S::KS, ALONG_K>;
-    static constexpr int ACROSS = (ALONG_K ? S::KS : R) / 8;                                   // units of a row
-    static constexpr int UNITS = R * S::KS / 8 / kBringThreads, STEP = kBringThreads / ACROSS;   // rows between a thread's units
+    static constexpr int WIDTH = ALONG_K ? S::KS : R, VALUES = R * S::KS / kBringThreads, MOST = 16 / sizeof(T);
     static constexpr unsigned PLANE = R * S::KS * 2;
-    using Eight = std::conditional_t<sizeof(T) == 4, float[8], unsigned[4]>;
-    struct Eights { Eight v[UNITS]; };
+    using Word = std::conditional_t<sizeof(T) == 4, float, unsigned>;
+    struct Values { Word v[VALUES * sizeof(T) / 4]; };
     Operand<T> from;
-    int row, unit;
+    int row, column, rows_apart;      // of the thread's first values, and to its next
     const T *at = nullptr;
-    int limit = 0, k = 0;      // rows or columns of the tile that exist; of K until the share's end
+    int limit = 0, k = 0;             // rows or columns of the tile that exist; of K until the share's end
 
-    __device__ Share(const Operand<T> &o, int thread) : from(o), row(thread / ACROSS), unit(thread % ACROSS) {}
+    __device__ Share(const Operand<T> &o, int thread) : from(o) {
+        const int v = o.bytes == 16 ? MOST : 2;
+        row = thread / (WIDTH / v), column = thread % (WIDTH / v) * v, rows_apart = kBringThreads / (WIDTH / v);
+    }
     __device__ void begin(long long start, int size, int k0, int k1) {
-        at = ALONG_K ? from.at + (start + row) * from.ld + k0 + unit * 8 : from.at + (long long)(k0 + row) * from.ld + start + unit * 8;
+        at = ALONG_K ? from.at + (start + row) * from.ld + k0 + column : from.at + (long long)(k0 + row) * from.ld + start + column;
         limit = size, k = k1 - k0;
     }
-    __device__ void load(Eights &to) {
+    template <int V>
+    __device__ void load_each(Values &to) {
+        const T *p = at;
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const int r = row + u * STEP;
+        for (int u = 0; u < VALUES / V; ++u, p += rows_apart * from.ld) {
+            const int r = row + u * rows_apart;
             const bool in_row = ALONG_K ? r < limit : r < k;
-            load_eight(at + (long long)(u * STEP) * from.ld, in_row ? (ALONG_K ? k : limit) - unit * 8 : 0, from.bytes, to.v[u]);
+            load_values<V>(p, in_row ? (ALONG_K ? k : limit) - column : 0, from.bytes, to.v + u * V * sizeof(T) / 4);
         }
+    }
+    __device__ void load(Values &to) {
+        if (from.bytes == 16) load_each<MOST>(to);
+        else load_each<2>(to);
         k -= S::KS;
         at += ALONG_K ? S::KS : S::KS * from.ld;
     }
-    __device__ void store(unsigned to, const Eights &v) const {
+    template <int V>
+    __device__ void store_each(unsigned to, const Values &v) const {
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) store_eight(to + L::offset(row + u * STEP, unit), PLANE, v.v[u]);
+        for (int u = 0; u < VALUES / V; ++u)
+            store_values<V>(to + L::offset(row + u * rows_apart, column >> 3) + (column & 7) * 2, PLANE, v.v + u * V * sizeof(T) / 4);
+    }
+    __device__ void store(unsigned to, const Values &v) const {
+        if (from.bytes == 16) store_each<MOST>(to, v);
+        else store_each<2>(to, v);
     }
 };
 
@@ -306,10 +321,31 @@ struct ProductArgs {
     LinearOut<T> out;
 };
 
+// The residual of 32 x 32 values: of 16-bit ones read before the accumulators are waited for, of floats (32 registers) when it is added.
+template <typename T>
+struct Residual {
+    static constexpr bool AHEAD = sizeof(T) == 2;
+    uint2 v[AHEAD ? 8 : 1];
+    __device__ __forceinline__ void read(const LinearOut<T> &out, long long row0, int rows, int col0, int width) {
+        const int lane = threadIdx.x & 31, c = (lane & 7) * 4;
+        if (!AHEAD || !out.fours || !out.residual || c >= width) return;
+        const T *from = out.residual + (row0 + (lane >> 3)) * out.ldr + col0 + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((lane >> 3) + i * 4 < rows) v[AHEAD ? i : 0] = *reinterpret_cast<const uint2 *>(from + (long long)(i * 4) * out.ldr);
+    }
+    __device__ __forceinline__ Values<T, 4> at(const LinearOut<T> &out, int i, long long row, int column) const {
+        Values<T, 4> x = {};
+        if constexpr (AHEAD) memcpy(&x, &v[i], 8);
+        else if (out.residual) x = *reinterpret_cast<const Values<T, 4> *>(out.residual + row * out.ldr + column);
+        return x;
+    }
+};
+
 // 32 x 32 values of a finished tile, of which the warp has written a row a lane to shared memory, to the outputs with neighbouring columns in
 // neighbouring lanes.
 template <typename T, int PITCH, int ACTIVATION>
-__device__ __forceinline__ void put_piece(const LinearOut<T> &out, const float *piece, long long row0, int rows, int col0, int width) {
+__device__ __forceinline__ void put_piece(const LinearOut<T> &out, const float *piece, const Residual<T> &residual, long long row0, int rows, int col0, int width) {
     const int lane = threadIdx.x & 31;
     if (out.fours) {
         using Four = Values<T, 4>;
@@ -317,14 +353,15 @@ __device__ __forceinline__ void put_piece(const LinearOut<T> &out, const float *
         if (c >= width) return;
         float4 b = make_float4(0, 0, 0, 0);
         if (out.bias) b = __ldg((const float4 *)(out.bias + col0 + c));
-#pragma unroll 4
-        for (int r = lane >> 3; r < rows; r += 4) {
+#pragma unroll(Residual<T>::AHEAD ? 8 : 2)
+        for (int i8 = 0; i8 < 8; ++i8) {
+            const int r = (lane >> 3) + i8 * 4;
+            if (r >= rows) break;
             const long long row = row0 + r;
-            Four x = {}, y;
-            if (out.residual) x = *reinterpret_cast<const Four *>(out.residual + row * out.ldr + col0 + c);
+            Four y;
             const float4 acc = *reinterpret_cast<const float4 *>(piece + r * PITCH + c);
             float z[4] = {acc.x + b.x, acc.y + b.y, acc.z + b.z, acc.w + b.w}, w[4], added[4];
-            x.get(added);
+            residual.at(out, i8, row, col0 + c).get(added);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 w[i] = activate<T, ACTIVATION>(z[i]);
@@ -357,6 +394,7 @@ __global__ void __launch_bounds__(kProductThreads<BRING>, 1)
 product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_ALONG_K> p) {
     using S = TileShape<T>;
     constexpr int OUT = kOutWarps<BRING>;
+    constexpr bool SHARES = !A_ALONG_K;      // a weight gradient, in shares of K; else everything goes through the epilogue
     constexpr bool B_SHARED_ALONG_K = BRING == kImage || B_ALONG_K;
     using LA = SharedLayout<S::KS, A_ALONG_K>;
     using LB = SharedLayout<S::KS, B_SHARED_ALONG_K>;
@@ -398,7 +436,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         float *const row = piece + (threadIdx.x & 31) * S::PITCH;      // this lane's
         bool ended = true;      // no wait was given up
         unsigned chunk = 0;     // of the block, over all tiles
-        with_activation(p.out.activation, [&](auto act) {
+        auto take_out = [&](auto act) {
             constexpr int ACTIVATION = decltype(act)::value;
             // The residual of the tile after the one at work, on its way to L2.
             auto prefetch = [&](const TileWalk &of) {
@@ -413,18 +451,19 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                 const int rows = min(32, walk.rows() - lane_row), width = walk.width() - first;
                 upcoming.next();
                 prefetch(upcoming);
+                const long long row0 = walk.m0 + lane_row;
+                const int col0 = walk.n0 + first;
+                Residual<T> residual;
                 auto put = [&](const float *from, int c) {      // 32 columns from c on
                     if (rows <= 0 || width - c <= 0) return;
-                    const long long row0 = walk.m0 + lane_row;
-                    const int col0 = walk.n0 + first + c, live = min(32, width - c);
-                    if (p.out.shares) {
+                    if constexpr (SHARES) {
                         LinearOut<float> to = {};
                         to.y = p.out.shares + (long long)walk.index * p.M * p.N;
                         to.ldy = p.N;
                         to.fours = p.N % 4 == 0;
-                        put_piece<float, S::PITCH, DRONE_ACT_NONE>(to, from, row0, rows, col0, live);
+                        put_piece<float, S::PITCH, DRONE_ACT_NONE>(to, from, Residual<float>(), row0, rows, col0 + c, min(32, width - c));
                     } else {
-                        put_piece<T, S::PITCH, ACTIVATION>(p.out, from, row0, rows, col0, live);
+                        put_piece<T, S::PITCH, ACTIVATION>(p.out, from, residual, row0, rows, col0 + c, min(32, width - c));
                     }
                 };
                 if constexpr (S::PLANES > 1) {
@@ -473,6 +512,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
 #pragma unroll 1
                     for (int c = 0; c < COLUMNS; c += 32) {
                         if (c < width) {
+                            if (!SHARES) residual.read(p.out, row0, rows, col0 + c, width - c);
                             float v[32];
                             load_accumulators(at + c, v);
                             __syncwarp();      // the piece before has been read
@@ -491,7 +531,9 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                     if ((threadIdx.x & 31) == 0) barrier_arrive(taken + 8 * set);
                 }
             }
-        });
+        };
+        if constexpr (SHARES) take_out(std::integral_constant<int, DRONE_ACT_NONE>());
+        else with_activation(p.out.activation, take_out);
     } else if (threadIdx.x == OUT * 32) {
         // Issues the matrix instructions.
         constexpr unsigned TYPE = std::is_same_v<T, __half> ? 0 : 1;
@@ -572,8 +614,8 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         const int thread = threadIdx.x - kBringFrom<BRING>;
         Share<T, S::ROWS, A_ALONG_K> a(p.A, thread);
         Share<T, S::BN, B_ALONG_K> b(p.B, thread);
-        typename decltype(a)::Eights va[DEPTH];
-        typename decltype(b)::Eights vb[BRING == kThrough ? DEPTH : 1];
+        typename decltype(a)::Values va[DEPTH];
+        typename decltype(b)::Values vb[BRING == kThrough ? DEPTH : 1];
         int s = 0;
         unsigned asked = 0, step = 0;
         auto begin = [&] {
@@ -644,14 +686,11 @@ __global__ void __launch_bounds__(256) image_kernel(Operand<T> B, int N, int K, 
         T v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = n < N && k + e < K ? B.at[B_ALONG_K ? (long long)n * B.ld + k + e : (long long)(k + e) * B.ld + n] : from_float<T>(0.f);
-        uint4 planes[S::PLANES];
-        if constexpr (S::PLANES == 3) {
-            split_eight(v, planes);
-        } else {
-            memcpy(planes, v, 16);
-        }
+        unsigned planes[S::PLANES][4];
+        if constexpr (S::PLANES == 3) split_values<8>(v, planes);
+        else memcpy(planes, v, 16);
 #pragma unroll
-        for (int q = 0; q < S::PLANES; ++q) *reinterpret_cast<uint4 *>(to + q * S::B_PLANE + L::offset(row, unit)) = planes[q];
+        for (int q = 0; q < S::PLANES; ++q) *reinterpret_cast<uint4 *>(to + q * S::B_PLANE + L::offset(row, unit)) = make_uint4(planes[q][0], planes[q][1], planes[q][2], planes[q][3]);
     }
 }
 
