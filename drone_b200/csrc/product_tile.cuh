@@ -104,6 +104,26 @@ struct SharedLayout {
     }
 };
 
+// V values side by side that can be read at once.
+template <int V>
+__device__ __forceinline__ void load_whole(const float *p, float *v) {
+    if constexpr (V == 4) {
+        const float4 a = __ldg((const float4 *)p);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    } else {
+        const float2 a = __ldg((const float2 *)p);
+        v[0] = a.x, v[1] = a.y;
+    }
+}
+template <int V, typename T>
+__device__ __forceinline__ void load_whole(const T *p, unsigned *v) {
+    if constexpr (V == 8) {
+        const uint4 a = __ldg((const uint4 *)p);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    } else {
+        v[0] = __ldg((const unsigned *)p);
+    }
+}
 // V values side by side, of which `live` exist (the others are 0); `bytes` can be read at once.
 template <int V>
 __device__ __forceinline__ void load_values(const float *p, int live, int bytes, float *v) {
@@ -202,19 +222,31 @@ struct Share {
         at = ALONG_K ? from.at + (start + row) * from.ld + k0 + column : from.at + (long long)(k0 + row) * from.ld + start + column;
         limit = size, k = k1 - k0;
     }
-    template <int V>
-    __device__ void load_each(Values &to) {
+    // WHOLE: the step lies inside the operand; its loads follow one another without a condition, so that all of them are in flight
+    template <int V, bool WHOLE>
+    __device__ __forceinline__ void load_each(Values &to) {
         const T *p = at;
 #pragma unroll
         for (int u = 0; u < VALUES / V; ++u, p += rows_apart * from.ld) {
-            const int r = row + u * rows_apart;
-            const bool in_row = ALONG_K ? r < limit : r < k;
-            load_values<V>(p, in_row ? (ALONG_K ? k : limit) - column : 0, from.bytes, to.v + u * V * sizeof(T) / 4);
+            Word *const v = to.v + u * V * sizeof(T) / 4;
+            if constexpr (WHOLE) {
+                load_whole<V>(p, v);
+            } else {
+                const int r = row + u * rows_apart;
+                const bool in_row = ALONG_K ? r < limit : r < k;
+                load_values<V>(p, in_row ? (ALONG_K ? k : limit) - column : 0, from.bytes, v);
+            }
         }
     }
-    __device__ void load(Values &to) {
-        if (from.bytes == 16) load_each<MOST>(to);
-        else load_each<2>(to);
+    __device__ __forceinline__ void load(Values &to) {
+        const bool whole = limit >= R && k >= S::KS;
+        if (from.bytes == 16) {
+            if (whole) load_each<MOST, true>(to);
+            else load_each<MOST, false>(to);
+        } else {
+            if (whole && from.bytes >= 2 * (int)sizeof(T)) load_each<2, true>(to);
+            else load_each<2, false>(to);
+        }
         k -= S::KS;
         at += ALONG_K ? S::KS : S::KS * from.ld;
     }
@@ -408,7 +440,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
-            barrier_init(full + 8 * s, (BRING == kCopied ? 0 : kBringThreads) + (BRING == kThrough ? 0 : 1));
+            barrier_init(full + 8 * s, (BRING == kCopied ? 0 : kBringThreads / 32) + (BRING == kThrough ? 0 : 1));
             barrier_init(empty + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -437,7 +469,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         bool ended = true;      // no wait was given up
         unsigned chunk = 0;     // of the block, over all tiles
         auto take_out = [&](auto act) {
-            constexpr int ACTIVATION = decltype(act)::value;
+            [[maybe_unused]] constexpr int ACTIVATION = decltype(act)::value;
             // The residual of the tile after the one at work, on its way to L2.
             auto prefetch = [&](const TileWalk &of) {
                 const int r = threadIdx.x & 31;
@@ -453,7 +485,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                 prefetch(upcoming);
                 const long long row0 = walk.m0 + lane_row;
                 const int col0 = walk.n0 + first;
-                Residual<T> residual;
+                [[maybe_unused]] Residual<T> residual;
                 auto put = [&](const float *from, int c) {      // 32 columns from c on
                     if (rows <= 0 || width - c <= 0) return;
                     if constexpr (SHARES) {
@@ -543,6 +575,9 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             // float accumulators, both operands of this type, lying along K (0) or not (1), columns / 8, rows / 16
             const unsigned instruction = 1u << 4 | TYPE << 7 | TYPE << 10 | (A_ALONG_K ? 0u : 1u) << 15 | (B_SHARED_ALONG_K ? 0u : 1u) << 16 |
                                          (unsigned)(walk.columns() / 8) << 17 | (unsigned)(S::ROWS / 16) << 24;
+            // Where the tile is full the parts h' and m' of B along K are one operand of twice the columns, as are the accumulators: an instruction of
+            // 128 columns takes as long to read its operands as one of 256.
+            const unsigned both = B_SHARED_ALONG_K && walk.columns() == S::BN ? instruction + ((unsigned)(S::BN / 8) << 17) : 0;
             for (int s = 0; s < walk.steps && ended; ++s, ++step) {
                 const bool begins = s % S::CHUNK == 0;
                 const unsigned set = chunk & 1, to = accumulators + set * S::SET;
@@ -560,12 +595,16 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                     } else {
                         const unsigned long long ah = LA::descriptor(a, k), am = LA::descriptor(a + S::A_PLANE, k), al = LA::descriptor(a + 2 * S::A_PLANE, k);
                         const unsigned long long bh = LB::descriptor(b, k), bm = LB::descriptor(b + S::B_PLANE, k), bl = LB::descriptor(b + 2 * S::B_PLANE, k);
-                        mma(to, ah, bh, instruction, add);
-                        mma(to + S::BN, ah, bl, instruction, add);
-                        mma(to + S::BN, al, bh, instruction, true);
-                        mma(to + S::BN, am, bm, instruction, true);
-                        mma(to + S::BN, ah, bm, instruction, true);
+                        if (both) {      // h h' and h m' at once
+                            mma(to, ah, bh, both, add);
+                        } else {
+                            mma(to, ah, bh, instruction, add);
+                            mma(to + S::BN, ah, bm, instruction, add);
+                        }
                         mma(to + S::BN, am, bh, instruction, true);
+                        mma(to + S::BN, am, bm, instruction, true);
+                        mma(to + S::BN, ah, bl, instruction, true);
+                        mma(to + S::BN, al, bh, instruction, true);
                     }
                 }
                 mma_commit(empty + 8 * stage);
@@ -646,7 +685,8 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             a.store(to, va[D]);
             if constexpr (BRING == kThrough) b.store(to + S::A_BYTES, vb[D]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            barrier_arrive(full + 8 * stage);
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) barrier_arrive(full + 8 * stage);      // 256 arrivals at one barrier would queue
             ++step;
             load(d);
             return true;
