@@ -28,6 +28,68 @@ __global__ void __launch_bounds__(256) add_product_shares_kernel(const float *__
     }
 }
 
+// A few rows: W is read once for up to ROWS of them, by as many warps as there are loads to hide.
+//   W [K, N]: a block has 32 columns, a lane one of them, its 32 warps every 32nd k; the warps' sums are added in order.
+//   W [N, K]: a warp has a column, its lanes every 32nd k.
+constexpr int kFewRows = 8;
+constexpr int kFewRowsUpTo = 8;
+template <typename T, int ACTIVATION>
+__device__ __forceinline__ void put_value(const LinearOut<T> &out, long long row, int c, float z) {
+    if (out.bias) z += __ldg(out.bias + c);
+    if (out.pre) out.pre[row * out.ldp + c] = from_float<T>(z);
+    float v = activate<T, ACTIVATION>(z);
+    if (out.residual) v += to_float(out.residual[row * out.ldr + c]);
+    out.y[row * out.ldy + c] = from_float<T>(v);
+}
+template <typename T, bool TRANSPOSED>
+__global__ void __launch_bounds__(TRANSPOSED ? 256 : 1024) few_rows_kernel(Operand<T> X, Operand<T> W, int n, int N, int K, LinearOut<T> out) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = blockIdx.y * kFewRows, rows = min(kFewRows, n - row0);
+    const T *x = X.at + row0 * X.ld;
+    float acc[kFewRows];
+#pragma unroll
+    for (int r = 0; r < kFewRows; ++r) acc[r] = 0;
+    const int c = TRANSPOSED ? (int)blockIdx.x * 8 + warp : (int)blockIdx.x * 32 + lane;
+    if (c < N) {
+        const T *w = TRANSPOSED ? W.at + c * W.ld : W.at + c;
+        const long long along = TRANSPOSED ? 1 : W.ld;
+        auto add = [&](auto all) {      // rows that do not exist read the last one
+            constexpr int R = decltype(all)::value;
+#pragma unroll(R == 1 ? 8 : 4)
+            for (int k = TRANSPOSED ? lane : warp; k < K; k += 32) {
+                const float v = to_float(w[k * along]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r] = fmaf(to_float(x[(R == 1 ? 0 : min(r, rows - 1)) * X.ld + k]), v, acc[r]);
+            }
+        };
+        if (rows == 1) add(std::integral_constant<int, 1>());
+        else add(std::integral_constant<int, kFewRows>());
+    }
+    if constexpr (TRANSPOSED) {
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+        if (c < N && lane < rows) {
+            float z = 0;
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r) z = lane == r ? acc[r] : z;
+            with_activation(out.activation, [&](auto act) { put_value<T, decltype(act)::value>(out, row0 + lane, c, z); });
+        }
+    } else {
+        __shared__ float of_warp[32][kFewRows][32];
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r)
+            if (r < rows) of_warp[warp][r][lane] = acc[r];
+        __syncthreads();
+        if (warp < rows && c < N) {
+            float z = 0;
+#pragma unroll 8
+            for (int i = 0; i < 32; ++i) z += of_warp[i][warp][lane];
+            with_activation(out.activation, [&](auto act) { put_value<T, decltype(act)::value>(out, row0 + warp, c, z); });
+        }
+    }
+}
+
 int tile_map(CUtensorMap *map, bool bf16, const void *p, long long width, long long rows, long long ld, int box) {
     using Encode = decltype(&cuTensorMapEncodeTiled);
     static const Encode encode = [] {
@@ -71,29 +133,32 @@ activation_gradient_kernel(const T *G, long long ldg, const T *pre, long long ld
     if (sums) S::add_groups(sum, F, gl, sums + (long long)blockIdx.x * N + c0);
 }
 
-// A block has 32 of the columns, its warps every eighth of the sums.
-__global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ sums, int blocks, int columns, float *a, int split, float *b) {
-    __shared__ double of_warp[8][32];
+// A block has 32 of the columns, its 32 warps every 32nd of the sums (with 8 warps 888 blocks' sums of 128 columns took 20 us).
+__global__ void __launch_bounds__(1024) fold_columns_kernel(const float *__restrict__ sums, int blocks, int columns, float *a, int split, float *b) {
+    __shared__ double of_warp[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
     double sum = 0;
     if (c < columns) {
-#pragma unroll 4
-        for (int i = w; i < blocks; i += 8) sum += __ldg(sums + (long long)i * columns + c);
+#pragma unroll 8
+        for (int i = w; i < blocks; i += 32) sum += __ldg(sums + (long long)i * columns + c);
     }
-    of_warp[w][threadIdx.x & 31] = sum;
+    of_warp[threadIdx.x & 31][w] = sum;
     __syncthreads();
-    if (w == 0 && c < columns) {
-        for (int i = 1; i < 8; ++i) sum += of_warp[i][threadIdx.x];
-        if (c < split) {
-            if (a) a[c] = (float)sum;
+    sum = of_warp[w][threadIdx.x & 31];      // a warp a column
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int column = blockIdx.x * 32 + w;
+    if ((threadIdx.x & 31) == 0 && column < columns) {
+        if (column < split) {
+            if (a) a[column] = (float)sum;
         } else if (b) {
-            b[c - split] = (float)sum;
+            b[column - split] = (float)sum;
         }
     }
 }
 
 int fold_columns(const float *sums, int blocks, int columns, float *a, int split, float *b, cudaStream_t st) {
-    fold_columns_kernel<<<ceil_div(columns, 32), 256, 0, st>>>(sums, blocks, columns, a, split, b);
+    fold_columns_kernel<<<ceil_div(columns, 32), 1024, 0, st>>>(sums, blocks, columns, a, split, b);
     DRONE_LAUNCH_CHECK("fold_columns_kernel");
     return DRONE_OK;
 }
@@ -147,7 +212,7 @@ extern "C" {
 
 int drone_linear_scratch(int type, int n_rows, int K, int N, long long *n_floats) {
     DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && n_floats, "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d", type, n_rows, K, N);
-    *n_floats = n_rows == 0 ? 0 : type == DRONE_F32 ? image_floats<float>(K, N) : image_floats<__half>(K, N);
+    *n_floats = n_rows <= kFewRowsUpTo ? 0 : type == DRONE_F32 ? image_floats<float>(K, N) : image_floats<__half>(K, N);
     return DRONE_OK;
 }
 
@@ -165,7 +230,7 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
     long long need = 0;
     int sms = 0, rc = drone_linear_scratch(type, n_rows, K, N, &need);
     if (rc) return rc;
-    DRONE_REQUIRE(n_scratch >= need && d_scratch && (reinterpret_cast<uintptr_t>(d_scratch) & 15) == 0,
+    DRONE_REQUIRE(need == 0 || (n_scratch >= need && d_scratch && (reinterpret_cast<uintptr_t>(d_scratch) & 15) == 0),
                   "drone_linear: %lld floats of scratch on 16 bytes needed, %lld at %p given", need, n_scratch, (void *)d_scratch);
     rc = device_sms(&sms);
     if (rc) return rc;
@@ -176,6 +241,13 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
         const bool in_fours = N % 4 == 0 && (reinterpret_cast<uintptr_t>(d_bias) & 15) == 0 && fours(d_Y, ldy) && fours(d_residual, ldr) && fours(d_pre, ldp);
         const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr, in_fours};
         const Operand<T> x = operand<T>(d_X, ldx), w = operand<T>(d_W, ldw);
+        if (n_rows <= kFewRowsUpTo) {
+            const int groups = ceil_div(n_rows, kFewRows);
+            if (transposed) few_rows_kernel<T, true><<<dim3(ceil_div(N, 8), groups), 256, 0, st>>>(x, w, n_rows, N, K, out);
+            else few_rows_kernel<T, false><<<dim3(ceil_div(N, 32), groups), 1024, 0, st>>>(x, w, n_rows, N, K, out);
+            DRONE_LAUNCH_CHECK("few_rows_kernel");
+            return DRONE_OK;
+        }
         if constexpr (sizeof(T) == 2)
             if (x.bytes == 16 && w.bytes == 16)
                 return transposed ? launch_product_tiles<T, kCopied, true, true>(x, w, n_rows, N, K, K, 1, nullptr, out, sms, st)

@@ -762,7 +762,14 @@ int launch_product_tiles(const Operand<T> &A, const Operand<T> &B, int M, int N,
     }
     constexpr int bytes = S::shared(kOutWarps<BRING>);
     auto *const kernel = product_tile_kernel<T, BRING, A_ALONG_K, B_ALONG_K>;
-    DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    // once a device: the call costs more than the launch's other preparations together
+    static std::atomic<unsigned long long> devices{0};
+    int device = 0;
+    DRONE_CUDA(cudaGetDevice(&device));
+    if (device > 63 || !(devices.load(std::memory_order_relaxed) >> device & 1)) {
+        DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (device <= 63) devices.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
     const long long tiles = (long long)ceil_div(M, S::ROWS) * ceil_div(N, S::BN) * shares;
     kernel<<<(unsigned)std::min<long long>(tiles, sms), kProductThreads<BRING>, bytes, st>>>(p);
     DRONE_LAUNCH_CHECK("product_tile_kernel");

@@ -25,28 +25,36 @@ def _require(condition, message, *values):
 
 def _matrix(name, t, rows=None, width=None, dtype=None, device=None):
     """t's distance between rows, once it is a matrix that the kernels can read or write."""
+    try:
+        (n, f), (apart, step), its = t.shape, t.stride(), t.dtype
+        if ((its in _TYPES if dtype is None else its is dtype) and (t.is_cuda if device is None else t.device == device)
+                and (rows is None or n == rows) and (width is None or f == width) and f >= 1 and (n <= 1 or f <= apart < 1 << 31)
+                and (step == 1 or f == 1 or n == 0) and n <= _MAX_ROWS):
+            return apart if n > 1 else f
+    except (AttributeError, TypeError, ValueError):
+        pass
+    _refuse_matrix(name, t, rows, width, dtype, device)
+
+
+def _refuse_matrix(name, t, rows, width, dtype, device):
     _require(isinstance(t, torch.Tensor) and t.dim() == 2, "%s is not a matrix", name)
     _require(t.is_cuda and (device is None or t.device == device), "%s is on %s, not on %s", name, t.device, device or "a CUDA device")
     _require(t.dtype in _TYPES if dtype is None else t.dtype == dtype, "%s is of %s", name, t.dtype)
     _require((rows is None or t.shape[0] == rows) and (width is None or t.shape[1] == width), "%s is %d x %d where %s x %s are needed", name,
              *t.shape, "any" if rows is None else rows, "any" if width is None else width)
-    n, f = t.shape
-    _require(f >= 1 and n <= _MAX_ROWS, "%s has %d rows of %d", name, n, f)
-    _require(f == 1 or n == 0 or t.stride(1) == 1, "%s has values %d apart in its rows", name, t.stride(1))
-    if n <= 1:
-        return f
-    _require(f <= t.stride(0) < 1 << 31, "%s has rows of %d that are %d apart", name, f, t.stride(0))
-    return t.stride(0)
+    raise ValueError("%s has %d rows of %d values, %d apart, with values %d apart" % (name, *t.shape, *t.stride()))
 
 
 def _vector(name, t, size, dtype, device):
-    _require(isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == (size,) and t.device == device and t.is_contiguous(),
-             "%s is not %d values of %s side by side on %s", name, size, dtype, device)
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (size,) and t.device == device and t.is_contiguous()):
+        raise ValueError("%s is not %d values of %s side by side on %s" % (name, size, dtype, device))
 
 
 def _span(t):
-    last = t.data_ptr() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * t.element_size() + t.element_size()
-    return (t.data_ptr(), last) if t.numel() else (0, 0)
+    if t.numel() == 0:
+        return 0, 0
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
 def _apart(name, out, *others):
@@ -74,23 +82,29 @@ class _Call:
 
     def __init__(self, device):
         self.device = device
-        self.guard = torch.cuda.device(device)
+        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
-        self.guard.__enter__()
+        if self.guard is not None:
+            self.guard.__enter__()
         self.stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        self.lib = lib()
         return self
 
     def __exit__(self, *error):
-        return self.guard.__exit__(*error)
+        if self.guard is not None:
+            self.guard.__exit__(*error)
 
     def __call__(self, name, *args):
-        check(getattr(lib(), name)(*args, self.stream))
+        code = getattr(self.lib, name)(*args, self.stream)
+        if code:
+            check(code)
 
     def scratch(self, name, *sizes):
+        """Scratch for a call of these sizes and its number of floats."""
         floats = C.c_longlong(0)
-        check(getattr(lib(), name)(*sizes, C.byref(floats)))
-        return torch.empty(floats.value, dtype=torch.float32, device=self.device), floats.value
+        check(getattr(self.lib, name)(*sizes, C.byref(floats)))
+        return (torch.empty(floats.value, dtype=torch.float32, device=self.device) if floats.value else None), floats.value
 
 
 def _weights(w, inputs, dtype, device, transposed):
@@ -116,18 +130,20 @@ def linear(x, w, bias=None, activation=None, residual=None, transposed=False, ou
     if bias is not None:
         _vector("the bias", bias, outputs, torch.float32, device)
     act = _activation(activation)
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty((n, outputs), dtype=dtype, device=device)
-    ldy = _matrix("out", out, n, outputs, dtype, device)
+    ldy = outputs if made else _matrix("out", out, n, outputs, dtype, device)
     ldr = _matrix("the residual", residual, n, outputs, dtype, device) if residual is not None else 0
     ldp = _matrix("pre", pre, n, outputs, dtype, device) if pre is not None else 0
-    _apart("out", out, (x, False), (w, False), (bias, False), (residual, True), (pre, False))
+    if not made:
+        _apart("out", out, (x, False), (w, False), (bias, False), (residual, True), (pre, False))
     if pre is not None:
         _apart("pre", pre, (x, False), (w, False), (bias, False), (residual, False))
     with _Call(device) as call:
         image, floats = call.scratch("drone_linear_scratch", _TYPES[dtype], n, x.shape[1], outputs)
         call("drone_linear", _TYPES[dtype], n, x.shape[1], outputs, x.data_ptr(), ldx, w.data_ptr(), ldw, int(flipped), _pointer(bias), act,
-             _pointer(residual), ldr, out.data_ptr(), ldy, _pointer(pre), ldp, image.data_ptr(), floats)
+             _pointer(residual), ldr, out.data_ptr(), ldy, _pointer(pre), ldp, _pointer(image), floats)
     return out
 
 
@@ -177,10 +193,11 @@ def layer_norm(x, scale, shift, eps=1e-5, relu=False, out=None):
     _vector("shift", shift, f, torch.float32, device)
     _require(eps > 0, "eps=%r", eps)
     if out is None:
-        out = torch.empty((n, f), dtype=x.dtype, device=device)
-    ldy = _matrix("out", out, n, f, x.dtype, device)
-    _apart("out", out, (x, True), (scale, False), (shift, False))
-    mean, rstd = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(2))
+        out, ldy = torch.empty((n, f), dtype=x.dtype, device=device), f
+    else:
+        ldy = _matrix("out", out, n, f, x.dtype, device)
+        _apart("out", out, (x, True), (scale, False), (shift, False))
+    mean, rstd = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
     with _Call(device) as call:
         call("drone_layer_norm", _TYPES[x.dtype], n, f, x.data_ptr(), ldx, scale.data_ptr(), shift.data_ptr(), float(eps), int(bool(relu)),
              out.data_ptr(), ldy, mean.data_ptr(), rstd.data_ptr())
@@ -206,7 +223,7 @@ def layer_norm_backward(grad, x, scale, mean, rstd, out=None, mirror_rows=None):
         sums, floats = call.scratch("drone_layer_norm_backward_scratch", _TYPES[dtype], n, f)
         call("drone_layer_norm_backward", _TYPES[dtype], n, f, grad.data_ptr(), ldg, x.data_ptr(), ldx, scale.data_ptr(), mean.data_ptr(),
              rstd.data_ptr(), _pointer(out), ldo, _pointer(mirror_rows), grad_x.data_ptr(), f, grad_scale.data_ptr(), grad_shift.data_ptr(),
-             sums.data_ptr(), floats)
+             _pointer(sums), floats)
     return grad_x, grad_scale, grad_shift
 
 
