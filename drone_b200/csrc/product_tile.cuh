@@ -72,17 +72,20 @@ template <Bring BRING> constexpr int kProductThreads = kBringFrom<BRING> + (BRIN
 __device__ __forceinline__ unsigned shared_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrier_init(unsigned bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); }
 __device__ __forceinline__ void barrier_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
-// Waits for a phase of a barrier, two seconds at most: false if it did not end.
+// Waits for a phase of a barrier, two seconds at most: false if it did not end.  (The clock is looked at every 256 polls: a look takes longer than
+// most waits.)
 __device__ __forceinline__ bool barrier_wait(unsigned bar, unsigned parity) {
     unsigned long long began = 0;
-    for (;;) {
+    for (unsigned polls = 1;; ++polls) {
         unsigned done;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
         if (done) return true;
-        unsigned long long now;
-        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-        if (began == 0) began = now;
-        else if (now - began > 2000000000ull) return false;
+        if ((polls & 255) == 0) {
+            unsigned long long now;
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+            if (began == 0) began = now;
+            else if (now - began > 2000000000ull) return false;
+        }
     }
 }
 
@@ -302,6 +305,13 @@ __device__ __noinline__ float plain_product(Operand<T> A, Operand<T> B, long lon
     return acc;
 }
 
+// One lane of a warp whose lanes go the same way.  (A branch of one thread by its number would leave the compiler without uniform registers, in
+// which these instructions take their operands: a matrix instruction then took about as long to issue as to run.)
+__device__ __forceinline__ bool elected() {
+    unsigned mine;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(mine));
+    return mine != 0;
+}
 __device__ __forceinline__ void expect_bytes(unsigned bar, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
 }
@@ -436,7 +446,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
     char *const shared = bytes + ((1024 - (shared_address(bytes) & 1023)) & 1023);
     const unsigned stages = shared_address(shared), full = shared_address(bars), empty = full + 8 * S::STAGES, done = full + 16 * S::STAGES, taken = done + 16,
                    last = taken + 16;
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);      // the same in all lanes, for the compiler too
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
@@ -566,7 +576,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         };
         if constexpr (SHARES) take_out(std::integral_constant<int, DRONE_ACT_NONE>());
         else with_activation(p.out.activation, take_out);
-    } else if (threadIdx.x == OUT * 32) {
+    } else if (warp == OUT) {
         // Issues the matrix instructions.
         constexpr unsigned TYPE = std::is_same_v<T, __half> ? 0 : 1;
         bool ended = true;
@@ -587,35 +597,36 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                 if (!ended) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned a = stages + stage * S::STAGE, b = a + S::A_BYTES;
+                if (elected()) {
 #pragma unroll
-                for (int k = 0; k < S::KS; k += 16) {
-                    const bool add = !begins || k > 0;
-                    if (S::PLANES == 1) {
-                        mma(to, LA::descriptor(a, k), LB::descriptor(b, k), instruction, add);
-                    } else {
-                        const unsigned long long ah = LA::descriptor(a, k), am = LA::descriptor(a + S::A_PLANE, k), al = LA::descriptor(a + 2 * S::A_PLANE, k);
-                        const unsigned long long bh = LB::descriptor(b, k), bm = LB::descriptor(b + S::B_PLANE, k), bl = LB::descriptor(b + 2 * S::B_PLANE, k);
-                        if (both) {      // h h' and h m' at once
-                            mma(to, ah, bh, both, add);
+                    for (int k = 0; k < S::KS; k += 16) {
+                        const bool add = !begins || k > 0;
+                        if (S::PLANES == 1) {
+                            mma(to, LA::descriptor(a, k), LB::descriptor(b, k), instruction, add);
                         } else {
-                            mma(to, ah, bh, instruction, add);
-                            mma(to + S::BN, ah, bm, instruction, add);
+                            const unsigned long long ah = LA::descriptor(a, k), am = LA::descriptor(a + S::A_PLANE, k), al = LA::descriptor(a + 2 * S::A_PLANE, k);
+                            const unsigned long long bh = LB::descriptor(b, k), bm = LB::descriptor(b + S::B_PLANE, k), bl = LB::descriptor(b + 2 * S::B_PLANE, k);
+                            if (both) {      // h h' and h m' at once
+                                mma(to, ah, bh, both, add);
+                            } else {
+                                mma(to, ah, bh, instruction, add);
+                                mma(to + S::BN, ah, bm, instruction, add);
+                            }
+                            mma(to + S::BN, am, bh, instruction, true);
+                            mma(to + S::BN, am, bm, instruction, true);
+                            mma(to + S::BN, ah, bl, instruction, true);
+                            mma(to + S::BN, al, bh, instruction, true);
                         }
-                        mma(to + S::BN, am, bh, instruction, true);
-                        mma(to + S::BN, am, bm, instruction, true);
-                        mma(to + S::BN, ah, bl, instruction, true);
-                        mma(to + S::BN, al, bh, instruction, true);
                     }
+                    mma_commit(empty + 8 * stage);
+                    if (s + 1 == walk.steps || (s + 1) % S::CHUNK == 0) mma_commit(done + 8 * set);
                 }
-                mma_commit(empty + 8 * stage);
-                if (s + 1 == walk.steps || (s + 1) % S::CHUNK == 0) {
-                    mma_commit(done + 8 * set);
-                    ++chunk;
-                }
+                __syncwarp();
+                if (s + 1 == walk.steps || (s + 1) % S::CHUNK == 0) ++chunk;
             }
         }
-        mma_commit(last);
-    } else if (threadIdx.x == (OUT + 1) * 32) {
+        if (elected()) mma_commit(last);
+    } else if (warp == OUT + 1) {
         // Issues the copies.
         bool ended = true;
         unsigned step = 0;
@@ -628,21 +639,24 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                     if (step >= S::STAGES) ended = barrier_wait(empty + 8 * stage, (step / S::STAGES - 1) & 1);
                     if (!ended) break;
                     const unsigned bar = full + 8 * stage, a = stages + stage * S::STAGE, b = a + S::A_BYTES;
-                    expect_bytes(bar, a_bytes + b_bytes);
-                    if constexpr (BRING == kCopied) {
-                        if (A_ALONG_K) {
-                            copy_tile(a, &p.map_a, k, (int)walk.m0, bar);
+                    if (elected()) {
+                        expect_bytes(bar, a_bytes + b_bytes);
+                        if constexpr (BRING == kCopied) {
+                            if (A_ALONG_K) {
+                                copy_tile(a, &p.map_a, k, (int)walk.m0, bar);
+                            } else {
+                                for (int i = 0; i < S::ROWS / 64; ++i) copy_tile(a + i * (S::KS * 128), &p.map_a, (int)walk.m0 + i * 64, k, bar);
+                            }
+                            if (B_ALONG_K) {
+                                copy_tile(b, &p.map_b, k, walk.n0, bar);
+                            } else {
+                                for (int i = 0; i < pieces; ++i) copy_tile(b + i * (S::KS * 128), &p.map_b, walk.n0 + i * 64, k, bar);
+                            }
                         } else {
-                            for (int i = 0; i < S::ROWS / 64; ++i) copy_tile(a + i * (S::KS * 128), &p.map_a, (int)walk.m0 + i * 64, k, bar);
+                            copy_bytes(b, p.image + ((long long)(walk.n0 / S::BN) * walk.steps + s) * S::B_BYTES, S::B_BYTES, bar);
                         }
-                        if (B_ALONG_K) {
-                            copy_tile(b, &p.map_b, k, walk.n0, bar);
-                        } else {
-                            for (int i = 0; i < pieces; ++i) copy_tile(b + i * (S::KS * 128), &p.map_b, walk.n0 + i * 64, k, bar);
-                        }
-                    } else {
-                        copy_bytes(b, p.image + ((long long)(walk.n0 / S::BN) * walk.steps + s) * S::B_BYTES, S::B_BYTES, bar);
                     }
+                    __syncwarp();
                 }
             }
         if (!ended)      // copies in flight land before the block goes
