@@ -55,13 +55,13 @@ template <typename T> struct TileShape {
     static constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
     static constexpr int ROWS = 128, BN = sizeof(T) == 4 ? 128 : 256;
     static constexpr int KS = sizeof(T) == 4 ? 32 : 64;          // of K in a step
-    static constexpr int STAGES = 3;
+    static constexpr int STAGES = 3;                             // at most
     static constexpr int CHUNK = sizeof(T) == 4 ? 256 / KS : 1 << 30;      // steps until the accumulators are added up
     static constexpr int A_PLANE = ROWS * KS * 2, B_PLANE = BN * KS * 2, A_BYTES = PLANES * A_PLANE, B_BYTES = PLANES * B_PLANE, STAGE = A_BYTES + B_BYTES;
     static constexpr int SET = (sizeof(T) == 4 ? 2 : 1) * BN;    // columns of tensor memory of a set of accumulators, of which there are two
     // floats between the rows on their way out: of a whole tile whose sums are kept there, or of a warp's piece of 32 x 32
     static constexpr int PITCH = sizeof(T) == 4 ? BN + 4 : 36;
-    static constexpr int shared(int out_warps) { return 1024 + STAGES * STAGE + (sizeof(T) == 4 ? ROWS : out_warps * 32) * PITCH * 4; }
+    static constexpr int shared(int stages, int out_warps) { return 1024 + stages * STAGE + (sizeof(T) == 4 ? ROWS : out_warps * 32) * PITCH * 4; }
 };
 // Warps that take tiles out, threads that bring operands.  (17 warps and more leave 96 registers a thread.)
 template <Bring BRING> constexpr int kOutWarps = BRING == kCopied ? 16 : 8;
@@ -184,11 +184,14 @@ template <int V>
 __device__ __forceinline__ void split_values(const float *v, unsigned (&planes)[3][V / 2]) {
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
-        float a = v[2 * i], b = v[2 * i + 1];
+        unsigned a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]);
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
-            const unsigned pair = planes[q][i] = bf16_pair(a, b);
-            a -= __uint_as_float(pair << 16), b -= __uint_as_float(pair & 0xffff0000u);
+            const unsigned pair = planes[q][i] = bf16_pair(__uint_as_float(a), __uint_as_float(b));
+            if (q == 2) break;
+            // what is left of both, in one instruction (the products with -1 are exact)
+            asm("{\n.reg .b64 x, y, m;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nmov.b64 m, 0xbf800000bf800000;\nfma.rn.f32x2 x, y, m, x;\nmov.b64 {%0, %1}, x;\n}"
+                : "+r"(a), "+r"(b) : "r"(pair << 16), "r"(pair & 0xffff0000u));
         }
     }
 }
@@ -213,13 +216,14 @@ struct Share {
     using Word = std::conditional_t<sizeof(T) == 4, float, unsigned>;
     struct Values { Word v[VALUES * sizeof(T) / 4]; };
     Operand<T> from;
-    int row, column, rows_apart;      // of the thread's first values, and to its next
+    template <int V> static constexpr int APART = kBringThreads / (WIDTH / V);      // rows between a thread's values
+    int row, column;                  // of its first
     const T *at = nullptr;
     int limit = 0, k = 0;             // rows or columns of the tile that exist; of K until the share's end
 
     __device__ Share(const Operand<T> &o, int thread) : from(o) {
         const int v = o.bytes == 16 ? MOST : 2;
-        row = thread / (WIDTH / v), column = thread % (WIDTH / v) * v, rows_apart = kBringThreads / (WIDTH / v);
+        row = thread / (WIDTH / v), column = thread % (WIDTH / v) * v;
     }
     __device__ void begin(long long start, int size, int k0, int k1) {
         at = ALONG_K ? from.at + (start + row) * from.ld + k0 + column : from.at + (long long)(k0 + row) * from.ld + start + column;
@@ -230,12 +234,12 @@ struct Share {
     __device__ __forceinline__ void load_each(Values &to) {
         const T *p = at;
 #pragma unroll
-        for (int u = 0; u < VALUES / V; ++u, p += rows_apart * from.ld) {
+        for (int u = 0; u < VALUES / V; ++u, p += APART<V> * from.ld) {
             Word *const v = to.v + u * V * sizeof(T) / 4;
             if constexpr (WHOLE) {
                 load_whole<V>(p, v);
             } else {
-                const int r = row + u * rows_apart;
+                const int r = row + u * APART<V>;
                 const bool in_row = ALONG_K ? r < limit : r < k;
                 load_values<V>(p, in_row ? (ALONG_K ? k : limit) - column : 0, from.bytes, v);
             }
@@ -256,8 +260,12 @@ struct Share {
     template <int V>
     __device__ void store_each(unsigned to, const Values &v) const {
 #pragma unroll
-        for (int u = 0; u < VALUES / V; ++u)
-            store_values<V>(to + L::offset(row + u * rows_apart, column >> 3) + (column & 7) * 2, PLANE, v.v + u * V * sizeof(T) / 4);
+        for (int u = 0; u < VALUES / V; ++u) {
+            // rows 8 apart, and with them all values of a thread but the first, have the same place in the swizzle pattern
+            constexpr bool SAME = APART<V> % 8 == 0;
+            const unsigned at = SAME ? L::offset(row, column >> 3) + u * (L::offset(APART<V>, 0) - L::offset(0, 0)) : L::offset(row + u * APART<V>, column >> 3);
+            store_values<V>(to + at + (column & 7) * 2, PLANE, v.v + u * V * sizeof(T) / 4);
+        }
     }
     __device__ void store(unsigned to, const Values &v) const {
         if (from.bytes == 16) store_each<MOST>(to, v);
@@ -323,6 +331,18 @@ __device__ __forceinline__ void copy_bytes(unsigned to, const void *from, unsign
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" :: "r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
 }
 
+// A block's stages in turn.  The barriers' phases: `filled` ends with the stage's filling at hand, `emptied` with the use before it (there is none
+// before the first: that phase counts as over).
+struct Ring {
+    int stages, stage = 0;
+    unsigned filled = 0;
+    __device__ explicit Ring(int n) : stages(n) {}
+    __device__ unsigned emptied() const { return filled ^ 1; }
+    __device__ void next() {
+        if (++stage == stages) stage = 0, filled ^= 1;
+    }
+};
+
 // The tiles of a block, in turn: columns first, so that blocks at work at the same time share their rows, then rows, then shares of K.
 struct TileWalk {
     int tiles_n, tiles_m, M, N, K, share, bn, ks;
@@ -359,7 +379,7 @@ struct ProductArgs {
     Operand<T> A, B;
     CUtensorMap map_a, map_b;      // kCopied
     const char *image;             // kImage
-    int M, N, K, share, shares;
+    int M, N, K, share, shares, stages;
     LinearOut<T> out;
 };
 
@@ -474,7 +494,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         // Takes tiles out: a quarter of the rows (the lanes of tensor memory that the warp can read) and some of the columns.
         constexpr int COLUMNS = S::BN / (OUT / 4);
         const int lane_row = (warp & 3) * 32, first = (warp >> 2) * COLUMNS;
-        float *const piece = reinterpret_cast<float *>(shared + S::STAGES * S::STAGE) + (S::PLANES > 1 ? lane_row * S::PITCH + first : warp * 32 * S::PITCH);
+        float *const piece = reinterpret_cast<float *>(shared + p.stages * S::STAGE) + (S::PLANES > 1 ? lane_row * S::PITCH + first : warp * 32 * S::PITCH);
         float *const row = piece + (threadIdx.x & 31) * S::PITCH;      // this lane's
         bool ended = true;      // no wait was given up
         unsigned chunk = 0;     // of the block, over all tiles
@@ -580,7 +600,8 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         // Issues the matrix instructions.
         constexpr unsigned TYPE = std::is_same_v<T, __half> ? 0 : 1;
         bool ended = true;
-        unsigned step = 0, chunk = 0;      // of the block, over all tiles
+        Ring ring(p.stages);
+        unsigned chunk = 0;      // of the block, over all tiles
         for (; walk.valid() && ended; walk.next()) {
             // float accumulators, both operands of this type, lying along K (0) or not (1), columns / 8, rows / 16
             const unsigned instruction = 1u << 4 | TYPE << 7 | TYPE << 10 | (A_ALONG_K ? 0u : 1u) << 15 | (B_SHARED_ALONG_K ? 0u : 1u) << 16 |
@@ -588,12 +609,12 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             // Where the tile is full the parts h' and m' of B along K are one operand of twice the columns, as are the accumulators: an instruction of
             // 128 columns takes as long to read its operands as one of 256.
             const unsigned both = B_SHARED_ALONG_K && walk.columns() == S::BN ? instruction + ((unsigned)(S::BN / 8) << 17) : 0;
-            for (int s = 0; s < walk.steps && ended; ++s, ++step) {
+            for (int s = 0; s < walk.steps && ended; ++s, ring.next()) {
                 const bool begins = s % S::CHUNK == 0;
                 const unsigned set = chunk & 1, to = accumulators + set * S::SET;
                 if (begins && chunk >= 2) ended = barrier_wait(taken + 8 * set, ((chunk >> 1) - 1) & 1);
-                const int stage = step % S::STAGES;
-                ended = ended && barrier_wait(full + 8 * stage, (step / S::STAGES) & 1);
+                const int stage = ring.stage;
+                ended = ended && barrier_wait(full + 8 * stage, ring.filled);
                 if (!ended) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned a = stages + stage * S::STAGE, b = a + S::A_BYTES;
@@ -629,15 +650,17 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
     } else if (warp == OUT + 1) {
         // Issues the copies.
         bool ended = true;
-        unsigned step = 0;
+        Ring ring(p.stages);
+        int used = 0;      // stages
         if (BRING != kThrough)
             for (; walk.valid() && ended; walk.next()) {
                 const int pieces = (walk.columns() + 63) / 64;      // of 64 columns, of B along N
                 const unsigned a_bytes = BRING == kCopied ? S::A_BYTES : 0, b_bytes = BRING == kCopied && !B_ALONG_K ? pieces * (S::KS * 128) : S::B_BYTES;
-                for (int s = 0; s < walk.steps; ++s, ++step) {
-                    const int stage = step % S::STAGES, k = walk.k0 + s * S::KS;
-                    if (step >= S::STAGES) ended = barrier_wait(empty + 8 * stage, (step / S::STAGES - 1) & 1);
+                for (int s = 0; s < walk.steps; ++s, ring.next()) {
+                    const int stage = ring.stage, k = walk.k0 + s * S::KS;
+                    ended = barrier_wait(empty + 8 * stage, ring.emptied());
                     if (!ended) break;
+                    used = max(used, stage + 1);
                     const unsigned bar = full + 8 * stage, a = stages + stage * S::STAGE, b = a + S::A_BYTES;
                     if (elected()) {
                         expect_bytes(bar, a_bytes + b_bytes);
@@ -660,7 +683,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                 }
             }
         if (!ended)      // copies in flight land before the block goes
-            for (unsigned back = 1; back <= (unsigned)S::STAGES && back <= step; ++back) barrier_wait(full + 8 * ((step - back) % S::STAGES), ((step - back) / S::STAGES) & 1);
+            for (int stage = 0; stage < used; ++stage) barrier_wait(full + 8 * stage, stage < ring.stage ? ring.filled : ring.emptied());
     } else if (BRING != kCopied && warp >= OUT + 2) {
         // Bring what goes through registers, DEPTH steps ahead.
         constexpr int DEPTH = BRING == kImage ? 3 : sizeof(T) == 4 ? 2 : 1;      // by the registers that a step takes: 16, 32, 48
@@ -671,6 +694,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         typename decltype(b)::Values vb[BRING == kThrough ? DEPTH : 1];
         int s = 0;
         unsigned asked = 0, step = 0;
+        Ring ring(p.stages);
         auto begin = [&] {
             if (!walk.valid()) return;
             a.begin(walk.m0, walk.rows(), walk.k0, walk.k1);
@@ -692,8 +716,8 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         auto store = [&](auto d) {
             constexpr int D = decltype(d)::value;
             if (step == asked || !ended) return false;
-            const int stage = step % S::STAGES;
-            if (step >= S::STAGES) ended = barrier_wait(empty + 8 * stage, (step / S::STAGES - 1) & 1);
+            const int stage = ring.stage;
+            ended = barrier_wait(empty + 8 * stage, ring.emptied());
             if (!ended) return false;
             const unsigned to = stages + stage * S::STAGE;
             a.store(to, va[D]);
@@ -702,6 +726,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             __syncwarp();
             if ((threadIdx.x & 31) == 0) barrier_arrive(full + 8 * stage);      // 256 arrivals at one barrier would queue
             ++step;
+            ring.next();
             load(d);
             return true;
         };
@@ -774,14 +799,17 @@ int launch_product_tiles(const Operand<T> &A, const Operand<T> &B, int M, int N,
         image_kernel<T, B_ALONG_K><<<dim3(blocks, S::BN * S::KS / 8 / 256), 256, 0, st>>>(B, N, K, (char *)image);
         DRONE_LAUNCH_CHECK("image_kernel");
     }
-    constexpr int bytes = S::shared(kOutWarps<BRING>);
+    // Rows that do not start on 16 bytes share lines between neighbouring steps: what two stages leave of an SM's memory is L1 that keeps them.
+    // 232,965 x 602 x 128 floats 278 us with three, 243 with two; 232,965 x 128 x 602, on 16 bytes, 260 and 296.
+    p.stages = BRING == kImage && A.bytes < 16 ? 2 : S::STAGES;
+    const int bytes = S::shared(p.stages, kOutWarps<BRING>);
     auto *const kernel = product_tile_kernel<T, BRING, A_ALONG_K, B_ALONG_K>;
     // once a device: the call costs more than the launch's other preparations together
     static std::atomic<unsigned long long> devices{0};
     int device = 0;
     DRONE_CUDA(cudaGetDevice(&device));
     if (device > 63 || !(devices.load(std::memory_order_relaxed) >> device & 1)) {
-        DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        DRONE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::shared(S::STAGES, kOutWarps<BRING>)));
         if (device <= 63) devices.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     const long long tiles = (long long)ceil_div(M, S::ROWS) * ceil_div(N, S::BN) * shares;
