@@ -104,11 +104,11 @@ def _declare(lib):
         "drone_relu_mask": (i, [i, i, vp, i, vp, i, vp]),
         "drone_weight_gradient_scratch": (i, [i, i, i, C.POINTER(ll)]),
         "drone_weight_gradient": (i, [i, i, i, vp, i, vp, i, vp, vp, ll, vp]),
-        "drone_linear_scratch": (i, [i, i, i, i, C.POINTER(ll)]),
+        "drone_linear_scratch": (i, [i, i, i, i, vp, i, vp, i, i, C.POINTER(ll)]),
         "drone_linear": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, i, vp, i, vp, i, vp, ll, vp]),
         "drone_activation_gradient_scratch": (i, [i, i, i, C.POINTER(ll)]),
         "drone_activation_gradient": (i, [i, i, i, vp, i, vp, i, i, vp, i, vp, vp, ll, vp]),
-        "drone_linear_weight_gradient_scratch": (i, [i, i, i, i, i, C.POINTER(ll)]),
+        "drone_linear_weight_gradient_scratch": (i, [i, i, i, i, vp, i, vp, i, i, C.POINTER(ll)]),
         "drone_linear_weight_gradient": (i, [i, i, i, i, vp, i, vp, i, i, vp, i, vp, ll, vp]),
         "drone_layer_norm": (i, [i, i, i, vp, i, vp, vp, f, i, vp, i, vp, vp, vp]),
         "drone_layer_norm_backward_scratch": (i, [i, i, i, C.POINTER(ll)]),

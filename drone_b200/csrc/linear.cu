@@ -90,6 +90,44 @@ __global__ void __launch_bounds__(TRANSPOSED ? 256 : 1024) few_rows_kernel(Opera
     }
 }
 
+// 16-bit rows to rows that start on 16 bytes: a thread 16 bytes of them.  What lies behind a row's end is never read.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short *__restrict__ from, long long ld, int n, int width, uint4 *__restrict__ to, int vectors) {
+    const bool pairs = (reinterpret_cast<uintptr_t>(from) & 3) == 0 && ld % 2 == 0;
+    for (RowColumn at(blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL, vectors); at.row < n; at.advance()) {
+        const unsigned short *p = from + at.row * ld + at.col * 8;
+        const int live = width - at.col * 8;
+        unsigned v[4];
+        if (pairs && live >= 8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __ldg((const unsigned *)p + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (2 * i < live ? (unsigned)__ldg(p + 2 * i) : 0u) | (2 * i + 1 < live ? (unsigned)__ldg(p + 2 * i + 1) : 0u) << 16;
+        }
+        to[(long long)at.row * vectors + at.col] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+// Floats that the copy of such a matrix takes: none if its rows are on 16 bytes as they are.
+static long long padded_floats(const void *p, long long ld, long long rows, int width) {
+    return rows_on_16_bytes(p, ld, 2) ? 0 : rows * ((width + 7) / 8) * 4;
+}
+// The matrix itself, or its copy at *scratch, which moves on.
+template <typename T>
+static int on_16_bytes(const void *p, long long ld, int rows, int width, float **scratch, int sms, cudaStream_t st, Operand<T> *out) {
+    const long long floats = padded_floats(p, ld, rows, width);
+    if (floats == 0) {
+        *out = operand<T>(p, ld);
+        return DRONE_OK;
+    }
+    const int vectors = (width + 7) / 8;
+    pad_rows_kernel<<<(int)std::min<long long>(((long long)rows * vectors + 255) / 256, sms * 16), 256, 0, st>>>((const unsigned short *)p, ld, rows, width, (uint4 *)*scratch,
+                                                                                                            vectors);
+    DRONE_LAUNCH_CHECK("pad_rows_kernel");
+    *out = operand<T>(*scratch, vectors * 8);
+    *scratch += floats;
+    return DRONE_OK;
+}
+
 int tile_map(CUtensorMap *map, bool bf16, const void *p, long long width, long long rows, long long ld, int box) {
     using Encode = decltype(&cuTensorMapEncodeTiled);
     static const Encode encode = [] {
@@ -180,13 +218,6 @@ static Shares product_shares(int type, int M, int N, int K, int sms) {
     return type == DRONE_F32 ? product_shares<float>(M, N, K, sms) : product_shares<__half>(M, N, K, sms);
 }
 
-// Floats of the image of a product's weights.
-template <typename T>
-static long long image_floats(int K, int N) {
-    using S = TileShape<T>;
-    return (long long)ceil_div(N, S::BN) * ceil_div(K, S::KS) * (S::B_BYTES / 4);
-}
-
 // Blocks of the activations' gradient: as many as the SMs hold, of at most 128 vectors a row.
 struct GradientBlocks {
     int width, columns, rows;      // of a block; blocks along the columns and the rows
@@ -210,9 +241,13 @@ using namespace drone;
 
 extern "C" {
 
-int drone_linear_scratch(int type, int n_rows, int K, int N, long long *n_floats) {
-    DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && n_floats, "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d", type, n_rows, K, N);
-    *n_floats = n_rows <= kFewRowsUpTo ? 0 : type == DRONE_F32 ? image_floats<float>(K, N) : image_floats<__half>(K, N);
+int drone_linear_scratch(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_W, int ldw, int transposed, long long *n_floats) {
+    DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && (transposed == 0 || transposed == 1) && n_floats,
+                  "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d transposed=%d", type, n_rows, K, N, transposed);
+    using S = TileShape<float>;
+    if (n_rows <= kFewRowsUpTo) *n_floats = 0;
+    else if (type == DRONE_F32) *n_floats = (long long)ceil_div(N, S::BN) * ceil_div(K, S::KS) * (S::B_BYTES / 4);      // the image of the weights
+    else *n_floats = padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_W, ldw, transposed ? N : K, transposed ? K : N);
     return DRONE_OK;
 }
 
@@ -228,7 +263,7 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
     DRONE_REQUIRE(DRONE_ALIGNED(d_X, type) && DRONE_ALIGNED(d_W, type) && DRONE_ALIGNED(d_Y, type) && DRONE_ALIGNED(d_residual, type) &&
                   DRONE_ALIGNED(d_pre, type) && (reinterpret_cast<uintptr_t>(d_bias) & 3) == 0, "drone_linear: an operand is not aligned to its type");
     long long need = 0;
-    int sms = 0, rc = drone_linear_scratch(type, n_rows, K, N, &need);
+    int sms = 0, rc = drone_linear_scratch(type, n_rows, K, N, d_X, ldx, d_W, ldw, transposed, &need);
     if (rc) return rc;
     DRONE_REQUIRE(need == 0 || (n_scratch >= need && d_scratch && (reinterpret_cast<uintptr_t>(d_scratch) & 15) == 0),
                   "drone_linear: %lld floats of scratch on 16 bytes needed, %lld at %p given", need, n_scratch, (void *)d_scratch);
@@ -248,12 +283,18 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
             DRONE_LAUNCH_CHECK("few_rows_kernel");
             return DRONE_OK;
         }
-        if constexpr (sizeof(T) == 2)
-            if (x.bytes == 16 && w.bytes == 16)
-                return transposed ? launch_product_tiles<T, kCopied, true, true>(x, w, n_rows, N, K, K, 1, nullptr, out, sms, st)
-                                  : launch_product_tiles<T, kCopied, true, false>(x, w, n_rows, N, K, K, 1, nullptr, out, sms, st);
-        return transposed ? launch_product_tiles<T, kImage, true, true>(x, w, n_rows, N, K, K, 1, d_scratch, out, sms, st)
-                          : launch_product_tiles<T, kImage, true, false>(x, w, n_rows, N, K, K, 1, d_scratch, out, sms, st);
+        if constexpr (sizeof(T) == 2) {
+            Operand<T> a, b;
+            float *scratch = d_scratch;
+            int failed = on_16_bytes(d_X, ldx, n_rows, K, &scratch, sms, st, &a);
+            if (!failed) failed = on_16_bytes(d_W, ldw, transposed ? N : K, transposed ? K : N, &scratch, sms, st, &b);
+            if (failed) return failed;
+            return transposed ? launch_product_tiles<T, kCopied, true, true>(a, b, n_rows, N, K, K, 1, nullptr, out, sms, st)
+                              : launch_product_tiles<T, kCopied, true, false>(a, b, n_rows, N, K, K, 1, nullptr, out, sms, st);
+        } else {
+            return transposed ? launch_product_tiles<T, kImage, true, true>(x, w, n_rows, N, K, K, 1, d_scratch, out, sms, st)
+                              : launch_product_tiles<T, kImage, true, false>(x, w, n_rows, N, K, K, 1, d_scratch, out, sms, st);
+        }
     });
 }
 
@@ -311,14 +352,16 @@ int drone_activation_gradient(int type, int n_rows, int N, const void *d_G, int 
     return d_bias_grad ? fold_columns(d_scratch, b.rows, N, d_bias_grad, N, nullptr, st) : DRONE_OK;
 }
 
-int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, int transposed, long long *n_floats) {
+int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_dZ, int ldz, int transposed,
+                                         long long *n_floats) {
     DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && (transposed == 0 || transposed == 1) && n_floats,
                   "drone_linear_weight_gradient_scratch: type=%d n_rows=%d K=%d N=%d transposed=%d", type, n_rows, K, N, transposed);
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
     const Shares s = product_shares(type, transposed ? N : K, transposed ? K : N, n_rows, sms);
-    *n_floats = (long long)s.count * K * N;
+    *n_floats = n_rows == 0 ? 0 : (long long)s.count * K * N;
+    if (type != DRONE_F32) *n_floats = (*n_floats + 3) / 4 * 4 + padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_dZ, ldz, n_rows, N);
     return DRONE_OK;
 }
 
@@ -341,17 +384,24 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
         return DRONE_OK;
     }
     const Shares s = product_shares(type, rows, columns, n_rows, sms);
-    const long long need = (long long)s.count * K * N;
-    DRONE_REQUIRE(n_scratch >= need && d_scratch, "drone_linear_weight_gradient: %lld floats of scratch, %lld needed", n_scratch, need);
+    long long need = 0;
+    const int sized = drone_linear_weight_gradient_scratch(type, n_rows, K, N, d_X, ldx, d_dZ, ldz, transposed, &need);
+    if (sized) return sized;
+    DRONE_REQUIRE(n_scratch >= need && d_scratch && (reinterpret_cast<uintptr_t>(d_scratch) & 15) == 0,
+                  "drone_linear_weight_gradient: %lld floats of scratch on 16 bytes needed, %lld at %p given", need, n_scratch, (void *)d_scratch);
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
-        const Operand<T> a = transposed ? operand<T>(d_dZ, ldz) : operand<T>(d_X, ldx), b = transposed ? operand<T>(d_X, ldx) : operand<T>(d_dZ, ldz);
+        Operand<T> x = operand<T>(d_X, ldx), dz = operand<T>(d_dZ, ldz);
+        if constexpr (sizeof(T) == 2) {
+            float *scratch = d_scratch + ((long long)s.count * K * N + 3) / 4 * 4;
+            int failed = on_16_bytes(d_X, ldx, n_rows, K, &scratch, sms, st, &x);
+            if (!failed) failed = on_16_bytes(d_dZ, ldz, n_rows, N, &scratch, sms, st, &dz);
+            if (failed) return failed;
+        }
+        const Operand<T> a = transposed ? dz : x, b = transposed ? x : dz;
         const LinearOut<T> out = {nullptr, DRONE_ACT_NONE, nullptr, 0, nullptr, 0, nullptr, 0, d_scratch, false};
-        const int launched = [&] {
-            if constexpr (sizeof(T) == 2)
-                if (a.bytes == 16 && b.bytes == 16) return launch_product_tiles<T, kCopied, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
-            return launch_product_tiles<T, kThrough, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
-        }();
+        constexpr Bring BRING = sizeof(T) == 2 ? kCopied : kThrough;
+        const int launched = launch_product_tiles<T, BRING, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
         if (launched) return launched;
         const long long values = (long long)rows * columns;
         if (s.count <= 32) add_product_shares_kernel<T, 1><<<ceil_div(values, 256), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);

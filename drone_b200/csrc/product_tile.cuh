@@ -2,11 +2,11 @@
 // tensor memory, so that a tile's way to global memory and the next one's products overlap.
 //
 // Its warps: 8 or 16 take finished tiles out (bias, activation, residual), one issues the matrix instructions, one the asynchronous copies, and
-// where an operand needs registers on its way 8 more bring it.  Operands come in one of three ways:
-//   kCopied    both 16-bit and on 16-byte boundaries: tensor copies, tiles lie in shared memory as they do in global memory (along K or not)
-//   kImage     A through registers, from any address (features of 602 or 47 values start anywhere, which no tensor map takes), floats split on
-//              the way; B from an image of it that image_kernel has written, a copy a step
-//   kThrough   both through registers
+// where floats have to be split on their way 8 more bring them.  Operands come in one of three ways:
+//   kCopied    16-bit: tensor copies, tiles lie in shared memory as they do in global memory (along K or not).  Rows that are not on 16 bytes
+//              (features of 602 or 47 values), which no tensor map takes, are copied to rows that are by pad_rows_kernel first
+//   kImage     floats: A through registers, from any address; B from an image of it, split, that image_kernel has written, a copy a step
+//   kThrough   floats: both through registers
 //
 // Floats are split into three bfloat16 of 8 bits each, x = h + m + l exactly (but for values below 2^-110), and six of the nine products are added:
 // h h' in one accumulator, h m' + m h' + m m' + h l' + l h' in a second one that is 2^-8 of it, so that neither loses bits of the other.
@@ -118,15 +118,6 @@ __device__ __forceinline__ void load_whole(const float *p, float *v) {
         v[0] = a.x, v[1] = a.y;
     }
 }
-template <int V, typename T>
-__device__ __forceinline__ void load_whole(const T *p, unsigned *v) {
-    if constexpr (V == 8) {
-        const uint4 a = __ldg((const uint4 *)p);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    } else {
-        v[0] = __ldg((const unsigned *)p);
-    }
-}
 // V values side by side, of which `live` exist (the others are 0); `bytes` can be read at once.
 template <int V>
 __device__ __forceinline__ void load_values(const float *p, int live, int bytes, float *v) {
@@ -151,24 +142,6 @@ __device__ __forceinline__ void load_values(const float *p, int live, int bytes,
         v[0] = a.x, v[1] = a.y;
     }
 }
-// 16-bit values in pairs
-template <int V, typename T>
-__device__ __forceinline__ void load_values(const T *p, int live, int bytes, unsigned *v) {
-    const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
-    if (V == 8 && live >= 8) {
-        const uint4 a = __ldg((const uint4 *)p);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    } else if (V == 2 && live >= 2 && bytes >= 4) {
-        v[0] = __ldg((const unsigned *)p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-            const unsigned low = 2 * i < live ? __ldg(q + 2 * i) : 0, high = 2 * i + 1 < live ? __ldg(q + 2 * i + 1) : 0;
-            v[i] = low | high << 16;
-        }
-    }
-}
-
 template <int WORDS>
 __device__ __forceinline__ void store_shared(unsigned at, const unsigned *v) {
     if constexpr (WORDS == 1) asm volatile("st.shared.b32 [%0], %1;" :: "r"(at), "r"(v[0]) : "memory");
@@ -202,27 +175,24 @@ __device__ __forceinline__ void store_values(unsigned at, unsigned plane_bytes, 
 #pragma unroll
     for (int q = 0; q < 3; ++q) store_shared<V / 2>(at + q * plane_bytes, planes[q]);
 }
-template <int V>
-__device__ __forceinline__ void store_values(unsigned at, unsigned, const unsigned *v) { store_shared<V / 2>(at, v); }
 
 // What a thread brings of an operand's tile in each step.  Neighbouring threads have neighbouring values: 16 bytes each where rows allow it,
 // else pairs (lanes with 32 bytes each of rows that are not on 16 bytes touch four times the lines with every load).
-template <typename T, int R, bool ALONG_K>
+template <int R, bool ALONG_K>
 struct Share {
-    using S = TileShape<T>;
+    using S = TileShape<float>;
     using L = SharedLayout<S::KS, ALONG_K>;
-    static constexpr int WIDTH = ALONG_K ? S::KS : R, VALUES = R * S::KS / kBringThreads, MOST = 16 / sizeof(T);
+    static constexpr int WIDTH = ALONG_K ? S::KS : R, VALUES = R * S::KS / kBringThreads;
     static constexpr unsigned PLANE = R * S::KS * 2;
-    using Word = std::conditional_t<sizeof(T) == 4, float, unsigned>;
-    struct Values { Word v[VALUES * sizeof(T) / 4]; };
-    Operand<T> from;
+    struct Values { float v[VALUES]; };
+    Operand<float> from;
     template <int V> static constexpr int APART = kBringThreads / (WIDTH / V);      // rows between a thread's values
     int row, column;                  // of its first
-    const T *at = nullptr;
+    const float *at = nullptr;
     int limit = 0, k = 0;             // rows or columns of the tile that exist; of K until the share's end
 
-    __device__ Share(const Operand<T> &o, int thread) : from(o) {
-        const int v = o.bytes == 16 ? MOST : 2;
+    __device__ Share(const Operand<float> &o, int thread) : from(o) {
+        const int v = o.bytes == 16 ? 4 : 2;
         row = thread / (WIDTH / v), column = thread % (WIDTH / v) * v;
     }
     __device__ void begin(long long start, int size, int k0, int k1) {
@@ -232,10 +202,10 @@ struct Share {
     // WHOLE: the step lies inside the operand; its loads follow one another without a condition, so that all of them are in flight
     template <int V, bool WHOLE>
     __device__ __forceinline__ void load_each(Values &to) {
-        const T *p = at;
+        const float *p = at;
 #pragma unroll
         for (int u = 0; u < VALUES / V; ++u, p += APART<V> * from.ld) {
-            Word *const v = to.v + u * V * sizeof(T) / 4;
+            float *const v = to.v + u * V;
             if constexpr (WHOLE) {
                 load_whole<V>(p, v);
             } else {
@@ -248,10 +218,10 @@ struct Share {
     __device__ __forceinline__ void load(Values &to) {
         const bool whole = limit >= R && k >= S::KS;
         if (from.bytes == 16) {
-            if (whole) load_each<MOST, true>(to);
-            else load_each<MOST, false>(to);
+            if (whole) load_each<4, true>(to);
+            else load_each<4, false>(to);
         } else {
-            if (whole && from.bytes >= 2 * (int)sizeof(T)) load_each<2, true>(to);
+            if (whole && from.bytes >= 8) load_each<2, true>(to);
             else load_each<2, false>(to);
         }
         k -= S::KS;
@@ -264,11 +234,11 @@ struct Share {
             // rows 8 apart, and with them all values of a thread but the first, have the same place in the swizzle pattern
             constexpr bool SAME = APART<V> % 8 == 0;
             const unsigned at = SAME ? L::offset(row, column >> 3) + u * (L::offset(APART<V>, 0) - L::offset(0, 0)) : L::offset(row + u * APART<V>, column >> 3);
-            store_values<V>(to + at + (column & 7) * 2, PLANE, v.v + u * V * sizeof(T) / 4);
+            store_values<V>(to + at + (column & 7) * 2, PLANE, v.v + u * V);
         }
     }
     __device__ void store(unsigned to, const Values &v) const {
-        if (from.bytes == 16) store_each<MOST>(to, v);
+        if (from.bytes == 16) store_each<4>(to, v);
         else store_each<2>(to, v);
     }
 };
@@ -684,12 +654,12 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             }
         if (!ended)      // copies in flight land before the block goes
             for (int stage = 0; stage < used; ++stage) barrier_wait(full + 8 * stage, stage < ring.stage ? ring.filled : ring.emptied());
-    } else if (BRING != kCopied && warp >= OUT + 2) {
+    } else if constexpr (BRING != kCopied) {
         // Bring what goes through registers, DEPTH steps ahead.
-        constexpr int DEPTH = BRING == kImage ? 3 : sizeof(T) == 4 ? 2 : 1;      // by the registers that a step takes: 16, 32, 48
+        constexpr int DEPTH = BRING == kImage ? 3 : 2;      // by the registers that a step takes: 16 or 32
         const int thread = threadIdx.x - kBringFrom<BRING>;
-        Share<T, S::ROWS, A_ALONG_K> a(p.A, thread);
-        Share<T, S::BN, B_ALONG_K> b(p.B, thread);
+        Share<S::ROWS, A_ALONG_K> a(p.A, thread);
+        Share<S::BN, B_ALONG_K> b(p.B, thread);
         typename decltype(a)::Values va[DEPTH];
         typename decltype(b)::Values vb[BRING == kThrough ? DEPTH : 1];
         int s = 0;
@@ -736,11 +706,9 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             load(std::integral_constant<int, 1>());
             load(std::integral_constant<int, 2>());
             while (store(std::integral_constant<int, 0>()) && store(std::integral_constant<int, 1>()) && store(std::integral_constant<int, 2>())) {}
-        } else if constexpr (DEPTH == 2) {
+        } else {
             load(std::integral_constant<int, 1>());
             while (store(std::integral_constant<int, 0>()) && store(std::integral_constant<int, 1>())) {}
-        } else {
-            while (store(std::integral_constant<int, 0>())) {}
         }
     }
     __syncwarp();
@@ -753,21 +721,20 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
     }
 }
 
-// The image of B that kImage copies: for every tile of columns and step of K its values as they lie in shared memory (along K, split if floats).
-template <typename T, bool B_ALONG_K>
-__global__ void __launch_bounds__(256) image_kernel(Operand<T> B, int N, int K, char *image) {
-    using S = TileShape<T>;
+// The image of B that kImage copies: for every tile of columns and step of K its values as they lie in shared memory (along K, split).
+template <bool B_ALONG_K>
+__global__ void __launch_bounds__(256) image_kernel(Operand<float> B, int N, int K, char *image) {
+    using S = TileShape<float>;
     using L = SharedLayout<S::KS, true>;
     const int steps = (K + S::KS - 1) / S::KS, n0 = (int)blockIdx.x / steps * S::BN, k0 = (int)blockIdx.x % steps * S::KS;
     char *const to = image + (long long)blockIdx.x * S::B_BYTES;
     for (int i = blockIdx.y * 256 + threadIdx.x; i < S::BN * S::KS / 8; i += gridDim.y * 256) {
         const int row = B_ALONG_K ? i / (S::KS / 8) : i % S::BN, unit = B_ALONG_K ? i % (S::KS / 8) : i / S::BN, n = n0 + row, k = k0 + unit * 8;
-        T v[8];
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = n < N && k + e < K ? B.at[B_ALONG_K ? (long long)n * B.ld + k + e : (long long)(k + e) * B.ld + n] : from_float<T>(0.f);
-        unsigned planes[S::PLANES][4];
-        if constexpr (S::PLANES == 3) split_values<8>(v, planes);
-        else memcpy(planes, v, 16);
+        for (int e = 0; e < 8; ++e) v[e] = n < N && k + e < K ? B.at[B_ALONG_K ? (long long)n * B.ld + k + e : (long long)(k + e) * B.ld + n] : 0.f;
+        unsigned planes[3][4];
+        split_values<8>(v, planes);
 #pragma unroll
         for (int q = 0; q < S::PLANES; ++q) *reinterpret_cast<uint4 *>(to + q * S::B_PLANE + L::offset(row, unit)) = make_uint4(planes[q][0], planes[q][1], planes[q][2], planes[q][3]);
     }
@@ -789,14 +756,14 @@ int launch_product_tiles(const Operand<T> &A, const Operand<T> &B, int M, int N,
     using S = TileShape<T>;
     ProductArgs<T, BRING, A_ALONG_K, B_ALONG_K> p = {};
     p.A = A, p.B = B, p.image = (const char *)image, p.M = M, p.N = N, p.K = K, p.share = share, p.shares = shares, p.out = out;
-    if (BRING == kCopied) {
+    if constexpr (BRING == kCopied) {
         constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
         int rc = A_ALONG_K ? tile_map(&p.map_a, bf16, A.at, K, M, A.ld, S::ROWS) : tile_map(&p.map_a, bf16, A.at, M, K, A.ld, S::KS);
         if (!rc) rc = B_ALONG_K ? tile_map(&p.map_b, bf16, B.at, K, N, B.ld, S::BN) : tile_map(&p.map_b, bf16, B.at, N, K, B.ld, S::KS);
         if (rc) return rc;
-    } else if (BRING == kImage) {
+    } else if constexpr (BRING == kImage) {
         const int blocks = ceil_div(N, S::BN) * ceil_div(K, S::KS);
-        image_kernel<T, B_ALONG_K><<<dim3(blocks, S::BN * S::KS / 8 / 256), 256, 0, st>>>(B, N, K, (char *)image);
+        image_kernel<B_ALONG_K><<<dim3(blocks, S::BN * S::KS / 8 / 256), 256, 0, st>>>(B, N, K, (char *)image);
         DRONE_LAUNCH_CHECK("image_kernel");
     }
     // Rows that do not start on 16 bytes share lines between neighbouring steps: what two stages leave of an SM's memory is L1 that keeps them.

@@ -141,7 +141,7 @@ def linear(x, w, bias=None, activation=None, residual=None, transposed=False, ou
     if pre is not None:
         _apart("pre", pre, (x, False), (w, False), (bias, False), (residual, False))
     with _Call(device) as call:
-        image, floats = call.scratch("drone_linear_scratch", _TYPES[dtype], n, x.shape[1], outputs)
+        image, floats = call.scratch("drone_linear_scratch", _TYPES[dtype], n, x.shape[1], outputs, x.data_ptr(), ldx, w.data_ptr(), ldw, int(flipped))
         call("drone_linear", _TYPES[dtype], n, x.shape[1], outputs, x.data_ptr(), ldx, w.data_ptr(), ldw, int(flipped), _pointer(bias), act,
              _pointer(residual), ldr, out.data_ptr(), ldy, _pointer(pre), ldp, _pointer(image), floats)
     return out
@@ -167,17 +167,19 @@ def linear_backward(grad, x, w, pre=None, activation=None, transposed=False, bia
     with _Call(device) as call:
         dz, ldz = grad, ldg
         if act != ACT_NONE:
-            dz, ldz = torch.empty((n, outputs), dtype=dtype, device=device), outputs
+            ldz = outputs if dtype == torch.float32 else (outputs + 7) // 8 * 8      # rows on 16 bytes, as the products want them
+            dz = torch.empty((n, ldz), dtype=dtype, device=device)
         if act != ACT_NONE or bias:
             size = call.scratch("drone_activation_gradient_scratch", kind, n, outputs) if bias else (None, 0)
             call("drone_activation_gradient", kind, n, outputs, grad.data_ptr(), ldg, _pointer(pre) if act != ACT_NONE else None,
                  ldp if act != ACT_NONE else 0, act, dz.data_ptr() if act != ACT_NONE else None, ldz, _pointer(grad_b), _pointer(size[0]), size[1])
         if input_gradient:
-            size = call.scratch("drone_linear_scratch", kind, n, outputs, inputs)
+            size = call.scratch("drone_linear_scratch", kind, n, outputs, inputs, dz.data_ptr(), ldz, w.data_ptr(), ldw, int(not flipped))
             call("drone_linear", kind, n, outputs, inputs, dz.data_ptr(), ldz, w.data_ptr(), ldw, int(not flipped), None, ACT_NONE, None, 0,
                  grad_x.data_ptr(), inputs, None, 0, _pointer(size[0]), size[1])
         # in the weights' own order
-        size = call.scratch("drone_linear_weight_gradient_scratch", kind, n, inputs, outputs, int(bool(transposed)))
+        size = call.scratch("drone_linear_weight_gradient_scratch", kind, n, inputs, outputs, x.data_ptr(), ldx, dz.data_ptr(), ldz,
+                            int(bool(transposed)))
         call("drone_linear_weight_gradient", kind, n, inputs, outputs, x.data_ptr(), ldx, dz.data_ptr(), ldz, int(bool(transposed)),
              grad_w.data_ptr(), grad_w.shape[1], _pointer(size[0]), size[1])
     return grad_x, grad_w, grad_b

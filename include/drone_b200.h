@@ -380,7 +380,8 @@ int drone_weight_gradient(int K, int M, int N, const float *d_A, int lda, const 
  * d_bias, d_residual, d_pre may be NULL; d_pre receives the values before the activation.  d_residual may be d_Y with the
  * same leading dimension; no other operand may overlap an output.  Products of floats are as exact as float
  * multiply-adds. */
-int drone_linear_scratch(int type, int n_rows, int K, int N, long long *n_floats);
+int drone_linear_scratch(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_W, int ldw, int transposed,
+                         long long *n_floats);
 int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_W, int ldw, int transposed,
                  const float *d_bias, int activation, const void *d_residual, int ldr, void *d_Y, int ldy, void *d_pre, int ldp,
                  float *d_scratch, long long n_scratch, void *stream);
@@ -394,7 +395,8 @@ int drone_activation_gradient(int type, int n_rows, int N, const void *d_G, int 
 
 /* dW [K, N] = X^T . dZ, or with `transposed` dW [N, K] = dZ^T . X.  (dX is drone_linear of dZ with W and the other value of
  * `transposed`.) */
-int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, int transposed, long long *n_floats);
+int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_dZ, int ldz,
+                                         int transposed, long long *n_floats);
 int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void *d_X, int ldx, const void *d_dZ, int ldz, int transposed,
                                  void *d_dW, int ldw, float *d_scratch, long long n_scratch, void *stream);
 
