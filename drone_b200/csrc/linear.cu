@@ -32,7 +32,13 @@ __global__ void __launch_bounds__(256) add_product_shares_kernel(const float *__
 //   W [K, N]: a block has 32 columns, a lane one of them, its 32 warps every 32nd k; the warps' sums are added in order.
 //   W [N, K]: a warp has a column, its lanes every 32nd k.
 constexpr int kFewRows = 8;
-constexpr int kFewRowsUpTo = 8;
+// Where that is faster than a few tiles, whose steps of K follow one another however few rows there are.  us here / with tiles: floats 602 x 128
+// 256 rows 7.9 / 21.8, 512 rows 14 / 21.8, 1024 rows 26 / 21.8; 256 x 256 256 rows 7.9 / 12.9, 512 rows 14 / 12.9; 2048 x 2048 32 rows 36 / 58, 64
+// rows 68 / 58; bfloat16 256 x 256 32 rows 5.1 / 6.8, 256 rows 9.2 / 7.2; 2048 x 2048 1 row 6.6 / 13.9, 4 rows 24 / 13.9.
+static bool few_rows(int type, int n, int N, int K) {
+    const long long outputs = (long long)n * N;
+    return n == 1 || (type == DRONE_F32 ? n <= 512 && outputs <= 1 << 16 : outputs <= 1 << 13 && outputs * K <= 1 << 22);
+}
 template <typename T, int ACTIVATION>
 __device__ __forceinline__ void put_value(const LinearOut<T> &out, long long row, int c, float z) {
     if (out.bias) z += __ldg(out.bias + c);
@@ -245,7 +251,7 @@ int drone_linear_scratch(int type, int n_rows, int K, int N, const void *d_X, in
     DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && (transposed == 0 || transposed == 1) && n_floats,
                   "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d transposed=%d", type, n_rows, K, N, transposed);
     using S = TileShape<float>;
-    if (n_rows <= kFewRowsUpTo) *n_floats = 0;
+    if (few_rows(type, n_rows, N, K)) *n_floats = 0;
     else if (type == DRONE_F32) *n_floats = (long long)ceil_div(N, S::BN) * ceil_div(K, S::KS) * (S::B_BYTES / 4);      // the image of the weights
     else *n_floats = padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_W, ldw, transposed ? N : K, transposed ? K : N);
     return DRONE_OK;
@@ -276,7 +282,7 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
         const bool in_fours = N % 4 == 0 && (reinterpret_cast<uintptr_t>(d_bias) & 15) == 0 && fours(d_Y, ldy) && fours(d_residual, ldr) && fours(d_pre, ldp);
         const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr, in_fours};
         const Operand<T> x = operand<T>(d_X, ldx), w = operand<T>(d_W, ldw);
-        if (n_rows <= kFewRowsUpTo) {
+        if (few_rows(type, n_rows, N, K)) {
             const int groups = ceil_div(n_rows, kFewRows);
             if (transposed) few_rows_kernel<T, true><<<dim3(ceil_div(N, 8), groups), 256, 0, st>>>(x, w, n_rows, N, K, out);
             else few_rows_kernel<T, false><<<dim3(ceil_div(N, 32), groups), 1024, 0, st>>>(x, w, n_rows, N, K, out);

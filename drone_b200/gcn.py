@@ -11,6 +11,7 @@ import ctypes as C
 
 import torch
 
+from . import dense
 from ._lib import LOSS_SCRATCH, OP_A, OP_AT, check, lib
 from .graphsum import aggregate_and_exchange, clear_mirror_rows, exchange_sum
 
@@ -205,6 +206,103 @@ class GCN:
                 if l == 1:
                     self.d_z1 = g
         return tuple(self.d_w)
+
+
+class ResidualGCN(GCN):
+    """A deep model of residual layers, which aggregate before they multiply (a layer as wide as its input gathers no wider rows for it):
+
+      Z_0 = x . W_0 + b_0
+      Z_l = Z_{l-1} + S_l . W_l + b_l,  S_l = A^T-aggregation of A_l + mirror/master sync,  A_l = ReLU(norm_l(Z_{l-1})),  l = 1..L
+      logits = A_{L+1} . W_{L+1} + b_{L+1},  A_{L+1} = ReLU(norm_{L+1}(Z_L))
+
+    weights: L + 2 matrices [inputs, outputs]; biases: a vector for each; norms: L + 1 pairs (scale, shift); all float32.  The layers are
+    drone_b200.dense's products (bias and residual in their epilogue) and norms, the aggregation is the graph's.  No counterpart in the
+    reference, whose layers are those of GCN above.
+
+    teacher: None for the cross-entropy over the labelled rows, or (values [n, top], classes [n, top]) of a teacher's best logits: then
+    the loss is soft * (distance from the teacher at `temperature`) + hard * cross-entropy, see dense.distillation_loss.  As in GCN the gradients
+    are those of sums over rows."""
+
+    def __init__(self, graph, x, truth, weights, biases, norms, comm=None, worker_num=1, aggregate=None, sync=None, teacher=None, temperature=1.0,
+                 soft=1.0, hard=0.0, eps=1e-5):
+        self.g, self.x, self.truth = graph, x, truth
+        self.weights, self.biases, self.norms = list(weights), list(biases), [tuple(pair) for pair in norms]
+        self.n_layers = len(self.weights)
+        if self.n_layers < 2 or len(self.biases) != self.n_layers or len(self.norms) != self.n_layers - 1:
+            raise ValueError("%d weights, %d biases and %d norms are no model" % (self.n_layers, len(self.biases), len(self.norms)))
+        self.comm, self.worker_num = comm, worker_num
+        self.aggregate = aggregate or (lambda op, src, out, relu=False: graph.plan.spmm(op, src, out=out, relu=relu))
+        self._custom_aggregate, self._sync, self.fuse_relu = aggregate is not None, sync, False
+        self.mirror2worker = graph.mirror2worker if worker_num > 1 else None
+        self.teacher, self.temperature, self.soft, self.hard, self.eps = teacher, temperature, soft, hard, eps
+        if not x.is_cuda or any(t.dtype != torch.float32 for t in (x, *self.weights)):
+            raise ValueError("rows and weights have to be float32 on a CUDA device")
+        self._kernels = True
+        self._scratch = torch.empty(LOSS_SCRATCH, dtype=torch.float64, device=x.device)
+        self._shares = {}
+        self.labelled = truth >= 0
+        self.safe_truth = truth.clamp(min=0).long()
+        self.d_w, self.d_b = [None] * self.n_layers, [None] * self.n_layers
+        self.d_norms = [None] * (self.n_layers - 1)
+        self.loss = None
+
+    def parameters(self):
+        return [*self.weights, *self.biases, *(t for pair in self.norms for t in pair)]
+
+    def gradients(self):
+        """In the order of parameters()."""
+        return [*self.d_w, *self.d_b, *(t for pair in self.d_norms for t in pair)]
+
+    def broadcast_weights(self):
+        if self.worker_num > 1:
+            for t in self.parameters():
+                self.comm.bcast(t, root=0)
+
+    def reduce_gradients(self):
+        if self.worker_num > 1:
+            for t in self.gradients():
+                self.comm.reduce_sum(t, root=0)
+
+    def forward(self):
+        self.z = [dense.linear(self.x, self.weights[0], bias=self.biases[0])]      # Z_0 .. Z_L
+        self.a, self.s = [], []                                                    # (A_l, mean, rstd) and S_l
+        for l in range(1, self.n_layers):
+            self.a.append(dense.layer_norm(self.z[-1], *self.norms[l - 1], eps=self.eps, relu=True))
+            if l == self.n_layers - 1:
+                break
+            self.s.append(self._aggregate_and_sync(OP_AT, self.a[-1][0], torch.empty_like(self.z[-1])))
+            self.z.append(dense.linear(self.s[-1], self.weights[l], bias=self.biases[l], residual=self.z[-1]))
+        self.logits = dense.linear(self.a[-1][0], self.weights[-1], bias=self.biases[-1])
+        if self.teacher is None:
+            return self._softmax_loss(self.logits)
+        parts, self.d_logits = dense.distillation_loss(self.logits, *self.teacher, temperature=self.temperature, truth=self.safe_truth,
+                                                       labelled=self.labelled, soft=self.soft, hard=self.hard)
+        self.loss = self.soft * parts[0] + self.hard * parts[1]
+        return self.loss
+
+    def _product_gradients(self, l, rows, grad):
+        """Gradients of product l's weights and bias, every replicated vertex counted once, and of its rows."""
+        d_rows = dense.linear(grad, self.weights[l], transposed=True) if l > 0 else None
+        if self.mirror2worker is not None:
+            grad = clear_mirror_rows(grad.clone(), self.mirror2worker)
+        _, self.d_w[l], self.d_b[l] = dense.linear_backward(grad, rows, self.weights[l], input_gradient=False)
+        return d_rows
+
+    def _norm_gradients(self, l, grad):
+        a, mean, rstd = self.a[l]
+        d_rows, *self.d_norms[l] = dense.layer_norm_backward(grad, self.z[l], self.norms[l][0], mean, rstd, out=a, mirror_rows=self.mirror2worker)
+        return d_rows
+
+    def backward(self):
+        """The gradients of weights, biases and norms, in the order of parameters()."""
+        last = self.n_layers - 1
+        grad = self._norm_gradients(last - 1, self._product_gradients(last, self.a[-1][0], self.d_logits))      # of Z_L
+        for l in range(last - 1, 0, -1):
+            d_s = self._product_gradients(l, self.s[l - 1], grad)
+            d_a = self._aggregate_and_sync(OP_A, d_s, torch.empty_like(d_s))
+            grad = grad.add_(self._norm_gradients(l - 1, d_a))
+        self._product_gradients(0, self.x, grad)
+        return tuple(self.gradients())
 
 
 class GCNStep(GCN):

@@ -16,7 +16,7 @@ def refused(name, *args):
 
 
 def linear_args(**change):
-    a = dict(type=0, rows=500, K=6, N=7, X=P, ldx=6, W=P, ldw=7, transposed=0, bias=None, act=0, R=None, ldr=0, Y=P, ldy=7, pre=None, ldp=0, scratch=P, floats=1 << 24, stream=None)
+    a = dict(type=0, rows=5000, K=6, N=7, X=P, ldx=6, W=P, ldw=7, transposed=0, bias=None, act=0, R=None, ldr=0, Y=P, ldy=7, pre=None, ldp=0, scratch=P, floats=1 << 24, stream=None)
     a.update(change)
     return list(a.values())
 
