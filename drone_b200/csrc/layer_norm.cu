@@ -13,30 +13,31 @@
 
 namespace drone {
 
-// Sum of one value per lane over the L lanes of a row (L <= 32: within the warp; above: the block is the row).
+// Sums of two values per lane over the L lanes of a row (L <= 32: within the warp; above: the block is the row).  Calls alternate between two buffers, so that one barrier a call is enough: nobody writes a buffer before everybody has passed the
+// barrier behind its last reads.
 template <int L>
-__device__ __forceinline__ float2 sum_over_row(float2 v) {
+__device__ __forceinline__ float2 sum_over_row(float2 v, int buffer) {
 #pragma unroll
     for (int o = (L < 32 ? L : 32) / 2; o > 0; o >>= 1) {
         v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
         v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
-    if (L > 32) {
-        __shared__ float2 of_warp[2][L / 32 + 1];
-        __syncthreads();      // the sums of the call before have been read
-        if ((threadIdx.x & 31) == 0) of_warp[0][threadIdx.x >> 5] = v;
+    if constexpr (L > 32) {
+        __shared__ float2 of_warp[2][L / 32];
+        if ((threadIdx.x & 31) == 0) of_warp[buffer][threadIdx.x >> 5] = v;
         __syncthreads();
-        v = of_warp[0][0];
+        v = of_warp[buffer][0];
+#pragma unroll
         for (int w = 1; w < L / 32; ++w) {
-            v.x += of_warp[0][w].x;
-            v.y += of_warp[0][w].y;
+            v.x += of_warp[buffer][w].x;
+            v.y += of_warp[buffer][w].y;
         }
     }
     return v;
 }
 
 template <typename T, int L, int U, bool VEC>
-__global__ void __launch_bounds__(L > 256 ? L : 256)
+__global__ void __launch_bounds__(L > 32 ? L : 256)
 layer_norm_kernel(const T *x, long long ldx, const float *__restrict__ scale, const float *__restrict__ shift, int n, int F, float eps, bool relu,
                   T *y, long long ldy, float *__restrict__ mean, float *__restrict__ rstd) {
     using S = RowShape<T, L, U, VEC>;
@@ -54,14 +55,14 @@ layer_norm_kernel(const T *x, long long ldx, const float *__restrict__ scale, co
         float2 s = make_float2(0, 0);
 #pragma unroll
         for (int i = 0; i < S::PER; ++i) s.x += v[i];
-        const float m = sum_over_row<L>(s).x / F;
+        const float m = sum_over_row<L>(s, 0).x / F;
         s.x = 0;
 #pragma unroll
         for (int i = 0; i < S::PER; ++i) {
             v[i] -= m;
             if (S::column(gl, i) < F) s.x += v[i] * v[i];
         }
-        const float r = 1.f / sqrtf(sum_over_row<L>(s).x / F + eps);
+        const float r = 1.f / sqrtf(sum_over_row<L>(s, 1).x / F + eps);
         if (!live) continue;
 #pragma unroll
         for (int i = 0; i < S::PER; ++i) {
@@ -87,13 +88,13 @@ layer_norm_wide_kernel(const T *x, long long ldx, const float *__restrict__ scal
         T *out = y + row * ldy;
         float2 s = make_float2(0, 0);
         for (int c = threadIdx.x; c < F; c += kWideThreads) s.x += to_float(in[c]);
-        const float m = sum_over_row<kWideThreads>(s).x / F;
+        const float m = sum_over_row<kWideThreads>(s, 0).x / F;
         s.x = 0;
         for (int c = threadIdx.x; c < F; c += kWideThreads) {
             const float d = to_float(in[c]) - m;
             s.x += d * d;
         }
-        const float r = 1.f / sqrtf(sum_over_row<kWideThreads>(s).x / F + eps);
+        const float r = 1.f / sqrtf(sum_over_row<kWideThreads>(s, 1).x / F + eps);
         for (int c = threadIdx.x; c < F; c += kWideThreads) {
             const float z = (to_float(in[c]) - m) * r * __ldg(scale + c) + __ldg(shift + c);
             out[c] = from_float<T>(relu && z < 0.f ? 0.f : z);
@@ -119,7 +120,7 @@ struct NormBackward {
 };
 
 template <typename T, int L, int U, bool VEC>
-__global__ void __launch_bounds__(L > 256 ? L : 256) layer_norm_backward_kernel(NormBackward<T> p) {
+__global__ void __launch_bounds__(L > 32 ? L : 256) layer_norm_backward_kernel(NormBackward<T> p) {
     using S = RowShape<T, L, U, VEC>;
     const int gl = threadIdx.x % L, F = p.F;
     float a[S::PER], d_scale[S::PER], d_shift[S::PER];
@@ -127,39 +128,64 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) layer_norm_backward_kernel(
 #pragma unroll
     for (int i = 0; i < S::PER; ++i) d_scale[i] = d_shift[i] = 0;
     const long long first = (long long)blockIdx.x * S::GROUPS, group = threadIdx.x / L, step = (long long)gridDim.x * S::GROUPS;
-    for (long long row0 = first; row0 < p.n; row0 += step) {
-        const bool live = row0 + group < p.n;
-        const long long row = live ? row0 + group : p.n - 1;
-        float g[S::PER], h[S::PER];
-        S::load(p.g + row * p.ldg, F, gl, g);
-        S::load(p.x + row * p.ldx, F, gl, h);
+    // what a row reads, one row ahead where the registers allow it
+    constexpr bool AHEAD = S::PER <= 8;
+    struct Row {
+        float g[S::PER], x[S::PER], o[AHEAD ? S::PER : 1], m, r;
+        bool counts;
+    };
+    auto read = [&](Row &to, long long row0) {
+        const long long row = row0 + group < p.n ? row0 + group : p.n - 1;      // whole warps stay for the shuffles
+        S::load(p.g + row * p.ldg, F, gl, to.g);
+        S::load(p.x + row * p.ldx, F, gl, to.x);
         if (p.out) {
-            float o[S::PER];
-            S::load(p.out + row * p.ldo, F, gl, o);
+            if constexpr (AHEAD) {
+                S::load(p.out + row * p.ldo, F, gl, to.o);
+            } else {
+                float o[S::PER];
+                S::load(p.out + row * p.ldo, F, gl, o);
 #pragma unroll
-            for (int i = 0; i < S::PER; ++i) g[i] = o[i] > 0.f ? g[i] : 0.f;
+                for (int i = 0; i < S::PER; ++i) to.g[i] = o[i] > 0.f ? to.g[i] : 0.f;
+            }
         }
-        const float m = __ldg(p.mean + row), r = __ldg(p.rstd + row);
-        const bool counts = live && (!p.mirror2worker || __ldg(p.mirror2worker + row) == -1);
+        to.m = __ldg(p.mean + row);
+        to.r = __ldg(p.rstd + row);
+        to.counts = row0 + group < p.n && (!p.mirror2worker || __ldg(p.mirror2worker + row) == -1);
+    };
+    Row next;
+    if (AHEAD && first < p.n) read(next, first);
+    int buffer = 0;
+    for (long long row0 = first; row0 < p.n; row0 += step, buffer ^= 1) {
+        const bool live = row0 + group < p.n;
+        Row now;
+        if (AHEAD) {
+            now = next;
+            if (row0 + step < p.n) read(next, row0 + step);
+        } else {
+            read(now, row0);
+        }
         float2 s = make_float2(0, 0);
 #pragma unroll
         for (int i = 0; i < S::PER; ++i) {
-            h[i] = S::column(gl, i) < F ? (h[i] - m) * r : 0.f;
-            if (counts) {
-                d_scale[i] += g[i] * h[i];
-                d_shift[i] += g[i];
+            float g = now.g[i];
+            if (AHEAD && p.out) g = now.o[AHEAD ? i : 0] > 0.f ? g : 0.f;
+            const float hat = S::column(gl, i) < F ? (now.x[i] - now.m) * now.r : 0.f;
+            if (now.counts) {
+                d_scale[i] += g * hat;
+                d_shift[i] += g;
             }
-            g[i] *= a[i];
-            s.x += g[i];
-            s.y += g[i] * h[i];
+            now.x[i] = hat;
+            now.g[i] = g * a[i];
+            s.x += now.g[i];
+            s.y += now.g[i] * hat;
         }
-        s = sum_over_row<L>(s);
+        s = sum_over_row<L>(s, buffer);
         s.x /= F;
         s.y /= F;
         if (!live) continue;
 #pragma unroll
-        for (int i = 0; i < S::PER; ++i) g[i] = r * (g[i] - s.x - h[i] * s.y);
-        S::store(p.dx + row * p.ld, F, gl, g);
+        for (int i = 0; i < S::PER; ++i) now.g[i] = now.r * (now.g[i] - s.x - now.x[i] * s.y);
+        S::store(p.dx + (row0 + group) * p.ld, F, gl, now.g);
     }
     float *of_block = p.sums + (long long)blockIdx.x * 2 * F;
     S::add_groups(d_scale, F, gl, of_block);
@@ -171,7 +197,8 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(
     const int F = p.F;
     float *d_scale = p.sums + (long long)blockIdx.x * 2 * F, *d_shift = d_scale + F;      // a thread always has the same columns
     for (int c = threadIdx.x; c < F; c += kWideThreads) d_scale[c] = d_shift[c] = 0;
-    for (long long row = blockIdx.x; row < p.n; row += gridDim.x) {
+    int buffer = 0;
+    for (long long row = blockIdx.x; row < p.n; row += gridDim.x, buffer ^= 1) {
         const T *in = p.x + row * p.ldx, *dy = p.g + row * p.ldg, *out = p.out ? p.out + row * p.ldo : nullptr;
         const float m = __ldg(p.mean + row), r = __ldg(p.rstd + row);
         const bool counts = !p.mirror2worker || __ldg(p.mirror2worker + row) == -1;
@@ -185,7 +212,7 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(
             s.x += g * __ldg(p.scale + c);
             s.y += g * __ldg(p.scale + c) * h;
         }
-        s = sum_over_row<kWideThreads>(s);
+        s = sum_over_row<kWideThreads>(s, buffer);
         for (int c = threadIdx.x; c < F; c += kWideThreads) {
             const float g = out && !(to_float(out[c]) > 0.f) ? 0.f : to_float(dy[c]), h = (to_float(in[c]) - m) * r;
             p.dx[row * p.ld + c] = from_float<T>(r * (g * __ldg(p.scale + c) - s.x / F - h * (s.y / F)));
@@ -196,14 +223,16 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(
 struct NormGrid {
     int groups, blocks;      // rows a block takes at once; blocks
 };
-static NormGrid norm_grid(int type, int n, int F, int sms, int blocks_per_sm) {
+static NormGrid norm_grid(int type, int n, int F, int sms, int threads_per_sm) {
     const int V = type == DRONE_F32 ? 4 : 8, vectors = ceil_div(F, V);
     NormGrid g;
     g.groups = vectors <= 16 ? 32 : vectors <= 128 ? 8 : 1;
-    g.blocks = (int)std::min<long long>(((long long)n + g.groups - 1) / g.groups, (long long)sms * blocks_per_sm);
+    const int threads = vectors <= 128 ? 256 : vectors <= 256 ? 128 : vectors <= 1024 ? 256 : 512;
+    g.blocks = (int)std::min<long long>(((long long)n + g.groups - 1) / g.groups, (long long)sms * (threads_per_sm / threads));
     return g;
 }
-constexpr int kBackwardBlocksPerSm = 4;
+// of the blocks: all that the registers hold at the shapes of most rows
+constexpr int kForwardThreadsPerSm = 2048, kBackwardThreadsPerSm = 1024;
 
 }  // namespace drone
 
@@ -222,7 +251,7 @@ int drone_layer_norm(int type, int n_rows, int F, const void *d_X, int ldx, cons
     cudaStream_t st = (cudaStream_t)stream;
     int sms = 0, rc = device_sms(&sms);
     if (rc) return rc;
-    const int blocks = norm_grid(type, n_rows, F, sms, 8).blocks;
+    const int blocks = norm_grid(type, n_rows, F, sms, kForwardThreadsPerSm).blocks;
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
         constexpr int V = kVector<T>;
@@ -233,8 +262,8 @@ int drone_layer_norm(int type, int n_rows, int F, const void *d_X, int ldx, cons
                 kernel<<<blocks, threads, 0, st>>>((const T *)d_X, ldx, d_scale, d_shift, n_rows, F, eps, relu != 0, (T *)d_Y, ldy, d_mean, d_rstd);
             };
             if constexpr (L == 0) launch(layer_norm_wide_kernel<T>, kWideThreads);
-            else if (vec) launch(layer_norm_kernel<T, L, U, true>, L > 256 ? L : 256);
-            else launch(layer_norm_kernel<T, L, U, false>, L > 256 ? L : 256);
+            else if (vec) launch(layer_norm_kernel<T, L, U, true>, L > 32 ? L : 256);
+            else launch(layer_norm_kernel<T, L, U, false>, L > 32 ? L : 256);
             DRONE_LAUNCH_CHECK("layer_norm_kernel");
             return DRONE_OK;
         });
@@ -247,7 +276,7 @@ int drone_layer_norm_backward_scratch(int type, int n_rows, int F, long long *n_
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    *n_floats = 2LL * F * norm_grid(type, n_rows, F, sms, kBackwardBlocksPerSm).blocks;
+    *n_floats = 2LL * F * norm_grid(type, n_rows, F, sms, kBackwardThreadsPerSm).blocks;
     return DRONE_OK;
 }
 
@@ -263,7 +292,7 @@ int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int 
     cudaStream_t st = (cudaStream_t)stream;
     int sms = 0, rc = device_sms(&sms);
     if (rc) return rc;
-    const int blocks = norm_grid(type, n_rows, F, sms, kBackwardBlocksPerSm).blocks;
+    const int blocks = norm_grid(type, n_rows, F, sms, kBackwardThreadsPerSm).blocks;
     const long long need = 2LL * F * blocks;
     DRONE_REQUIRE(n_scratch >= need && (need == 0 || d_scratch), "drone_layer_norm_backward: %lld floats of scratch, %lld needed", n_scratch, need);
     if (n_rows > 0) {
@@ -277,8 +306,8 @@ int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int 
             return with_row_shape(ceil_div(F, V), [&](auto shape) {
                 constexpr int L = decltype(shape)::L, U = decltype(shape)::U;
                 if constexpr (L == 0) layer_norm_backward_wide_kernel<T><<<blocks, kWideThreads, 0, st>>>(p);
-                else if (vec) layer_norm_backward_kernel<T, L, U, true><<<blocks, L > 256 ? L : 256, 0, st>>>(p);
-                else layer_norm_backward_kernel<T, L, U, false><<<blocks, L > 256 ? L : 256, 0, st>>>(p);
+                else if (vec) layer_norm_backward_kernel<T, L, U, true><<<blocks, L > 32 ? L : 256, 0, st>>>(p);
+                else layer_norm_backward_kernel<T, L, U, false><<<blocks, L > 32 ? L : 256, 0, st>>>(p);
                 DRONE_LAUNCH_CHECK("layer_norm_backward_kernel");
                 return DRONE_OK;
             });

@@ -224,14 +224,14 @@ static Shares product_shares(int type, int M, int N, int K, int sms) {
     return type == DRONE_F32 ? product_shares<float>(M, N, K, sms) : product_shares<__half>(M, N, K, sms);
 }
 
-// Blocks of the activations' gradient: as many as the SMs hold, of at most 128 vectors a row.
+// Blocks of the activations' gradient: as many as the SMs hold, of at most 64 vectors a row.
 struct GradientBlocks {
     int width, columns, rows;      // of a block; blocks along the columns and the rows
 };
 static GradientBlocks gradient_blocks(int type, int n, int N, int sms) {
     const int V = 16 / type_size(type);
     GradientBlocks b;
-    b.width = std::min(N, 128 * V);
+    b.width = std::min(N, 64 * V);
     b.columns = ceil_div(N, b.width);
     const int groups = ceil_div(b.width, V) <= 16 ? 32 : 8;
     b.rows = (int)std::min<long long>(((long long)n + groups - 1) / groups, std::max(1, 6 * sms / b.columns));

@@ -9,7 +9,7 @@ namespace drone {
 // values a lane, L apart.
 template <typename T, int L, int U, bool VEC>
 struct RowShape {
-    static constexpr int V = kVector<T>, PER = U * V, THREADS = L > 256 ? L : 256, GROUPS = THREADS / L;
+    static constexpr int V = kVector<T>, PER = U * V, THREADS = L > 32 ? L : 256, GROUPS = THREADS / L;
     __device__ static int column(int gl, int i) { return VEC ? (gl + i / V * L) * V + i % V : gl + i * L; }
     // values beyond the row are 0
     __device__ static void load(const T *row, int F, int gl, float (&v)[PER]) {
@@ -25,19 +25,20 @@ struct RowShape {
             for (int i = 0; i < PER; ++i) v[i] = column(gl, i) < F ? to_float(row[column(gl, i)]) : 0.f;
         }
     }
-    __device__ static void store(T *row, int F, int gl, const float (&v)[PER]) {
-        if (VEC) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                Values<T, V> x;
-                x.set(v + u * V);
-                if (column(gl, u * V) < F) *reinterpret_cast<Values<T, V> *>(row + column(gl, u * V)) = x;
-            }
+    __device__ static void store_vector(T *row, int F, int gl, int u, const float *v) {
+        if constexpr (VEC) {
+            Values<T, V> x;
+            x.set(v);
+            if (column(gl, u * V) < F) *reinterpret_cast<Values<T, V> *>(row + column(gl, u * V)) = x;
         } else {
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (column(gl, i) < F) row[column(gl, i)] = from_float<T>(v[i]);
+            for (int e = 0; e < V; ++e)
+                if (column(gl, u * V + e) < F) row[column(gl, u * V + e)] = from_float<T>(v[e]);
         }
+    }
+    __device__ static void store(T *row, int F, int gl, const float (&v)[PER]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) store_vector(row, F, gl, u, v + u * V);
     }
     __device__ static void load_vector(const float *p, int F, int gl, float (&v)[PER]) {
 #pragma unroll
@@ -75,6 +76,7 @@ int with_row_shape(int vectors, const F &f) {
     if (vectors <= 32) return f(LanesOfRow<32, 1>());
     if (vectors <= 64) return f(LanesOfRow<32, 2>());
     if (vectors <= 128) return f(LanesOfRow<32, 4>());
+    if (vectors <= 256) return f(LanesOfRow<128, 2>());
     if (vectors <= 512) return f(LanesOfRow<256, 2>());
     if (vectors <= 1024) return f(LanesOfRow<256, 4>());
     if (vectors <= 2048) return f(LanesOfRow<512, 4>());
