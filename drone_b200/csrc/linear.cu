@@ -96,6 +96,65 @@ __global__ void __launch_bounds__(TRANSPOSED ? 256 : 1024) few_rows_kernel(Opera
     }
 }
 
+// Many rows, few products each: a block keeps W and some rows of X in shared memory as floats, a thread an output at a time, so that X and Y go
+// over neighbouring lanes whatever their widths and distances.  Bound: two reads of shared memory a product.  us here / with tiles: 1.38 M x 5 x 1
+// floats 28 / 149, bfloat16 28 / 228; 410,000 x 3 x 20 35 / 60 and 37 / 57; 3,000 x 16 x 7 18 / 25 and 18 / 24; but 192,000 x 154 x 2 floats 101 / 62,
+// 400,000 x 16 x 64 158 / 72.
+constexpr int kNarrowProducts = 128, kNarrowValues = 8192;
+static bool narrow_rows(int K, int N) { return (long long)K * N <= kNarrowProducts; }
+template <typename T>
+__global__ void __launch_bounds__(256) narrow_rows_kernel(Operand<T> X, Operand<T> W, bool transposed, int n, int N, int K, int rows_at_once, LinearOut<T> out) {
+    __shared__ float w[kNarrowProducts], x[kNarrowValues];
+    for (int i = threadIdx.x; i < K * N; i += 256) {
+        const int k = i / N, c = i % N;
+        w[i] = to_float(W.at[transposed ? c * W.ld + k : k * W.ld + c]);
+    }
+    const int pitch = K | 1;
+    with_activation(out.activation, [&](auto act) {
+        for (long long row0 = (long long)blockIdx.x * rows_at_once; row0 < n; row0 += (long long)gridDim.x * rows_at_once) {
+            const int rows = (int)min((long long)rows_at_once, n - row0);
+            __syncthreads();
+            for (RowColumn at(threadIdx.x, 256, K); at.row < rows; at.advance()) x[at.row * pitch + at.col] = to_float(X.at[(row0 + at.row) * X.ld + at.col]);
+            __syncthreads();
+            for (RowColumn at(threadIdx.x, 256, N); at.row < rows; at.advance()) {
+                float acc = 0;
+#pragma unroll 4
+                for (int k = 0; k < K; ++k) acc = fmaf(x[at.row * pitch + k], w[k * N + at.col], acc);
+                put_value<T, decltype(act)::value>(out, row0 + at.row, at.col, acc);
+            }
+        }
+    });
+}
+
+// Its weight gradient: a thread has a value of dW and every 256 / values-th row of what the block keeps; shares[block].
+template <typename T>
+__global__ void __launch_bounds__(256) narrow_gradient_kernel(Operand<T> X, Operand<T> Z, int n, int N, int K, bool transposed, int rows_at_once, float *shares) {
+    __shared__ float x[kNarrowValues / 2], z[kNarrowValues / 2];
+    const int values = K * N, parts = 256 / values, part = (int)threadIdx.x / values, value = (int)threadIdx.x % values;
+    const int k = transposed ? value % K : value / N, c = transposed ? value / K : value % N, pitch_x = K | 1, pitch_z = N | 1;
+    float acc = 0;
+    for (long long row0 = (long long)blockIdx.x * rows_at_once; row0 < n; row0 += (long long)gridDim.x * rows_at_once) {
+        const int rows = (int)min((long long)rows_at_once, n - row0);
+        __syncthreads();
+        for (RowColumn at(threadIdx.x, 256, K); at.row < rows; at.advance()) x[at.row * pitch_x + at.col] = to_float(X.at[(row0 + at.row) * X.ld + at.col]);
+        for (RowColumn at(threadIdx.x, 256, N); at.row < rows; at.advance()) z[at.row * pitch_z + at.col] = to_float(Z.at[(row0 + at.row) * Z.ld + at.col]);
+        __syncthreads();
+        if (part < parts)
+            for (int r = part; r < rows; r += parts) acc = fmaf(x[r * pitch_x + k], z[r * pitch_z + c], acc);
+    }
+    __syncthreads();
+    x[threadIdx.x] = acc;
+    __syncthreads();
+    if ((int)threadIdx.x < values) {
+        float sum = 0;
+        for (int i = 0; i < parts; ++i) sum += x[i * values + threadIdx.x];
+        shares[(long long)blockIdx.x * values + threadIdx.x] = sum;
+    }
+}
+// Rows that a block has at a time, of so many values each; blocks.
+static int narrow_rows_at_once(int width, int operands) { return std::min(256, kNarrowValues / operands / (width | 1)); }
+static int narrow_blocks(int n, int rows_at_once, int sms) { return (int)std::min<long long>(((long long)n + rows_at_once - 1) / rows_at_once, sms * 3); }
+
 // 16-bit rows to rows that start on 16 bytes: a thread 16 bytes of them.  What lies behind a row's end is never read.
 __global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short *__restrict__ from, long long ld, int n, int width, uint4 *__restrict__ to, int vectors) {
     const bool pairs = (reinterpret_cast<uintptr_t>(from) & 3) == 0 && ld % 2 == 0;
@@ -251,7 +310,7 @@ int drone_linear_scratch(int type, int n_rows, int K, int N, const void *d_X, in
     DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && (transposed == 0 || transposed == 1) && n_floats,
                   "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d transposed=%d", type, n_rows, K, N, transposed);
     using S = TileShape<float>;
-    if (few_rows(type, n_rows, N, K)) *n_floats = 0;
+    if (few_rows(type, n_rows, N, K) || narrow_rows(K, N)) *n_floats = 0;
     else if (type == DRONE_F32) *n_floats = (long long)ceil_div(N, S::BN) * ceil_div(K, S::KS) * (S::B_BYTES / 4);      // the image of the weights
     else *n_floats = padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_W, ldw, transposed ? N : K, transposed ? K : N);
     return DRONE_OK;
@@ -287,6 +346,13 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
             if (transposed) few_rows_kernel<T, true><<<dim3(ceil_div(N, 8), groups), 256, 0, st>>>(x, w, n_rows, N, K, out);
             else few_rows_kernel<T, false><<<dim3(ceil_div(N, 32), groups), 1024, 0, st>>>(x, w, n_rows, N, K, out);
             DRONE_LAUNCH_CHECK("few_rows_kernel");
+            return DRONE_OK;
+        }
+        if (narrow_rows(K, N)) {
+            const int rows_at_once = narrow_rows_at_once(K, 1);
+            narrow_rows_kernel<T><<<(int)std::min<long long>(((long long)n_rows + rows_at_once - 1) / rows_at_once, sms * 5), 256, 0, st>>>(x, w, transposed != 0, n_rows, N,
+                                                                                                                                 K, rows_at_once, out);
+            DRONE_LAUNCH_CHECK("narrow_rows_kernel");
             return DRONE_OK;
         }
         if constexpr (sizeof(T) == 2) {
@@ -365,9 +431,10 @@ int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, con
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    const Shares s = product_shares(type, transposed ? N : K, transposed ? K : N, n_rows, sms);
-    *n_floats = n_rows == 0 ? 0 : (long long)s.count * K * N;
-    if (type != DRONE_F32) *n_floats = (*n_floats + 3) / 4 * 4 + padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_dZ, ldz, n_rows, N);
+    const bool narrow = narrow_rows(K, N);
+    const int shares = narrow ? narrow_blocks(n_rows, narrow_rows_at_once(std::max(K, N), 2), sms) : product_shares(type, transposed ? N : K, transposed ? K : N, n_rows, sms).count;
+    *n_floats = n_rows == 0 ? 0 : (long long)shares * K * N;
+    if (type != DRONE_F32 && !narrow) *n_floats = (*n_floats + 3) / 4 * 4 + padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_dZ, ldz, n_rows, N);
     return DRONE_OK;
 }
 
@@ -398,6 +465,14 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
         Operand<T> x = operand<T>(d_X, ldx), dz = operand<T>(d_dZ, ldz);
+        if (narrow_rows(K, N)) {
+            const int rows_at_once = narrow_rows_at_once(std::max(K, N), 2), blocks = narrow_blocks(n_rows, rows_at_once, sms);
+            narrow_gradient_kernel<T><<<blocks, 256, 0, st>>>(x, dz, n_rows, N, K, transposed != 0, rows_at_once, d_scratch);
+            DRONE_LAUNCH_CHECK("narrow_gradient_kernel");
+            add_product_shares_kernel<T, 8><<<ceil_div((long long)rows * columns, 32), 256, 0, st>>>(d_scratch, blocks, rows, columns, (T *)d_dW, ldw);
+            DRONE_LAUNCH_CHECK("add_product_shares_kernel");
+            return DRONE_OK;
+        }
         if constexpr (sizeof(T) == 2) {
             float *scratch = d_scratch + ((long long)s.count * K * N + 3) / 4 * 4;
             int failed = on_16_bytes(d_X, ldx, n_rows, K, &scratch, sms, st, &x);

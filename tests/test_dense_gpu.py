@@ -402,3 +402,21 @@ def test_distillation_of_masked_logits(cuda_device, dtype):
         logits[1, 5:], logits[2], teacher[3, 1:], teacher[4] = low, low, low, low
         check_distillation(logits, teacher, classes, 1.0)
         check_distillation(logits, teacher, classes, 4.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", [(2, 1, 1), (600, 5, 1), (513, 1, 128), (70001, 16, 8), (9999, 128, 1), (300007, 3, 20), (5, 2, 64)])
+def test_narrow_products_and_their_gradients(cuda_device, n, k, m, dtype):
+    """Few products a row: forward, and the weights' gradient in both orders."""
+    gen = torch.Generator(cuda_device).manual_seed(n + k + m)
+    for pad, lead in ((0, 0), (3, 1)):
+        check_linear(gen, n, k, m, dtype, bias=True, residual=True, activation="silu", keep=True, pad=pad, lead=lead)
+        x, g = rows_of(gen, n, k, dtype, pad, lead), rows_of(gen, n, m, dtype, pad, lead)
+        for transposed in (False, True):
+            check_linear(gen, n, k, m, dtype, transposed=transposed, pad=pad, lead=lead)
+            w = rows_of(gen, m, k, dtype) if transposed else rows_of(gen, k, m, dtype)
+            dx, dw, db = dense.linear_backward(g, x, w, transposed=transposed)
+            wd = w.double().t() if transposed else w.double()
+            want, bound = x.double().t() @ g.double(), (n + 16) * STEP * (x.double().abs().t() @ g.double().abs())
+            check_rounded(dw, want.t() if transposed else want, bound.t() if transposed else bound, dtype)
+            check_rounded(dx, g.double() @ wd.t(), (m + 16) * STEP * (g.double().abs() @ wd.t().abs()), dtype)
