@@ -16,15 +16,15 @@ def refused(name, *args):
 
 
 def linear_args(**change):
-    a = dict(type=0, rows=5000, K=6, N=7, X=P, ldx=6, W=P, ldw=7, transposed=0, bias=None, act=0, R=None, ldr=0, Y=P, ldy=7, pre=None, ldp=0, scratch=P, floats=1 << 24, stream=None)
+    a = dict(type=0, rows=5000, K=60, N=70, X=P, ldx=60, W=P, ldw=70, transposed=0, bias=None, act=0, R=None, ldr=0, Y=P, ldy=70, pre=None, ldp=0, scratch=P, floats=1 << 24, stream=None)
     a.update(change)
     return list(a.values())
 
 
 @pytest.mark.parametrize("change", [
-    dict(type=3), dict(type=-1), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(K=0), dict(K=(1 << 15) + 1, ldx=1 << 16), dict(N=0), dict(N=-3), dict(ldx=5), dict(ldw=6),
-    dict(transposed=1, ldw=5), dict(transposed=2), dict(act=4), dict(act=-1), dict(R=P, ldr=6), dict(ldy=6), dict(pre=P, ldp=6), dict(X=None), dict(W=None),
-    dict(Y=None), dict(X=P + 2), dict(type=1, Y=P + 1), dict(R=P + 1, ldr=7), dict(type=2, pre=P + 1, ldp=7), dict(scratch=None), dict(scratch=P + 4), dict(floats=16), dict(bias=P + 2)])
+    dict(type=3), dict(type=-1), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(K=0), dict(K=(1 << 15) + 1, ldx=1 << 16), dict(N=0), dict(N=-3), dict(ldx=59), dict(ldw=69),
+    dict(transposed=1, ldw=59), dict(transposed=2), dict(act=4), dict(act=-1), dict(R=P, ldr=69), dict(ldy=69), dict(pre=P, ldp=69), dict(X=None), dict(W=None),
+    dict(Y=None), dict(X=P + 2), dict(type=1, Y=P + 1), dict(R=P + 1, ldr=70), dict(type=2, pre=P + 1, ldp=70), dict(scratch=None), dict(scratch=P + 4), dict(floats=16), dict(bias=P + 2)])
 def test_linear_refuses(change):
     assert "drone_linear" in refused("drone_linear", *linear_args(**change))
 
