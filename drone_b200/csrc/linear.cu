@@ -337,9 +337,12 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
     cudaStream_t st = (cudaStream_t)stream;
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
-        const auto fours = [](const void *p, long long ld) { return !p || ((reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && ld % 4 == 0); };
-        const bool in_fours = N % 4 == 0 && (reinterpret_cast<uintptr_t>(d_bias) & 15) == 0 && fours(d_Y, ldy) && fours(d_residual, ldr) && fours(d_pre, ldp);
-        const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr, in_fours};
+        const auto in_steps_of = [&](int values) {
+            const auto fits = [&](const void *p, long long ld) { return !p || ((reinterpret_cast<uintptr_t>(p) & (values * sizeof(T) - 1)) == 0 && ld % values == 0); };
+            return N % values == 0 && (reinterpret_cast<uintptr_t>(d_bias) & 15) == 0 && fits(d_Y, ldy) && fits(d_residual, ldr) && fits(d_pre, ldp);
+        };
+        const int at_once = in_steps_of(kVector<T>) ? kVector<T> : in_steps_of(4) ? 4 : 1;
+        const LinearOut<T> out = {d_bias, activation, (const T *)d_residual, ldr, (T *)d_Y, ldy, (T *)d_pre, ldp, nullptr, at_once};
         const Operand<T> x = operand<T>(d_X, ldx), w = operand<T>(d_W, ldw);
         if (few_rows(type, n_rows, N, K)) {
             const int groups = ceil_div(n_rows, kFewRows);
@@ -480,7 +483,7 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
             if (failed) return failed;
         }
         const Operand<T> a = transposed ? dz : x, b = transposed ? x : dz;
-        const LinearOut<T> out = {nullptr, DRONE_ACT_NONE, nullptr, 0, nullptr, 0, nullptr, 0, d_scratch, false};
+        const LinearOut<T> out = {nullptr, DRONE_ACT_NONE, nullptr, 0, nullptr, 0, nullptr, 0, d_scratch, 1};
         constexpr Bring BRING = sizeof(T) == 2 ? kCopied : kThrough;
         const int launched = launch_product_tiles<T, BRING, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
         if (launched) return launched;

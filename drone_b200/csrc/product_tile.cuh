@@ -38,7 +38,7 @@ struct LinearOut {
     T *pre;
     long long ldp;
     float *shares;      // not NULL: [share][M][N]
-    bool fours;         // four columns of every operand can be read and written at once
+    int at_once;        // columns of every operand that can be read and written at once: 16 bytes of them, 4, or 1
 };
 
 // An operand: values `ld` apart along one dimension and side by side along the other; read `bytes` at a time.
@@ -353,60 +353,93 @@ struct ProductArgs {
     LinearOut<T> out;
 };
 
-// The residual of 32 x 32 values: of 16-bit ones read before the accumulators are waited for, of floats (32 registers) when it is added.
+// The residual of 32 x 32 values, W of a row a lane: of 16-bit ones read before the accumulators are waited for, of floats (32 registers) when it
+// is added.
 template <typename T>
 struct Residual {
     static constexpr bool AHEAD = sizeof(T) == 2;
-    uint2 v[AHEAD ? 8 : 1];
-    __device__ __forceinline__ void read(const LinearOut<T> &out, long long row0, int rows, int col0, int width) {
-        const int lane = threadIdx.x & 31, c = (lane & 7) * 4;
-        if (!AHEAD || !out.fours || !out.residual || c >= width) return;
-        const T *from = out.residual + (row0 + (lane >> 3)) * out.ldr + col0 + c;
+    unsigned v[AHEAD ? 16 : 1];
+    template <int W>
+    __device__ __forceinline__ void read_each(const LinearOut<T> &out, long long row0, int rows, int col0, int width) {
+        constexpr int LANES = 32 / W, STEP = 32 / LANES;      // of a row; rows at once
+        const int lane = threadIdx.x & 31, c = lane % LANES * W;
+        if (c >= width) return;
+        const T *from = out.residual + (row0 + lane / LANES) * out.ldr + col0 + c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if ((lane >> 3) + i * 4 < rows) v[AHEAD ? i : 0] = *reinterpret_cast<const uint2 *>(from + (long long)(i * 4) * out.ldr);
+        for (int i = 0; i < LANES; ++i)
+            if (lane / LANES + i * STEP < rows) {
+                if constexpr (W == 8) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(from + (long long)(i * STEP) * out.ldr);
+                    v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(from + (long long)(i * STEP) * out.ldr);
+                    v[2 * i] = x.x, v[2 * i + 1] = x.y;
+                }
+            }
     }
-    __device__ __forceinline__ Values<T, 4> at(const LinearOut<T> &out, int i, long long row, int column) const {
-        Values<T, 4> x = {};
-        if constexpr (AHEAD) memcpy(&x, &v[i], 8);
-        else if (out.residual) x = *reinterpret_cast<const Values<T, 4> *>(out.residual + row * out.ldr + column);
+    __device__ __forceinline__ void read(const LinearOut<T> &out, long long row0, int rows, int col0, int width) {
+        if constexpr (AHEAD) {
+            if (!out.residual) return;
+            if (out.at_once == 8) read_each<8>(out, row0, rows, col0, width);
+            else if (out.at_once == 4) read_each<4>(out, row0, rows, col0, width);
+        }
+    }
+    template <int W>
+    __device__ __forceinline__ Values<T, W> at(const LinearOut<T> &out, int i, long long row, int column) const {
+        Values<T, W> x = {};
+        if constexpr (AHEAD) memcpy(&x, &v[i * W / 2], W * 2);
+        else if (out.residual) x = *reinterpret_cast<const Values<T, W> *>(out.residual + row * out.ldr + column);
         return x;
     }
 };
 
 // 32 x 32 values of a finished tile, of which the warp has written a row a lane to shared memory, to the outputs with neighbouring columns in
 // neighbouring lanes.
+template <typename T, int PITCH, int ACTIVATION, int W>
+__device__ __forceinline__ void put_vectors(const LinearOut<T> &out, const float *piece, const Residual<T> &residual, long long row0, int rows, int col0, int width) {
+    constexpr int LANES = 32 / W, STEP = 32 / LANES;
+    const int lane = threadIdx.x & 31, c = lane % LANES * W;
+    if (c >= width) return;
+    float b[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) b[i] = 0;
+    if (out.bias) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) *reinterpret_cast<float4 *>(b + i) = __ldg((const float4 *)(out.bias + col0 + c + i));
+    }
+#pragma unroll(Residual<T>::AHEAD ? LANES : 2)
+    for (int step = 0; step < LANES; ++step) {
+        const int r = lane / LANES + step * STEP;
+        if (r >= rows) break;
+        const long long row = row0 + r;
+        float z[W], w[W], added[W];
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const float4 acc = *reinterpret_cast<const float4 *>(piece + r * PITCH + c + i);
+            z[i] = acc.x + b[i], z[i + 1] = acc.y + b[i + 1], z[i + 2] = acc.z + b[i + 2], z[i + 3] = acc.w + b[i + 3];
+        }
+        residual.template at<W>(out, step, row, col0 + c).get(added);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            w[i] = activate<T, ACTIVATION>(z[i]);
+            if (out.residual) w[i] += added[i];
+        }
+        Values<T, W> y;
+        if (out.pre) {
+            y.set(z);
+            *reinterpret_cast<Values<T, W> *>(out.pre + row * out.ldp + col0 + c) = y;
+        }
+        y.set(w);
+        *reinterpret_cast<Values<T, W> *>(out.y + row * out.ldy + col0 + c) = y;
+    }
+}
 template <typename T, int PITCH, int ACTIVATION>
 __device__ __forceinline__ void put_piece(const LinearOut<T> &out, const float *piece, const Residual<T> &residual, long long row0, int rows, int col0, int width) {
     const int lane = threadIdx.x & 31;
-    if (out.fours) {
-        using Four = Values<T, 4>;
-        const int c = (lane & 7) * 4;
-        if (c >= width) return;
-        float4 b = make_float4(0, 0, 0, 0);
-        if (out.bias) b = __ldg((const float4 *)(out.bias + col0 + c));
-#pragma unroll(Residual<T>::AHEAD ? 8 : 2)
-        for (int i8 = 0; i8 < 8; ++i8) {
-            const int r = (lane >> 3) + i8 * 4;
-            if (r >= rows) break;
-            const long long row = row0 + r;
-            Four y;
-            const float4 acc = *reinterpret_cast<const float4 *>(piece + r * PITCH + c);
-            float z[4] = {acc.x + b.x, acc.y + b.y, acc.z + b.z, acc.w + b.w}, w[4], added[4];
-            residual.at(out, i8, row, col0 + c).get(added);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = activate<T, ACTIVATION>(z[i]);
-                if (out.residual) w[i] += added[i];
-            }
-            if (out.pre) {
-                Four p;
-                p.set(z);
-                *reinterpret_cast<Four *>(out.pre + row * out.ldp + col0 + c) = p;
-            }
-            y.set(w);
-            *reinterpret_cast<Four *>(out.y + row * out.ldy + col0 + c) = y;
-        }
+    if (sizeof(T) == 2 && out.at_once == 8) {
+        if constexpr (sizeof(T) == 2) put_vectors<T, PITCH, ACTIVATION, 8>(out, piece, residual, row0, rows, col0, width);
+    } else if (out.at_once == 4) {
+        put_vectors<T, PITCH, ACTIVATION, 4>(out, piece, residual, row0, rows, col0, width);
     } else if (lane < width) {
         const float b = out.bias ? __ldg(out.bias + col0 + lane) : 0.f;
 #pragma unroll 4
@@ -492,7 +525,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                         LinearOut<float> to = {};
                         to.y = p.out.shares + (long long)walk.index * p.M * p.N;
                         to.ldy = p.N;
-                        to.fours = p.N % 4 == 0;
+                        to.at_once = p.N % 4 == 0 ? 4 : 1;
                         put_piece<float, S::PITCH, DRONE_ACT_NONE>(to, from, Residual<float>(), row0, rows, col0 + c, min(32, width - c));
                     } else {
                         put_piece<T, S::PITCH, ACTIVATION>(p.out, from, residual, row0, rows, col0 + c, min(32, width - c));
