@@ -211,7 +211,7 @@ int tile_map(CUtensorMap *map, bool bf16, const void *p, long long width, long l
 // dZ = G * activation'(pre) and the sums of its columns, of those from blockIdx.y * width on; sums[blockIdx.x] = those of the block's rows.
 // Bound: HBM, two reads and a write.
 template <typename T, int L, int U, bool VEC, int ACTIVATION>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 activation_gradient_kernel(const T *G, long long ldg, const T *pre, long long ldp, int n, int N, int width, T *dZ, long long ldz, float *sums) {
     using S = RowShape<T, L, U, VEC>;
     const int gl = threadIdx.x % L, c0 = blockIdx.y * width, F = min(width, N - c0);
@@ -293,7 +293,7 @@ static GradientBlocks gradient_blocks(int type, int n, int N, int sms) {
     b.width = std::min(N, 64 * V);
     b.columns = ceil_div(N, b.width);
     const int groups = ceil_div(b.width, V) <= 16 ? 32 : 8;
-    b.rows = (int)std::min<long long>(((long long)n + groups - 1) / groups, std::max(1, 6 * sms / b.columns));
+    b.rows = (int)std::min<long long>(((long long)n + groups - 1) / groups, std::max(1, 4 * sms / b.columns));
     return b;
 }
 

@@ -609,9 +609,8 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
             // float accumulators, both operands of this type, lying along K (0) or not (1), columns / 8, rows / 16
             const unsigned instruction = 1u << 4 | TYPE << 7 | TYPE << 10 | (A_ALONG_K ? 0u : 1u) << 15 | (B_SHARED_ALONG_K ? 0u : 1u) << 16 |
                                          (unsigned)(walk.columns() / 8) << 17 | (unsigned)(S::ROWS / 16) << 24;
-            // Where the tile is full the parts h' and m' of B along K are one operand of twice the columns, as are the accumulators: an instruction of
-            // 128 columns takes as long to read its operands as one of 256.
-            const unsigned both = B_SHARED_ALONG_K && walk.columns() == S::BN ? instruction + ((unsigned)(S::BN / 8) << 17) : 0;
+            // Where the tile is full the parts h' and m' of B are one operand of twice the columns, as are the accumulators: A is read once for both.
+            const unsigned both = walk.columns() == S::BN ? instruction + ((unsigned)(S::BN / 8) << 17) : 0;
             for (int s = 0; s < walk.steps && ended; ++s, ring.next()) {
                 const bool begins = s % S::CHUNK == 0;
                 const unsigned set = chunk & 1, to = accumulators + set * S::SET;
