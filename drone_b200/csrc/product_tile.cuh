@@ -63,11 +63,11 @@ template <typename T> struct TileShape {
     static constexpr int PITCH = sizeof(T) == 4 ? BN + 4 : 36;
     static constexpr int shared(int stages, int out_warps) { return 1024 + stages * STAGE + (sizeof(T) == 4 ? ROWS : out_warps * 32) * PITCH * 4; }
 };
-// Warps that take tiles out, threads that bring operands.  (17 warps and more leave 96 registers a thread.)
-template <Bring BRING> constexpr int kOutWarps = BRING == kCopied ? 16 : 8;
-constexpr int kBringThreads = 256;
+// Warps that take tiles out, threads that bring operands.
+template <Bring BRING> constexpr int kOutWarps = BRING == kCopied ? 16 : BRING == kImage ? 8 : 4;
+template <Bring BRING> constexpr int kBringThreads = BRING == kCopied ? 0 : BRING == kImage ? 256 : 512;
 template <Bring BRING> constexpr int kBringFrom = (kOutWarps<BRING> + 2) * 32;
-template <Bring BRING> constexpr int kProductThreads = kBringFrom<BRING> + (BRING == kCopied ? 0 : kBringThreads);
+template <Bring BRING> constexpr int kProductThreads = kBringFrom<BRING> + kBringThreads<BRING>;
 
 __device__ __forceinline__ unsigned shared_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrier_init(unsigned bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); }
@@ -178,15 +178,15 @@ __device__ __forceinline__ void store_values(unsigned at, unsigned plane_bytes, 
 
 // What a thread brings of an operand's tile in each step.  Neighbouring threads have neighbouring values: 16 bytes each where rows allow it,
 // else pairs (lanes with 32 bytes each of rows that are not on 16 bytes touch four times the lines with every load).
-template <int R, bool ALONG_K>
+template <int THREADS, int R, bool ALONG_K>
 struct Share {
     using S = TileShape<float>;
     using L = SharedLayout<S::KS, ALONG_K>;
-    static constexpr int WIDTH = ALONG_K ? S::KS : R, VALUES = R * S::KS / kBringThreads;
+    static constexpr int WIDTH = ALONG_K ? S::KS : R, VALUES = R * S::KS / THREADS;
     static constexpr unsigned PLANE = R * S::KS * 2;
     struct Values { float v[VALUES]; };
     Operand<float> from;
-    template <int V> static constexpr int APART = kBringThreads / (WIDTH / V);      // rows between a thread's values
+    template <int V> static constexpr int APART = THREADS / (WIDTH / V);      // rows between a thread's values
     int row, column;                  // of its first
     const float *at = nullptr;
     int limit = 0, k = 0;             // rows or columns of the tile that exist; of K until the share's end
@@ -473,7 +473,7 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
-            barrier_init(full + 8 * s, (BRING == kCopied ? 0 : kBringThreads / 32) + (BRING == kThrough ? 0 : 1));
+            barrier_init(full + 8 * s, kBringThreads<BRING> / 32 + (BRING == kThrough ? 0 : 1));
             barrier_init(empty + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -690,8 +690,8 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
         // Bring what goes through registers, DEPTH steps ahead.
         constexpr int DEPTH = BRING == kImage ? 3 : 2;      // by the registers that a step takes: 16 or 32
         const int thread = threadIdx.x - kBringFrom<BRING>;
-        Share<S::ROWS, A_ALONG_K> a(p.A, thread);
-        Share<S::BN, B_ALONG_K> b(p.B, thread);
+        Share<kBringThreads<BRING>, S::ROWS, A_ALONG_K> a(p.A, thread);
+        Share<kBringThreads<BRING>, S::BN, B_ALONG_K> b(p.B, thread);
         typename decltype(a)::Values va[DEPTH];
         typename decltype(b)::Values vb[BRING == kThrough ? DEPTH : 1];
         int s = 0;
