@@ -9,10 +9,10 @@
 //   kThrough   floats: both through registers
 //
 // Floats are split into three bfloat16 of 8 bits each, x = h + m + l exactly (but for values below 2^-110), and six of the nine products are added:
-// h h' in one accumulator, h m' + m h' + m m' + h l' + l h' in a second one that is 2^-8 of it, so that neither loses bits of the other.
-// The rest is below 2^-25 of |x y|.  The accumulators cut off what they cannot hold, half a unit an addition in the mean and always towards
-// 0: after every 256 of K they are added up in shared memory, rounding to nearest, and begin anew.  An output that is not finite (infinities split into NaN, values within
-// 2^-9 of the largest float round to infinity) is computed again from the operands.
+// h h' in one accumulator, h m' + m h' + m m' + h l' + l h' in a second one that is 2^-7 of it, so that neither loses bits of the other.
+// The rest is below 2^-22 of |x y|, and 2^-25 in the mean.  The accumulators cut off what they cannot hold, half a unit an addition in the mean and always
+// towards 0: after every 256 of K they are added up in shared memory, rounding to nearest, and begin anew.  h is cut off, so that a finite x has
+// a finite one.  Infinities and NaN have themselves for h (and NaN for m): where the first accumulator is not finite it is the result.
 //
 // All waits end after two seconds; a block whose wait did leaves NaN in its outputs.
 //
@@ -157,6 +157,11 @@ __device__ __forceinline__ unsigned bf16_pair(float low, float high) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(low, high);
     return reinterpret_cast<const unsigned &>(p);
 }
+__device__ __forceinline__ unsigned bf16_pair_cut(float low, float high) {      // towards 0
+    unsigned pair;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(pair) : "f"(high), "f"(low));
+    return pair;
+}
 // Pairs of floats in three pairs of bfloat16.
 template <int V>
 __device__ __forceinline__ void split_values(const float *v, unsigned (&planes)[3][V / 2]) {
@@ -165,7 +170,7 @@ __device__ __forceinline__ void split_values(const float *v, unsigned (&planes)[
         unsigned a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]);
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
-            const unsigned pair = planes[q][i] = bf16_pair(__uint_as_float(a), __uint_as_float(b));
+            const unsigned pair = planes[q][i] = q == 0 ? bf16_pair_cut(__uint_as_float(a), __uint_as_float(b)) : bf16_pair(__uint_as_float(a), __uint_as_float(b));
             if (q == 2) break;
             // what is left of both, in one instruction (the products with -1 are exact)
             asm("{\n.reg .b64 x, y, m;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nmov.b64 m, 0xbf800000bf800000;\nfma.rn.f32x2 x, y, m, x;\nmov.b64 {%0, %1}, x;\n}"
@@ -277,15 +282,6 @@ __device__ __forceinline__ void load_accumulators16(unsigned at, float *v) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// One output from the operands, for those that the split does not give.
-template <typename T, bool A_ALONG_K, bool B_ALONG_K>
-__device__ __noinline__ float plain_product(Operand<T> A, Operand<T> B, long long m, int n, int k0, int k1) {
-    float acc = 0;
-    for (int k = k0; k < k1; ++k)
-        acc = fmaf(to_float(A.at[A_ALONG_K ? m * A.ld + k : k * A.ld + m]), to_float(B.at[B_ALONG_K ? n * B.ld + k : k * B.ld + n]), acc);
-    return acc;
 }
 
 // One lane of a warp whose lanes go the same way.  (A branch of one thread by its number would leave the compiler without uniform registers, in
@@ -541,35 +537,28 @@ product_tile_kernel(const __grid_constant__ ProductArgs<T, BRING, A_ALONG_K, B_A
                         const unsigned set = chunk & 1, at = accumulators + ((unsigned)lane_row << 16) + set * S::SET + first;
                         ended = ended && barrier_wait(done + 8 * set, (chunk >> 1) & 1);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        bool fine = true;
 #pragma unroll 1
                         for (int c = 0; c < COLUMNS && c < width; c += 16) {
                             float a[16], b[16];
                             load_accumulators16(at + c, a);
                             load_accumulators16(at + S::BN + c, b);
 #pragma unroll
+                            for (int i = 0; i < 16; ++i) a[i] += fabsf(a[i]) < INFINITY ? b[i] : 0.f;
+#pragma unroll
                             for (int i = 0; i < 16; i += 4) {
                                 float4 *const to = reinterpret_cast<float4 *>(row + c + i);
-                                float4 v = make_float4(a[i] + b[i], a[i + 1] + b[i + 1], a[i + 2] + b[i + 2], a[i + 3] + b[i + 3]);
+                                float4 v = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
                                 if (s > 0) {
                                     const float4 before = *to;
                                     v = make_float4(before.x + v.x, before.y + v.y, before.z + v.z, before.w + v.w);
                                 }
                                 if (!ended) v = make_float4(NAN, NAN, NAN, NAN);      // a wait was given up: nothing plausible comes out
-                                fine = fine && fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
                                 *to = v;
                             }
                         }
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if ((threadIdx.x & 31) == 0) barrier_arrive(taken + 8 * set);
-                        if (s + S::CHUNK >= walk.steps && !fine && ended && (int)(threadIdx.x & 31) < rows) {      // what the split does not give
-#pragma unroll 1
-                            for (int c = 0; c < COLUMNS && c < width; ++c)
-                                if (!(fabsf(row[c]) < INFINITY))
-                                    row[c] = plain_product<T, A_ALONG_K, B_ALONG_K>(p.A, p.B, walk.m0 + lane_row + (threadIdx.x & 31), walk.n0 + first + c, walk.k0, walk.k1);
-                        }
-                        __syncwarp();
                     }
 #pragma unroll 1
                     for (int c = 0; c < COLUMNS; c += 32) put(piece + c, c);

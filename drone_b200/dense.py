@@ -166,13 +166,15 @@ def linear_backward(grad, x, w, pre=None, activation=None, transposed=False, bia
     grad_b = torch.empty(outputs, dtype=torch.float32, device=device) if bias else None
     with _Call(device) as call:
         dz, ldz = grad, ldg
-        if act != ACT_NONE:
+        # 16-bit rows that are not on 16 bytes are copied to rows that are here, once for both products
+        own = act != ACT_NONE or (dtype != torch.float32 and (ldg % 8 != 0 or grad.data_ptr() % 16 != 0))
+        if own:
             ldz = outputs if dtype == torch.float32 else (outputs + 7) // 8 * 8      # rows on 16 bytes, as the products want them
             dz = torch.empty((n, ldz), dtype=dtype, device=device)
-        if act != ACT_NONE or bias:
+        if own or bias:
             size = call.scratch("drone_activation_gradient_scratch", kind, n, outputs) if bias else (None, 0)
             call("drone_activation_gradient", kind, n, outputs, grad.data_ptr(), ldg, _pointer(pre) if act != ACT_NONE else None,
-                 ldp if act != ACT_NONE else 0, act, dz.data_ptr() if act != ACT_NONE else None, ldz, _pointer(grad_b), _pointer(size[0]), size[1])
+                 ldp if act != ACT_NONE else 0, act, dz.data_ptr() if own else None, ldz, _pointer(grad_b), _pointer(size[0]), size[1])
         if input_gradient:
             size = call.scratch("drone_linear_scratch", kind, n, outputs, inputs, dz.data_ptr(), ldz, w.data_ptr(), ldw, int(not flipped))
             call("drone_linear", kind, n, outputs, inputs, dz.data_ptr(), ldz, w.data_ptr(), ldw, int(not flipped), None, ACT_NONE, None, 0,

@@ -120,6 +120,30 @@ def test_products_of_floats_are_floats(cuda_device):
     assert ((got - want).abs() <= 2 * STEP * want.abs() + 2.0 ** -133).all()
 
 
+def test_large_floats_in_tiles(cuda_device):
+    """The same through many rows: values up to the largest float beside others, weights of 0, products that leave the range."""
+    gen = torch.Generator(cuda_device).manual_seed(12)
+    top = 3.4028234663852886e38
+    x = rows_of(gen, 700, 40, torch.float32)
+    w = rows_of(gen, 40, 200, torch.float32)
+    x[5], x[6], x[7], x[8, 3] = 0, 0, 0, 0
+    x[5, 1], x[6, 2], x[7, 30], x[8, 3] = top, -top, 3.39e38, 1e-44
+    w[1, 7], w[2, 9], w[30, 11], w[1, 12] = 0, 0, 0, 1e-30
+    got, want = dense.linear(x, w), x.double() @ w.double()
+    finite = want.abs() <= top
+    assert torch.equal(got.isfinite(), finite) and torch.equal(torch.sign(got[~finite]).double(), torch.sign(want[~finite]))
+    bound = (40 + 16) * STEP * (x.double().abs() @ w.double().abs()) + 2.0 ** -133
+    assert ((got - want).abs()[finite] <= bound[finite]).all()
+    g = torch.zeros((700, 200), device="cuda")
+    g[5, 3], g[6, 3], g[9, 4] = 1e-3, 1e-3, 2
+    dw = dense.linear_backward(g, x, w, input_gradient=False)[1]
+    want = x.double().t() @ g.double()
+    assert ((dw - want).abs() <= (700 + 16) * STEP * (x.double().abs().t() @ g.double().abs()) + 2.0 ** -133).all()
+    x[9, 5], x[10, 6] = math.inf, math.nan
+    dw = dense.linear_backward(g + 1e-3, x, w, input_gradient=False)[1]
+    assert (dw[5] == math.inf).all() and dw[6].isnan().all() and dw[7:].isfinite().all() and dw[:1].isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [3, 300])
 def test_linear_of_infinities(cuda_device, dtype, n):
