@@ -113,8 +113,9 @@ struct LongSum {
 
 // Rows of (PER - 1) * L + 1 to PER * L classes, L lanes a row: logits and exponentials stay in registers, the teacher's shares are added up in
 // shared memory, where the lane of an entry finds its class.
-// 2.4 M rows of 47 classes, 8 entries, labels: 1.18 GB in 341 us (53 % of the copy rate; instructions, and the round trips of a row's reductions); as exponentials by division and expf, computed twice, and every
-// entry shown to every lane 1171 us.
+// 2.4 M rows of 47 classes, 8 entries, labels: 1.18 GB in 341 us (53 % of the copy rate; instructions, and the round trips of a row's
+// reductions); with 74 registers instead of 64 421; as exponentials by division and expf, computed twice, and every entry shown to every
+// lane 1171 us.
 template <typename T, int L, int PER, bool HARD>
 __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<T> p) {
     constexpr int ROWS = 32 / L;      // of a warp

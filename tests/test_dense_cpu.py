@@ -80,7 +80,8 @@ def test_distillation_refuses(change):
 def test_scratch_sizes_refuse():
     size = C.c_longlong(0)
     for name, args in (("drone_linear_scratch", (3, 5, 4, 4, P, 4, P, 4, 0)), ("drone_linear_scratch", (0, -1, 4, 4, P, 4, P, 4, 0)),
-                       ("drone_linear_scratch", (0, 5, 0, 4, P, 4, P, 4, 0)), ("drone_linear_scratch", (0, 5, 4, 4, P, 4, P, 4, 3)), ("drone_activation_gradient_scratch", (0, -1, 4)), ("drone_activation_gradient_scratch", (0, 5, 0)), ("drone_activation_gradient_scratch", (1, (1 << 30) + 1, 4)),
+                       ("drone_linear_scratch", (0, 5, 0, 4, P, 4, P, 4, 0)), ("drone_linear_scratch", (0, 5, 4, 4, P, 4, P, 4, 3)), 
+                       ("drone_activation_gradient_scratch", (0, -1, 4)), ("drone_activation_gradient_scratch", (0, 5, 0)), ("drone_activation_gradient_scratch", (1, (1 << 30) + 1, 4)),
                        ("drone_activation_gradient_scratch", (7, 5, 4)),
                        ("drone_linear_weight_gradient_scratch", (0, -1, 4, 4, P, 4, P, 4, 0)), ("drone_linear_weight_gradient_scratch", (9, 5, 4, 4, P, 4, P, 4, 0)),
                        ("drone_linear_weight_gradient_scratch", (0, 5, 4, 4, P, 4, P, 4, 2)), ("drone_layer_norm_backward_scratch", (0, -1, 4)),
