@@ -73,7 +73,8 @@ def _pointer(t):
 
 
 def _activation(name):
-    _require(name in _ACTIVATIONS, "activation %r is none of none, relu, gelu, silu", name)
+    if name not in _ACTIVATIONS:
+        raise ValueError("activation %r is none of none, relu, gelu, silu" % (name,))
     return _ACTIVATIONS[name]
 
 
@@ -110,13 +111,17 @@ class _Call:
 def _weights(w, inputs, dtype, device, transposed):
     """Distance between the weights' rows, their other width and whether they lie as [outputs, inputs].  The transposed view of a
     contiguous matrix is read as that matrix."""
-    _require(isinstance(w, torch.Tensor) and w.dim() == 2, "the weights are not a matrix")
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise ValueError("the weights are not a matrix")
     if w.stride(1) != 1 and w.stride(0) == 1:
         w, transposed = w.t(), not transposed
     ldw = _matrix("the weights", w, dtype=dtype, device=device)
-    _require(w.shape[1 if transposed else 0] == inputs, "the weights are for rows of %d, not of %d", w.shape[1 if transposed else 0], inputs)
-    outputs = w.shape[0 if transposed else 1]
-    _require(max(inputs, outputs) <= _MAX_WIDTH, "weights of %d x %d: at most %d each way", *w.shape, _MAX_WIDTH)
+    rows, columns = w.shape
+    taken, outputs = (columns, rows) if transposed else (rows, columns)
+    if taken != inputs:
+        raise ValueError("the weights are for rows of %d, not of %d" % (taken, inputs))
+    if rows > _MAX_WIDTH or columns > _MAX_WIDTH:
+        raise ValueError("weights of %d x %d: at most %d each way" % (rows, columns, _MAX_WIDTH))
     return ldw, outputs, transposed
 
 
@@ -132,7 +137,7 @@ def linear(x, w, bias=None, activation=None, residual=None, transposed=False, ou
     act = _activation(activation)
     made = out is None
     if made:
-        out = torch.empty((n, outputs), dtype=dtype, device=device)
+        out = x.new_empty((n, outputs))
     ldy = outputs if made else _matrix("out", out, n, outputs, dtype, device)
     ldr = _matrix("the residual", residual, n, outputs, dtype, device) if residual is not None else 0
     ldp = _matrix("pre", pre, n, outputs, dtype, device) if pre is not None else 0
@@ -197,11 +202,11 @@ def layer_norm(x, scale, shift, eps=1e-5, relu=False, out=None):
     _vector("shift", shift, f, torch.float32, device)
     _require(eps > 0, "eps=%r", eps)
     if out is None:
-        out, ldy = torch.empty((n, f), dtype=x.dtype, device=device), f
+        out, ldy = x.new_empty((n, f)), f
     else:
         ldy = _matrix("out", out, n, f, x.dtype, device)
         _apart("out", out, (x, True), (scale, False), (shift, False))
-    mean, rstd = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
+    mean, rstd = scale.new_empty(n), scale.new_empty(n)
     with _Call(device) as call:
         call("drone_layer_norm", _TYPES[x.dtype], n, f, x.data_ptr(), ldx, scale.data_ptr(), shift.data_ptr(), float(eps), int(bool(relu)),
              out.data_ptr(), ldy, mean.data_ptr(), rstd.data_ptr())
@@ -221,8 +226,8 @@ def layer_norm_backward(grad, x, scale, mean, rstd, out=None, mirror_rows=None):
     _vector("rstd", rstd, n, torch.float32, device)
     if mirror_rows is not None:
         _vector("mirror_rows", mirror_rows, n, torch.int32, device)
-    grad_x = torch.empty((n, f), dtype=dtype, device=device)
-    grad_scale, grad_shift = (torch.empty(f, dtype=torch.float32, device=device) for _ in range(2))
+    grad_x = x.new_empty((n, f))
+    grad_scale, grad_shift = scale.new_empty(f), scale.new_empty(f)
     with _Call(device) as call:
         sums, floats = call.scratch("drone_layer_norm_backward_scratch", _TYPES[dtype], n, f)
         call("drone_layer_norm_backward", _TYPES[dtype], n, f, grad.data_ptr(), ldg, x.data_ptr(), ldx, scale.data_ptr(), mean.data_ptr(),
