@@ -88,7 +88,8 @@ __device__ __forceinline__ float activate(float z) {
         if (sizeof(T) == 4) return 0.5f * z * (1.f + erff(z * 0.70710678f));
         float bell;
         const float tail = normal_tail(z, &bell);
-        return fmaf(-fabsf(z), tail, z < 0.f ? 0.f : z);      // z Phi(z), of either sign; a NaN is the tail's
+        // z Phi(z), of either sign; a NaN is the tail's.  At +infinity the tail is 0, and its product with z would be a NaN of its own
+        return z == INFINITY ? z : fmaf(-fabsf(z), tail, z < 0.f ? 0.f : z);
     } else if constexpr (ACTIVATION == DRONE_ACT_SILU) {
         return sizeof(T) == 4 ? z / (1.f + expf(-z)) : z * reciprocal_fast(1.f + exp2_fast(z * -1.44269504f));
     } else {
