@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from drone_b200 import dense
-from test_dense_gpu import TYPES, activated, rows_of
+from test_dense_gpu import STEP, TYPES, activated, check_rounded, rows_of, slope
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,23 @@ def test_activations_of_infinities(cuda_device, activation, n, dtype):
         inf = want.abs() > top      # 1e30 is infinite in 16 bits of a 5-bit exponent
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), inf) and (got[inf] > 0).all()
         assert torch.equal(pre.isnan(), z.isnan()) and torch.equal(pre.isinf(), z.abs() > top)
+
+
+def test_gelu_tails_of_16_bits(cuda_device):
+    """z Phi(z) and its slope as good as their types as far out as there is anything.  The tail's polynomial is good to 4.4e-5 of the value; the exponent of its
+    bell, up to 126 and off by three half steps, makes 126 * 3 * 2^-24 * ln 2 = 1.6e-5 of it; together 2^-14.  Below 2^-126 the exponential is 0."""
+    for dtype in (torch.bfloat16, torch.float16):
+        z = torch.linspace(-14, 14, 4001, device="cuda").to(dtype)[:, None]
+        one = torch.ones((1, 1), dtype=dtype, device="cuda")
+        phi = lambda v: 0.5 * torch.special.erfc(-v * math.sqrt(0.5))      # torch.special.ndtr is a difference from 1, good to 2^-53 of that
+        got, want = dense.linear(z, one, activation="gelu"), z.double() * phi(z.double())
+        gone = 16 * 2.0 ** -126
+        tail = z.double().abs() * phi(-z.double().abs())
+        check_rounded(got, want, 2.0 ** -14 * tail + 2 * STEP * want.abs() + gone, dtype)
+        # of one row the bias gradient is the gradient before the activation, not rounded
+        pre = z.t().contiguous()
+        got = dense.linear_backward(torch.ones_like(pre), one, one.expand(1, pre.shape[1]).contiguous(), pre=pre, activation="gelu")[2]
+        v = pre.double()[0]
+        bell = torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+        size = phi(-v.abs()) + v.abs() * bell
+        assert ((got - (phi(v) + v * bell)).abs() <= 2.0 ** -14 * size + 2 * STEP * (v >= 0) + gone).all()
