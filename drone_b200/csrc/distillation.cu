@@ -10,7 +10,6 @@
 #include "dense_types.cuh"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace drone {
 
@@ -90,15 +89,14 @@ __device__ __forceinline__ void write_sums(LossSums s, LossSums *sums) {
 }
 
 // Exponentials are exp2_fast of (z - the row's maximum) log2(e) / t, whose rounding is off by as much.  (The difference comes first: a row whose
-// logits are all the type's lowest value is a row of equal ones.)
+// logits are all the type's lowest value is a row of equal ones, and what all of them have in common leaves no rounding behind.  One multiply-add on
+// the maximum times log2(e) / t would leave 2^-24 of that product in the exponent: 2.7e-5 of a share at logits around 1000.)
 constexpr float kLog2e = 1.44269504f;
 __device__ __forceinline__ float log_fast(float x) {      // off by 2^-22 and 2^-22 of the value
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y * 0.693147181f;
 }
-// Below this a logit times log2(e) / t is finite for every t that is allowed, and one multiply-add forms the exponent.
-constexpr float kLargeLogit = 1e30f;
 
 // A sum of floats with what its additions cut off.
 struct LongSum {
@@ -295,26 +293,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
         // adds values of which `to` is the largest
         auto add = [&](const float *z, int count, float to) {
             if (to > m) {
-                if (m != -INFINITY) {
-                    s *= exp2_fast((m - to) * scale);
-                    if (HARD) s1 *= exp2_fast((m - to) * kLog2e);
-                }
+                s *= exp2_fast((m - to) * scale);
+                if (HARD) s1 *= exp2_fast((m - to) * kLog2e);
                 m = to;
             }
-            if (fabsf(m) < kLargeLogit) {
-                const float shift = m * scale, shift1 = m * kLog2e;
+            const float from = m == -INFINITY ? 0.f : m;      // minus infinity adds 0, also where the thread has seen nothing else
 #pragma unroll
-                for (int k = 0; k < count; ++k) {
-                    s += exp2_fast(fmaf(z[k], scale, -shift));
-                    if (HARD) s1 += exp2_fast(fmaf(z[k], kLog2e, -shift1));
-                }
-            } else {      // minus infinity adds 0, also where the thread has seen nothing else
-#pragma unroll
-                for (int k = 0; k < count; ++k) {
-                    const float d = m == -INFINITY && z[k] == -INFINITY ? -INFINITY : z[k] - m;
-                    s += exp2_fast(d * scale);
-                    if (HARD) s1 += exp2_fast(d * kLog2e);
-                }
+            for (int k = 0; k < count; ++k) {
+                s += exp2_fast((z[k] - from) * scale);
+                if (HARD) s1 += exp2_fast((z[k] - from) * kLog2e);
             }
         };
         int i = tid;
@@ -389,16 +376,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
         }
         const float per_ts = 1.f / sum.z, soft_weight = any ? p.soft * t * (isnan(sum.z) ? NAN : 1.f) : 0.f, per_s = soft_weight / sum.x;
         const float hard_weight = label != 0.f ? p.hard * label : 0.f, per_s1 = hard_weight / sum.y;
-        const bool ordinary = fabsf(row_max) < kLargeLogit;
-        const float shift = row_max * scale, shift1 = row_max * kLog2e;
         // the gradient of a class whose logit is z, without the teacher's share and the label
-        auto gradient = [&](float z, bool fast) {
-            float d = exp2_fast(fast ? fmaf(z, scale, -shift) : (z - row_max) * scale) * per_s;
-            if (HARD) d = fmaf(exp2_fast(fast ? fmaf(z, kLog2e, -shift1) : (z - row_max) * kLog2e), per_s1, d);
+        auto gradient = [&](float z) {
+            float d = exp2_fast((z - row_max) * scale) * per_s;
+            if (HARD) d = fmaf(exp2_fast((z - row_max) * kLog2e), per_s1, d);
             return d;
         };
-        auto write = [&](auto fast) {
-            constexpr bool FAST = decltype(fast)::value;
+        auto write = [&] {
             int i = tid;
             for (; i + (AT_ONCE - 1) * THREADS < vectors; i += THREADS * AT_ONCE) {
                 Vector w[AT_ONCE];
@@ -409,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
                     float z[V];
                     w[b].get(z);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) z[k] = gradient(z[k], FAST);
+                    for (int k = 0; k < V; ++k) z[k] = gradient(z[k]);
                     w[b].set(z);
                     *reinterpret_cast<Vector *>(g + head + (long long)(i + b * THREADS) * V) = w[b];
                 }
@@ -419,21 +403,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
                 float z[V];
                 w.get(z);
 #pragma unroll
-                for (int k = 0; k < V; ++k) z[k] = gradient(z[k], FAST);
+                for (int k = 0; k < V; ++k) z[k] = gradient(z[k]);
                 w.set(z);
                 *reinterpret_cast<Vector *>(g + head + (long long)i * V) = w;
             }
             if (VEC) {
                 const int c = tid < head ? tid : tail + tid - head;
-                if (tid < head || (tid >= head && c < classes)) g[c] = from_float<T>(gradient(to_float(x[c]), FAST));
+                if (tid < head || (tid >= head && c < classes)) g[c] = from_float<T>(gradient(to_float(x[c])));
             }
         };
         if (!any && label == 0.f) {
             for (int c = tid; c < classes; c += THREADS) g[c] = from_float<T>(0.f);
-        } else if (ordinary) {
-            write(std::true_type());
         } else {
-            write(std::false_type());
+            write();
         }
         __syncthreads();
         if (first) {      // the first entry of a class has the share of all of them
@@ -441,7 +423,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
             if (again)
                 for (int j = tid + 1; j < p.top; ++j)
                     if (entry_class[j] == c_mine) all += entry_weight[j];
-            float d = gradient(z_mine, ordinary) - soft_weight * (all * per_ts);
+            float d = gradient(z_mine) - soft_weight * (all * per_ts);
             if (HARD && c_mine == truth) d -= hard_weight;
             g[c_mine] = from_float<T>(d);
         }
@@ -449,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
             bool entry = false;
             if (tid < p.top) entry = c_mine == truth;
             entry = __syncthreads_or(entry);
-            if (!entry && tid == 0 && truth >= 0 && label != 0.f) g[truth] = from_float<T>(gradient(at_truth, ordinary) - hard_weight);
+            if (!entry && tid == 0 && truth >= 0 && label != 0.f) g[truth] = from_float<T>(gradient(at_truth) - hard_weight);
         }
         if (tid == 0) {
             if (any) {

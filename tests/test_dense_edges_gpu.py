@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from drone_b200 import dense
-from test_dense_gpu import STEP, TYPES, activated, check_rounded, rows_of, slope
+from test_dense_gpu import STEP, TYPES, activated, check_rounded, distilled, rows_of, slope
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,26 @@ def test_gelu_tails_of_16_bits(cuda_device):
         bell = torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
         size = phi(-v.abs()) + v.abs() * bell
         assert ((got - (phi(v) + v * bell)).abs() <= 2.0 ** -14 * size + 2 * STEP * (v >= 0) + gone).all()
+
+
+@pytest.mark.parametrize("c", [47, 200, 257, 4096, 9001])
+@pytest.mark.parametrize("t", [1.0, 4.0, 1e-3, 1e-6])
+def test_logits_with_an_offset(cuda_device, c, t):
+    """What all logits of a row have in common leaves no trace, however large: a row's shares follow from differences, which are exact or off by half a step.  An exponent x
+    that is off by 4 half steps moves exp(-x) by x exp(-x) of them, less than one."""
+    gen = torch.Generator(cuda_device).manual_seed(c)
+    offsets = [0.0, 100.0, -1e4, 1e4, 1e5, 1e6, -1e9, 1e10, -1e10, 1e20, 3e30, -3e38]
+    n = len(offsets)
+    logits = rows_of(gen, n, c, torch.float32, scale=3.0 * min(t, 1.0)) + torch.tensor(offsets, device="cuda")[:, None]
+    logits[::2, 5:9] = -3e38      # classes that are masked with a low value beside the others
+    teacher, classes = rows_of(gen, n, 4, torch.float32, scale=min(t, 1.0)), torch.randint(9, c, (n, 4), device="cuda", generator=gen)
+    truth, labelled = torch.randint(9, c, (n,), device="cuda", generator=gen), torch.ones(n, dtype=torch.bool, device="cuda")
+    off = (16 + c / 64) * STEP
+    for r in range(n):      # a row at a time, so that each has its own bound
+        at = slice(r, r + 1)
+        loss, grad = dense.distillation_loss(logits[at], teacher[at], classes[at], temperature=t, truth=truth[at], labelled=labelled[at], soft=0.5, hard=0.5)
+        want_loss, want = distilled(logits[at], teacher[at], classes[at], t, truth[at], labelled[at], 0.5, 0.5)
+        check_rounded(grad, want, off * (0.5 * t + 0.5) * torch.ones_like(want), torch.float32)
+        apart = (logits[at].double().max() - logits[at].double().gather(1, torch.cat([classes[at], truth[at][:, None]], dim=1))).abs().max().item()
+        assert abs(loss[0] - want_loss[0]) <= off * t * t * (8 + (apart + 10 * t) / t), (offsets[r], loss, want_loss)
+        assert abs(loss[1] - want_loss[1]) <= off * (8 + apart), (offsets[r], loss, want_loss)
