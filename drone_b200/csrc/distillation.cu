@@ -33,7 +33,7 @@ struct Distillation {
     int top;
     const long long *truth;
     const unsigned char *labelled;
-    float temperature, per_temperature, soft, hard;
+    float temperature, soft, hard;
     T *grad;
     long long ldg;
     LossSums *sums;
@@ -44,12 +44,13 @@ __device__ __forceinline__ float load_as(const void *p, long long i, int type) {
     return type == DRONE_F32 ? __ldg((const float *)p + i) : type == DRONE_BF16 ? to_float(((const __nv_bfloat16 *)p)[i]) : to_float(((const __half *)p)[i]);
 }
 
-// Entry j of a row: class (-1: none) and value over the temperature.  A class that does not exist makes the value NaN, and with it the row.
+// Entry j of a row: class (-1: none) and value.  (Over the temperature only as a difference from the largest: the quotient of a value at either end of its
+// type need not be a float.)  A class that does not exist makes the value NaN, and with it the row.
 template <typename T>
 __device__ __forceinline__ int teacher_entry(const Distillation<T> &p, long long row, int j, float *value) {
     const long long c = __ldg(p.classes_of + row * p.ldc + j);
     const float v = load_as(p.teacher, row * p.ldt + j, p.teacher_type);
-    *value = c >= p.classes ? NAN : v * p.per_temperature;
+    *value = c >= p.classes ? NAN : v;
     if (c < 0 || v == -INFINITY) return -1;
     return c >= p.classes ? 0 : (int)c;
 }
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<
 #pragma unroll
     for (int u = 0; u < PER; ++u) target[gl + u * L] = 0;
     __syncwarp();
-    const float t = p.temperature, per_t = p.per_temperature, scale = kLog2e / t;
+    const float t = p.temperature, scale = kLog2e / t;
     LongSum soft_sum, hard_sum;
     float soft_rows = 0, hard_rows = 0;      // of this group: fewer than 2^24
     auto inside = [&](int u) { return u < PER - 1 || gl + u * L < classes; };
@@ -179,12 +180,12 @@ __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<
                 s1 += v[u];
             }
         }
-        // the weight of an entry in the teacher's softmax, and its part of the distance
+        // the weight of an entry in the teacher's softmax, and its part of the distance, times the temperature
         auto weigh = [&](int c, float of) {
             if (c < 0) return 0.f;
-            const float w = exp2_fast((of - tm) * kLog2e);
+            const float w = exp2_fast((of - tm) * scale);
             ts += w;
-            if (w != 0.f) apart += w * ((of - tm) - (to_float(x[c]) - m) * per_t);
+            if (w != 0.f) apart += w * ((of - tm) - (to_float(x[c]) - m));
             return w;
         };
         const float weight0 = weigh(c0, value0);
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<
         share(c0, weight0);
         for (int j0 = L; j0 < p.top; j0 += L) {
             const int c = j0 + gl < p.top ? teacher_entry(p, row, j0 + gl, &value) : -1;
-            share(c, c >= 0 ? exp2_fast((value - tm) * kLog2e) : 0.f);
+            share(c, c >= 0 ? exp2_fast((value - tm) * scale) : 0.f);
         }
         if (HARD && gl == 0 && truth >= 0) target[truth] += hard_weight;
         __syncwarp();      // and from here on the gradient may lie on the logits
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<
         __syncwarp();
         if (live) {      // the same in every lane of the row
             if (some) {
-                soft_sum.add(t * t * (apart * per_ts - log_fast(ts) + log_fast(s)));
+                soft_sum.add(t * (apart * per_ts) + t * t * (log_fast(s) - log_fast(ts)));
                 soft_rows += 1;
             }
             if (HARD && label != 0.f) {
@@ -341,10 +342,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
         float4 sum = make_float4(m == -INFINITY ? s : s * exp2_fast((m - row_max) * scale), m == -INFINITY ? s1 : s1 * exp2_fast((m - row_max) * kLog2e), 0, 0);
         bool first = c_mine >= 0, again = false;
         if (c_mine >= 0) {
-            weight = expf(value - tm);
+            weight = expf((value - tm) / t);
             z_mine = to_float(x[c_mine]);
             sum.z = weight;
-            if (weight != 0.f) sum.w = weight * ((value - tm) - (z_mine - row_max) / t);
+            if (weight != 0.f) sum.w = weight * ((value - tm) - (z_mine - row_max));
             entry_weight[tid] = weight;
 #pragma unroll 4
             for (int j = 0; j < p.top; ++j) {
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
         }
         if (tid == 0) {
             if (any) {
-                sums.soft += (double)(t * t * (sum.w * per_ts - logf(sum.z) + logf(sum.x)));
+                sums.soft += (double)(t * (sum.w * per_ts) + t * t * (logf(sum.x) - logf(sum.z)));
                 sums.soft_rows += 1;
             }
             if (HARD && label != 0.f) {
@@ -511,7 +512,7 @@ int drone_distillation_loss(int type, int n_rows, int classes, const void *d_log
     cudaStream_t st = (cudaStream_t)stream;
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
-        const Distillation<T> p = {(const T *)d_logits, ld, d_teacher, ldt, teacher_type, d_classes, ldc, top, d_truth, d_labelled, temperature, 1 / temperature, soft,
+        const Distillation<T> p = {(const T *)d_logits, ld, d_teacher, ldt, teacher_type, d_classes, ldc, top, d_truth, d_labelled, temperature, soft,
                                    hard, (T *)d_grad, ld_grad, (LossSums *)d_scratch, n_rows, classes};
         return d_truth ? launch_distillation<T, true>(p, d_loss, st) : launch_distillation<T, false>(p, d_loss, st);
     });

@@ -72,3 +72,20 @@ def test_logits_with_an_offset(cuda_device, c, t):
         apart = (logits[at].double().max() - logits[at].double().gather(1, torch.cat([classes[at], truth[at][:, None]], dim=1))).abs().max().item()
         assert abs(loss[0] - want_loss[0]) <= off * t * t * (8 + (apart + 10 * t) / t), (offsets[r], loss, want_loss)
         assert abs(loss[1] - want_loss[1]) <= off * (8 + apart), (offsets[r], loss, want_loss)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [7, 47, 200, 300])
+def test_teachers_of_extreme_values(cuda_device, c, dtype):
+    """Entries at either end of their type, at temperatures whose quotient with them is no float: equal entries have equal shares, the others none."""
+    gen = torch.Generator(cuda_device).manual_seed(c)
+    low, top = torch.finfo(dtype).min, torch.finfo(dtype).max
+    for t in (1.0, 0.5, 1e-3, 1e-6):
+        logits, teacher = rows_of(gen, 6, c, torch.float32, scale=min(t, 1.0)), rows_of(gen, 6, 4, dtype)
+        classes = torch.arange(4, device="cuda").expand(6, 4).contiguous()
+        teacher[1], teacher[2, 1:], teacher[3], teacher[4, 2], teacher[5] = low, low, top, top, torch.tensor([low, top, -math.inf, low]).to(teacher)
+        loss, grad = dense.distillation_loss(logits, teacher, classes, temperature=t)
+        want_loss, want = distilled(logits, teacher, classes, t, None, None, 1.0, 0.0)
+        # teachers' values around 1 over t = 1e-6: a share is exp(-x) with x off by 4 half steps
+        check_rounded(grad, want, (16 + c / 64) * STEP * t * torch.ones_like(want), torch.float32)
+        assert abs(loss[0] - want_loss[0]) <= (16 + c / 64) * STEP * t * t * (20 + (teacher[0].max() - teacher[0].min()).item() / t)
