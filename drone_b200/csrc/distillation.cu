@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<
         if (HARD) {
             s1 = sum_of_lanes<L>(s1);
             per_s1 = reciprocal_fast(s1);
-            label = truth < 0 ? NAN : labelled ? 1.f : 0.f;
+            label = !labelled ? 0.f : truth < 0 ? NAN : 1.f;
             at_truth = truth < 0 ? 0.f : to_float(x[truth]) - m;
         }
         const float per_ts = reciprocal_fast(ts), soft_weight = some ? p.soft * t * (isnan(ts) ? NAN : 1.f) : 0.f, hard_weight = label != 0.f ? p.hard * label : 0.f;
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_ke
         if (HARD) {
             const long long wanted = __ldg(p.truth + row);
             const bool exists = wanted >= 0 && wanted < classes;
-            label = !exists ? NAN : __ldg(p.labelled + row) ? 1.f : 0.f;
+            label = !__ldg(p.labelled + row) ? 0.f : exists ? 1.f : NAN;
             truth = exists ? (int)wanted : -1;
             at_truth = exists ? to_float(x[truth]) : 0.f;
         }

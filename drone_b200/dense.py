@@ -239,7 +239,8 @@ def layer_norm_backward(grad, x, scale, mean, rstd, out=None, mirror_rows=None):
 def distillation_loss(logits, teacher, classes, temperature=1.0, truth=None, labelled=None, soft=1.0, hard=0.0):
     """(loss, gradient) of logits [n, classes] against a teacher's top logits: values `teacher` [n, top] of the classes `classes`
     [n, top] (int64; negative: no entry).  loss[0]: mean over the rows with an entry of temperature^2 * KL(teacher || model) over the
-    entries; loss[1]: mean cross-entropy over the labelled rows (truth int64, labelled bool).  The gradient is soft times that of the
+    entries; loss[1]: mean cross-entropy over the labelled rows (truth int64, labelled bool;
+    where a row is not labelled its truth may be anything, such as -1).  The gradient is soft times that of the
     first sum over rows plus hard times that of the second, not divided by the numbers of rows, as the graph model's own loss has it."""
     ld = _matrix("logits", logits)
     n, c, device = logits.shape[0], logits.shape[1], logits.device

@@ -89,3 +89,19 @@ def test_teachers_of_extreme_values(cuda_device, c, dtype):
         # teachers' values around 1 over t = 1e-6: a share is exp(-x) with x off by 4 half steps
         check_rounded(grad, want, (16 + c / 64) * STEP * t * torch.ones_like(want), torch.float32)
         assert abs(loss[0] - want_loss[0]) <= (16 + c / 64) * STEP * t * t * (20 + (teacher[0].max() - teacher[0].min()).item() / t)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [5, 47, 200, 300])
+def test_rows_without_a_label_need_none(cuda_device, c, dtype):
+    """-1 for vertices without a label, as the graph models' own truth has it: the bits of any other class there."""
+    gen = torch.Generator(cuda_device).manual_seed(c)
+    n = 70
+    logits, teacher, classes = rows_of(gen, n, c, dtype), rows_of(gen, n, 3, dtype), torch.randint(-1, c, (n, 3), device="cuda", generator=gen)
+    truth = torch.randint(0, c, (n,), device="cuda", generator=gen)
+    labelled = torch.rand(n, device="cuda", generator=gen) < 0.4
+    run = lambda given: dense.distillation_loss(logits, teacher, classes, truth=given, labelled=labelled, soft=0.5, hard=0.5)
+    want = run(truth)
+    for none in (-1, c, -(1 << 40), 1 << 40):
+        got = run(torch.where(labelled, truth, none))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[0].isfinite().all() and got[1].isfinite().all()
