@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<
         for (int u = 0; u < PER; ++u) {
             float d = fmaf(e[u], of_e, -target[gl + u * L]);
             if (HARD) d = fmaf(v[u], of_v, d);
+            if (!some && label == 0.f) d = 0.f;      // counts for nothing, also where 0 times its exponentials is not 0 (a branch around the row costs 4 % more)
             if (inside(u) && live) g[gl + u * L] = from_float<T>(d);
         }
         __syncwarp();

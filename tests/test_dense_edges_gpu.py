@@ -105,3 +105,24 @@ def test_rows_without_a_label_need_none(cuda_device, c, dtype):
     for none in (-1, c, -(1 << 40), 1 << 40):
         got = run(torch.where(labelled, truth, none))
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[0].isfinite().all() and got[1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [5, 47, 200, 300])
+def test_rows_that_count_for_nothing_may_hold_anything(cuda_device, c, dtype):
+    """Rows without entry and label, such as padding: whatever their logits are, their gradient is 0 and the others' results are what they are without them."""
+    gen = torch.Generator(cuda_device).manual_seed(c)
+    n = 40
+    logits, teacher, classes = rows_of(gen, n, c, dtype), rows_of(gen, n, 3, dtype), torch.randint(0, c, (n, 3), device="cuda", generator=gen)
+    truth, labelled = torch.randint(0, c, (n,), device="cuda", generator=gen), torch.rand(n, device="cuda", generator=gen) < 0.5
+    none = torch.zeros(n, dtype=torch.bool, device="cuda")
+    none[3::5] = True
+    classes[none], labelled = -1, labelled & ~none
+    for hard in (False, True):
+        run = lambda: dense.distillation_loss(logits, teacher, classes, **(dict(truth=truth, labelled=labelled, soft=0.5, hard=0.5) if hard else {}))
+        logits[none] = 0
+        want = run()
+        for value in (math.nan, math.inf, -math.inf, torch.finfo(dtype).min):
+            logits[none] = value
+            got = run()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (got[1][none] == 0).all(), value
