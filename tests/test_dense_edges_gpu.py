@@ -126,3 +126,20 @@ def test_rows_that_count_for_nothing_may_hold_anything(cuda_device, c, dtype):
             logits[none] = value
             got = run()
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (got[1][none] == 0).all(), value
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weight_gradients_over_very_many_rows(cuda_device, dtype, transposed):
+    """Tiles that fill the GPU by themselves, so that none is cut along the rows, and factors of one sign: an accumulator that cuts off with every addition must not run through
+    all of them.  It runs through 8192 rows, 512 additions of 16 products, which lose a step of the sum each (measured: 0.8 of one); what it holds then is added 49 times."""
+    gen = torch.Generator(cuda_device).manual_seed(1)
+    n, k, m = 400_003, 2048, 1280
+    x, g = (torch.rand((n, f), device="cuda", generator=gen).add_(0.5).to(dtype) for f in (k, m))
+    w = torch.zeros((m, k) if transposed else (k, m), dtype=dtype, device="cuda")
+    g *= 2.0 ** -8      # sums of 400,003 products stay below the largest of any type
+    dw = dense.linear_backward(g, x, w, transposed=transposed, bias=False, input_gradient=False)[1]
+    for i, j in ((0, 0), (k - 100, m - 100), (1000, 200)):
+        want = x[:, i:i + 100].double().t() @ g[:, j:j + 100].double()
+        got = dw[j:j + 100, i:i + 100].t() if transposed else dw[i:i + 100, j:j + 100]
+        check_rounded(got, want, (512 + 49 + 16) * STEP * want, dtype)
