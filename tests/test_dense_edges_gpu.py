@@ -1,11 +1,12 @@
 """Edges of the dense operators: infinities through the activations, tails, logits with an offset, values at the ends of their type, rows that count for nothing, sums over very
 many rows."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
-from drone_b200 import dense
+from drone_b200 import _lib, dense
 from test_dense_gpu import STEP, TYPES, activated, check_rounded, distilled, rows_of, slope
 
 pytestmark = pytest.mark.gpu
@@ -143,3 +144,53 @@ def test_weight_gradients_over_very_many_rows(cuda_device, dtype, transposed):
         want = x[:, i:i + 100].double().t() @ g[:, j:j + 100].double()
         got = dw[j:j + 100, i:i + 100].t() if transposed else dw[i:i + 100, j:j + 100]
         check_rounded(got, want, (512 + 49 + 16) * STEP * want, dtype)
+
+
+def in_tiles(x, w, transposed=False):
+    """Whether such a product of floats goes through tiles, whose operands are split: it asks for an image of the weights."""
+    size = C.c_longlong(0)
+    rows, outputs = x.shape[0], w.shape[0 if transposed else 1]
+    _lib.check(_lib.lib().drone_linear_scratch(_lib.F32, rows, x.shape[1], outputs, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), int(transposed), C.byref(size)))
+    return size.value > 0
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+def test_split_products_one_by_one(cuda_device, transposed):
+    """One product an output, of full mantissas and any size: six products of a float's parts leave two steps of it, or six of the smallest floats."""
+    gen = torch.Generator(cuda_device).manual_seed(2)
+    x = rows_of(gen, 700, 1, torch.float32) * torch.exp2(torch.randint(-60, 60, (700, 1), device="cuda", generator=gen).float())
+    w = rows_of(gen, 1, 200, torch.float32) * torch.exp2(torch.randint(-60, 60, (1, 200), device="cuda", generator=gen).float())
+    given = w.t().contiguous() if transposed else w
+    assert in_tiles(x, given, transposed)
+    want, got = x.double() * w.double(), dense.linear(x, given, transposed=transposed)
+    assert ((got - want).abs() <= 2 * STEP * want.abs() + 6 * 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("n,k,m", [(700, 256, 200), (700, 602, 128), (1000, 1025, 41), (600, 4096, 130)])
+def test_split_products_are_as_good_as_floats(cuda_device, n, k, m, transposed):
+    """Factors of one sign, where what is left out or cut off adds up: a product is off by 2 steps, an accumulator by one with each of its 16 additions of 16 products (times
+    two: there are two accumulators, the second far smaller), and every 256 of K the sum is rounded.  Without the third parts it would be 256 steps."""
+    gen = torch.Generator(cuda_device).manual_seed(k)
+    x, w = (torch.rand(shape, device="cuda", generator=gen) + 0.5 for shape in ((n, k), (k, m)))
+    given = w.t().contiguous() if transposed else w
+    assert in_tiles(x, given, transposed)
+    want, got = x.double() @ w.double(), dense.linear(x, given, transposed=transposed)
+    assert ((got - want).abs() <= (2 + 18 + k / 256) * STEP * want).all()
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+def test_split_products_of_infinities(cuda_device, transposed):
+    """Infinities and NaN in float tiles reach the outputs that they reach in the formula, forward and in the gradient of the rows."""
+    gen = torch.Generator(cuda_device).manual_seed(3)
+    x, w = rows_of(gen, 700, 70, torch.float32), rows_of(gen, 70, 150, torch.float32)
+    x[0, 3], x[1, 69], x[2, 40], x[650, 0] = math.inf, -math.inf, math.nan, math.inf
+    w[10, 7], w[69, 8], w[0, 149] = math.inf, 0, -math.inf
+    for rows, weights in ((x, w), (rows_of(gen, 700, 150, torch.float32), w.t())):
+        given = weights.t().contiguous() if transposed else weights.contiguous()
+        assert in_tiles(rows, given, transposed)
+        got, want = dense.linear(rows, given, transposed=transposed), rows.double() @ weights.double()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()) and torch.equal(got[want.isinf()].double(), want[want.isinf()])
+        fine = want.isfinite()
+        size = rows.double().abs().nan_to_num(0, 0, 0) @ weights.double().abs().nan_to_num(0, 0, 0)
+        check_rounded(got[fine], want[fine], ((rows.shape[1] + 16) * STEP * size)[fine], torch.float32)
