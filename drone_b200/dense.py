@@ -28,7 +28,7 @@ def _matrix(name, t, rows=None, width=None, dtype=None, device=None):
     try:
         (n, f), (apart, step), its = t.shape, t.stride(), t.dtype
         if ((its in _TYPES if dtype is None else its is dtype) and (t.is_cuda if device is None else t.device == device)
-                and (rows is None or n == rows) and (width is None or f == width) and f >= 1 and (n <= 1 or f <= apart < 1 << 31)
+                and (rows is None or n == rows) and (width is None or f == width) and f >= 1 and f <= (apart if n > 1 else f) < 1 << 31
                 and (step == 1 or f == 1 or n == 0) and n <= _MAX_ROWS):
             return apart if n > 1 else f
     except (AttributeError, TypeError, ValueError):
@@ -38,7 +38,7 @@ def _matrix(name, t, rows=None, width=None, dtype=None, device=None):
 
 def _refuse_matrix(name, t, rows, width, dtype, device):
     _require(isinstance(t, torch.Tensor) and t.dim() == 2, "%s is not a matrix", name)
-    _require(t.is_cuda and (device is None or t.device == device), "%s is on %s, not on %s", name, t.device, device or "a CUDA device")
+    _require(t.is_cuda if device is None else t.device == device, "%s is on %s, not on %s", name, t.device, device or "a CUDA device")
     _require(t.dtype in _TYPES if dtype is None else t.dtype == dtype, "%s is of %s", name, t.dtype)
     _require((rows is None or t.shape[0] == rows) and (width is None or t.shape[1] == width), "%s is %d x %d where %s x %s are needed", name,
              *t.shape, "any" if rows is None else rows, "any" if width is None else width)
@@ -239,9 +239,9 @@ def layer_norm_backward(grad, x, scale, mean, rstd, out=None, mirror_rows=None):
 def distillation_loss(logits, teacher, classes, temperature=1.0, truth=None, labelled=None, soft=1.0, hard=0.0):
     """(loss, gradient) of logits [n, classes] against a teacher's top logits: values `teacher` [n, top] of the classes `classes`
     [n, top] (int64; negative: no entry).  loss[0]: mean over the rows with an entry of temperature^2 * KL(teacher || model) over the
-    entries; loss[1]: mean cross-entropy over the labelled rows (truth int64, labelled bool;
-    where a row is not labelled its truth may be anything, such as -1).  The gradient is soft times that of the
-    first sum over rows plus hard times that of the second, not divided by the numbers of rows, as the graph model's own loss has it."""
+    entries; loss[1]: mean cross-entropy over the labelled rows (truth int64, labelled bool; where a row is
+    not labelled its truth may be anything, such as -1).  The gradient is soft times that of the first sum over rows plus hard times that of the
+    second, not divided by the numbers of rows, as the graph model's own loss has it."""
     ld = _matrix("logits", logits)
     n, c, device = logits.shape[0], logits.shape[1], logits.device
     ldt = _matrix("teacher", teacher, n, device=device)

@@ -108,3 +108,14 @@ def test_constants_are_the_headers():
     defined = {name: int(value) for name, value in re.findall(r"#define DRONE_(\w+)\s+(-?\d+)\b", text)}
     for name in ("F32", "BF16", "F16", "ACT_NONE", "ACT_RELU", "ACT_GELU", "ACT_SILU", "NORM_MAX_WIDTH", "DISTILLATION_MAX_TOP", "DISTILLATION_SCRATCH"):
         assert getattr(_lib, name) == defined[name], name
+
+
+def test_widths_beyond_an_int_are_refused():
+    """A single row may be as long as memory is; the C ABI takes its length as an int, which 2^32 + 7 would reach as 7."""
+    for f in ((1 << 31) - 1, 1 << 31, (1 << 32) + 7):
+        row = torch.empty((1, f), dtype=torch.bfloat16, device="meta")
+        if f < 1 << 31:
+            assert dense._matrix("x", row, device=row.device) == f
+        else:
+            with pytest.raises(ValueError, match="x has 1 rows of %d" % f):
+                dense._matrix("x", row, device=row.device)
