@@ -6,8 +6,9 @@ import math
 import pytest
 import torch
 
-from drone_b200 import _lib, dense
+from drone_b200 import _lib, dense, gcn
 from test_dense_gpu import STEP, TYPES, activated, check_rounded, distilled, rows_of, slope
+from test_residual_gcn_gpu import graph_of, parameters
 
 pytestmark = pytest.mark.gpu
 
@@ -194,3 +195,32 @@ def test_split_products_of_infinities(cuda_device, transposed):
         fine = want.isfinite()
         size = rows.double().abs().nan_to_num(0, 0, 0) @ weights.double().abs().nan_to_num(0, 0, 0)
         check_rounded(got[fine], want[fine], ((rows.shape[1] + 16) * STEP * size)[fine], torch.float32)
+
+
+def test_captured_step_on_other_inputs(cuda_device, oracle):
+    """Captured on one input and replayed on two others, beside a second graph of the same model: the bits of the eager steps on these."""
+    n, _, (graph,) = graph_of(cuda_device, oracle)
+    gen = torch.Generator(cuda_device).manual_seed(7)
+    dims = (40, 32, 7)
+    inputs = [torch.randn((n, dims[0]), device=cuda_device, generator=gen) for _ in range(3)]
+    truth = torch.randint(-1, dims[2], (n,), device=cuda_device, generator=gen, dtype=torch.int32)
+    model = gcn.ResidualGCN(graph, inputs[0].clone(), truth, *parameters(cuda_device, gen, dims, 2))
+
+    def eager(rows):
+        model.x.copy_(rows)
+        return [model.forward().clone(), *(g.clone() for g in model.backward())]
+    wanted = [eager(rows) for rows in inputs]
+    assert all(not torch.equal(a, b) for i in range(3) for a, b in zip(wanted[i], wanted[i - 1]))
+    model.x.copy_(inputs[2])
+    captured = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outputs = [model.forward(), *model.backward()]
+        captured.append((g, outputs))
+    for rows, want in zip(inputs, wanted):
+        model.x.copy_(rows)
+        for g, outputs in captured:
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outputs, want))
