@@ -88,20 +88,21 @@ __device__ __forceinline__ float normal_part(float z, float tail) {
     return fabsf(above - tail);
 }
 
-// z -> activation(z) and its derivative, for values of type T.  A NaN stays one, also in the ReLU (max(NaN, 0) would be 0).
+// z -> activation(z) + added, and the activation's derivative, for values of type T.  A NaN stays one, also in the ReLU (max(NaN, 0) would be 0).  The
+// last product and the addition are one instruction, in words: left to the compiler, they would be one on some ways out of a product and two on others.
 template <typename T, int ACTIVATION>
-__device__ __forceinline__ float activate(float z) {
+__device__ __forceinline__ float activate(float z, float added) {
     if constexpr (ACTIVATION == DRONE_ACT_RELU) {
-        return z < 0.f ? 0.f : z;
+        return (z < 0.f ? 0.f : z) + added;
     } else if constexpr (ACTIVATION == DRONE_ACT_GELU) {
-        if (sizeof(T) == 4) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+        if (sizeof(T) == 4) return fmaf(0.5f * z, 1.f + erff(z * 0.70710678f), added);
         float bell;
         const float tail = normal_tail(z, &bell);
-        return z * normal_part(z, tail);
+        return fmaf(z, normal_part(z, tail), added);
     } else if constexpr (ACTIVATION == DRONE_ACT_SILU) {
-        return sizeof(T) == 4 ? z / (1.f + expf(-z)) : z * reciprocal_fast(1.f + exp2_fast(z * -1.44269504f));
+        return sizeof(T) == 4 ? __fadd_rn(z / (1.f + expf(-z)), added) : fmaf(z, reciprocal_fast(1.f + exp2_fast(z * -1.44269504f)), added);
     } else {
-        return z;
+        return z + added;
     }
 }
 template <typename T, int ACTIVATION>

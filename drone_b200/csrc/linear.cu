@@ -43,9 +43,7 @@ template <typename T, int ACTIVATION>
 __device__ __forceinline__ void put_value(const LinearOut<T> &out, long long row, int c, float z) {
     if (out.bias) z += __ldg(out.bias + c);
     if (out.pre) out.pre[row * out.ldp + c] = from_float<T>(z);
-    float v = activate<T, ACTIVATION>(z);
-    if (out.residual) v += to_float(out.residual[row * out.ldr + c]);
-    out.y[row * out.ldy + c] = from_float<T>(v);
+    out.y[row * out.ldy + c] = from_float<T>(activate<T, ACTIVATION>(z, out.residual ? to_float(out.residual[row * out.ldr + c]) : 0.f));
 }
 template <typename T, bool TRANSPOSED>
 __global__ void __launch_bounds__(TRANSPOSED ? 256 : 1024) few_rows_kernel(Operand<T> X, Operand<T> W, int n, int N, int K, LinearOut<T> out) {

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from drone_b200 import _lib, dense, gcn
-from test_dense_gpu import STEP, TYPES, activated, check_rounded, distilled, rows_of, slope
+from test_dense_gpu import STEP, TYPES, activated, check_linear, check_rounded, distilled, rows_of, slope
 from test_residual_gcn_gpu import graph_of, parameters
 
 pytestmark = pytest.mark.gpu
@@ -145,6 +145,18 @@ def test_weight_gradients_over_very_many_rows(cuda_device, dtype, transposed):
         want = x[:, i:i + 100].double().t() @ g[:, j:j + 100].double()
         got = dw[j:j + 100, i:i + 100].t() if transposed else dw[i:i + 100, j:j + 100]
         check_rounded(got, want, (512 + 49 + 16) * STEP * want, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [4, 9, 15, 16, 17, 31, 33, 47, 48, 49, 63, 65, 97, 129, 145, 257, 300])
+def test_tiles_of_few_columns(cuda_device, m, dtype):
+    """The warps that take a tile out share its columns, however few they are, also where the last tile of a row of tiles has fewer than the others; rows that lie any distance
+    apart are taken out a value a lane, the others 4 or 8."""
+    gen = torch.Generator(cuda_device).manual_seed(m)
+    for pad, lead in ((0, 0), (1, 0), (3, 1), (8, 0)):
+        check_linear(gen, 2100, 40, m, dtype, bias=True, residual=True, activation="gelu", keep=True, pad=pad, lead=lead)
+        check_linear(gen, 20011, 33, m, dtype, activation="silu", transposed=True, pad=pad, lead=lead)
+        check_linear(gen, 2100, 600, m, dtype, residual=True, pad=pad, lead=lead)
 
 
 def in_tiles(x, w, transposed=False):
