@@ -115,15 +115,17 @@ struct SharedLayout {
     }
 };
 
-// V values side by side that can be read at once.
-template <int V>
+// V values side by side, that can be read at once or (PAIR = false) one by one.
+template <int V, bool PAIR>
 __device__ __forceinline__ void load_whole(const float *p, float *v) {
     if constexpr (V == 4) {
         const float4 a = __ldg((const float4 *)p);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    } else {
+    } else if constexpr (PAIR) {
         const float2 a = __ldg((const float2 *)p);
         v[0] = a.x, v[1] = a.y;
+    } else {
+        v[0] = __ldg(p), v[1] = __ldg(p + 1);
     }
 }
 // V values side by side, of which `live` exist (the others are 0); `bytes` can be read at once.
@@ -213,14 +215,14 @@ struct Share {
         limit = size, k = k1 - k0;
     }
     // WHOLE: the step lies inside the operand; its loads follow one another without a condition, so that all of them are in flight
-    template <int V, bool WHOLE>
+    template <int V, bool WHOLE, bool PAIR = true>
     __device__ __forceinline__ void load_each(Values &to) {
         const float *p = at;
 #pragma unroll
         for (int u = 0; u < VALUES / V; ++u, p += APART<V> * from.ld) {
             float *const v = to.v + u * V;
             if constexpr (WHOLE) {
-                load_whole<V>(p, v);
+                load_whole<V, PAIR>(p, v);
             } else {
                 const int r = row + u * APART<V>;
                 const bool in_row = ALONG_K ? r < limit : r < k;
@@ -235,6 +237,7 @@ struct Share {
             else load_each<4, false>(to);
         } else {
             if (whole && from.bytes >= 8) load_each<2, true>(to);
+            else if (whole) load_each<2, true, false>(to);
             else load_each<2, false>(to);
         }
         k -= S::KS;
@@ -828,7 +831,9 @@ int launch_product_tiles(const Operand<T> &A, const Operand<T> &B, int M, int N,
         DRONE_LAUNCH_CHECK("image_kernel");
     }
     // Rows that do not start on 16 bytes share lines between neighbouring steps: what two stages leave of an SM's memory is L1 that keeps them.
-    // 232,965 x 602 x 128 floats 278 us with three, 243 with two; 232,965 x 128 x 602, on 16 bytes, 260 and 296.
+    // us with two and three, floats with bias and ReLU, calls one after another: 249,169 x 602 x 16 / 128 / 256 204 and 263 / 292 and 320 / 540 and 572; 600,000 x 154 x 16 /
+    // 128 144 and 180 / 217 and 240; 600,000 x 115 x 64 151 and 174; 149,850 x 1001 x 64 235 and 274; 600,000 x 47 x 128 147 and 150, but of two steps, 600,000 x
+    // 33 x 64, 105 and 98.  On 16 bytes 232,965 x 128 x 602 296 and 260.
     p.stages = BRING == kImage && A.bytes < 16 ? 2 : S::STAGES;
     const int bytes = S::shared(p.stages, kOutWarps<BRING>);
     auto *const kernel = product_tile_kernel<T, BRING, A_ALONG_K, B_ALONG_K>;
