@@ -1,6 +1,7 @@
 // Products of a dense layer, Y = activation(X W + bias) + residual, and its backward pass.
 #include "product_tile.cuh"
 #include "row_shape.cuh"
+#include "thin_products.cuh"
 
 #include <algorithm>
 
@@ -28,6 +29,15 @@ __global__ void __launch_bounds__(256) add_product_shares_kernel(const float *__
     }
 }
 
+template <typename T>
+static int add_product_shares(const float *parts, int shares, int M, int N, T *out, long long ld, cudaStream_t st) {
+    const long long values = (long long)M * N;
+    if (shares <= 32) add_product_shares_kernel<T, 1><<<ceil_div(values, 256), 256, 0, st>>>(parts, shares, M, N, out, ld);
+    else add_product_shares_kernel<T, 8><<<ceil_div(values, 32), 256, 0, st>>>(parts, shares, M, N, out, ld);
+    DRONE_LAUNCH_CHECK("add_product_shares_kernel");
+    return DRONE_OK;
+}
+
 // A few rows: W is read once for up to ROWS of them, by as many warps as there are loads to hide.
 //   W [K, N]: a block has 32 columns, a lane one of them, its 32 warps every 32nd k; the warps' sums are added in order.
 //   W [N, K]: a warp has a column, its lanes every 32nd k.
@@ -38,12 +48,6 @@ constexpr int kFewRows = 8;
 static bool few_rows(int type, int n, int N, int K) {
     const long long outputs = (long long)n * N;
     return n == 1 || (type == DRONE_F32 ? n <= 512 && outputs <= 1 << 16 : outputs <= 1 << 13 && outputs * K <= 1 << 22);
-}
-template <typename T, int ACTIVATION>
-__device__ __forceinline__ void put_value(const LinearOut<T> &out, long long row, int c, float z) {
-    if (out.bias) z += __ldg(out.bias + c);
-    if (out.pre) out.pre[row * out.ldp + c] = from_float<T>(z);
-    out.y[row * out.ldy + c] = from_float<T>(activate<T, ACTIVATION>(z, out.residual ? to_float(out.residual[row * out.ldr + c]) : 0.f));
 }
 template <typename T, bool TRANSPOSED>
 __global__ void __launch_bounds__(TRANSPOSED ? 256 : 1024) few_rows_kernel(Operand<T> X, Operand<T> W, int n, int N, int K, LinearOut<T> out) {
@@ -308,7 +312,7 @@ int drone_linear_scratch(int type, int n_rows, int K, int N, const void *d_X, in
     DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && (transposed == 0 || transposed == 1) && n_floats,
                   "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d transposed=%d", type, n_rows, K, N, transposed);
     using S = TileShape<float>;
-    if (few_rows(type, n_rows, N, K) || narrow_rows(K, N)) *n_floats = 0;
+    if (few_rows(type, n_rows, N, K) || narrow_rows(K, N) || few_columns(K, N) || short_rows(type, K)) *n_floats = 0;
     else if (type == DRONE_F32) *n_floats = (long long)ceil_div(N, S::BN) * ceil_div(K, S::KS) * (S::B_BYTES / 4);      // the image of the weights
     else *n_floats = padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_W, ldw, transposed ? N : K, transposed ? K : N);
     return DRONE_OK;
@@ -356,6 +360,8 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
             DRONE_LAUNCH_CHECK("narrow_rows_kernel");
             return DRONE_OK;
         }
+        if (few_columns(K, N)) return launch_few_columns<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
+        if (short_rows(type, K)) return launch_short_rows<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
         if constexpr (sizeof(T) == 2) {
             Operand<T> a, b;
             float *scratch = d_scratch;
@@ -432,10 +438,10 @@ int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, con
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    const bool narrow = narrow_rows(K, N);
-    const int shares = narrow ? narrow_blocks(n_rows, narrow_rows_at_once(std::max(K, N), 2), sms) : product_shares(type, transposed ? N : K, transposed ? K : N, n_rows, sms).count;
+    const bool narrow = narrow_rows(K, N), thin = !narrow && thin_gradient(type, K, N);
+    const int shares = thin ? thin_gradient_grid(n_rows, K, N, sms).rows : narrow ? narrow_blocks(n_rows, narrow_rows_at_once(std::max(K, N), 2), sms) : product_shares(type, transposed ? N : K, transposed ? K : N, n_rows, sms).count;
     *n_floats = n_rows == 0 ? 0 : (long long)shares * K * N;
-    if (type != DRONE_F32 && !narrow) *n_floats = (*n_floats + 3) / 4 * 4 + padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_dZ, ldz, n_rows, N);
+    if (type != DRONE_F32 && !narrow && !thin) *n_floats = (*n_floats + 3) / 4 * 4 + padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_dZ, ldz, n_rows, N);
     return DRONE_OK;
 }
 
@@ -470,9 +476,11 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
             const int rows_at_once = narrow_rows_at_once(std::max(K, N), 2), blocks = narrow_blocks(n_rows, rows_at_once, sms);
             narrow_gradient_kernel<T><<<blocks, 256, 0, st>>>(x, dz, n_rows, N, K, transposed != 0, rows_at_once, d_scratch);
             DRONE_LAUNCH_CHECK("narrow_gradient_kernel");
-            add_product_shares_kernel<T, 8><<<ceil_div((long long)rows * columns, 32), 256, 0, st>>>(d_scratch, blocks, rows, columns, (T *)d_dW, ldw);
-            DRONE_LAUNCH_CHECK("add_product_shares_kernel");
-            return DRONE_OK;
+            return add_product_shares<T>(d_scratch, blocks, rows, columns, (T *)d_dW, ldw, st);
+        }
+        if (thin_gradient(type, K, N)) {
+            const int failed = launch_thin_gradient<T>(x, dz, n_rows, N, K, transposed != 0, d_scratch, sms, st);
+            return failed ? failed : add_product_shares<T>(d_scratch, thin_gradient_grid(n_rows, K, N, sms).rows, rows, columns, (T *)d_dW, ldw, st);
         }
         if constexpr (sizeof(T) == 2) {
             float *scratch = d_scratch + ((long long)s.count * K * N + 3) / 4 * 4;
@@ -485,11 +493,7 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
         constexpr Bring BRING = sizeof(T) == 2 ? kCopied : kThrough;
         const int launched = launch_product_tiles<T, BRING, false, false>(a, b, rows, columns, n_rows, s.share, s.count, nullptr, out, sms, st);
         if (launched) return launched;
-        const long long values = (long long)rows * columns;
-        if (s.count <= 32) add_product_shares_kernel<T, 1><<<ceil_div(values, 256), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
-        else add_product_shares_kernel<T, 8><<<ceil_div(values, 32), 256, 0, st>>>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw);
-        DRONE_LAUNCH_CHECK("add_product_shares_kernel");
-        return DRONE_OK;
+        return add_product_shares<T>(d_scratch, s.count, rows, columns, (T *)d_dW, ldw, st);
     });
 }
 

@@ -169,14 +169,38 @@ def in_tiles(x, w, transposed=False):
 
 @pytest.mark.parametrize("transposed", [False, True])
 def test_split_products_one_by_one(cuda_device, transposed):
-    """One product an output, of full mantissas and any size: six products of a float's parts leave two steps of it, or six of the smallest floats."""
+    """One product an output, beside others with 0, of full mantissas and any size: six products of a float's parts leave two steps of it, or six of the smallest floats."""
     gen = torch.Generator(cuda_device).manual_seed(2)
     x = rows_of(gen, 700, 1, torch.float32) * torch.exp2(torch.randint(-60, 60, (700, 1), device="cuda", generator=gen).float())
-    w = rows_of(gen, 1, 200, torch.float32) * torch.exp2(torch.randint(-60, 60, (1, 200), device="cuda", generator=gen).float())
+    w = rows_of(gen, 40, 200, torch.float32) * torch.exp2(torch.randint(-60, 60, (1, 200), device="cuda", generator=gen).float())
+    at = torch.randint(0, 40, (700, 1), device="cuda", generator=gen)
+    x = torch.zeros((700, 40), device="cuda").scatter_(1, at, x)
     given = w.t().contiguous() if transposed else w
     assert in_tiles(x, given, transposed)
-    want, got = x.double() * w.double(), dense.linear(x, given, transposed=transposed)
+    want, got = x.double() @ w.double(), dense.linear(x, given, transposed=transposed)
     assert ((got - want).abs() <= 2 * STEP * want.abs() + 6 * 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", [(513, 129, 1), (600, 4096, 2), (700, 8192, 1), (700, 8193, 1), (3001, 2048, 4), (3001, 2049, 3), (20011, 33, 4), (20011, 200, 3), (5003, 602, 2), (70001, 65, 2),
+                                   (513, 1, 129), (600, 2, 65), (2100, 3, 43), (2100, 4, 128), (2100, 4, 1000), (3001, 1, 447), (3001, 3, 32768), (70001, 2, 131), (20011, 4, 33)])
+def test_thin_products_and_their_gradients(cuda_device, n, k, m, dtype):
+    """Weights of a few rows or columns: forward with everything that an epilogue may have, both orders of the weights, and all three gradients; some rows far apart, not on 16 bytes."""
+    gen = torch.Generator(cuda_device).manual_seed(n + k + m)
+    for pad, lead in ((0, 0), (3, 1)):
+        check_linear(gen, n, k, m, dtype, bias=True, residual=True, activation="gelu", keep=True, pad=pad, lead=lead)
+        check_linear(gen, n, k, m, dtype, transposed=True, activation="silu", pad=pad, lead=lead)
+        x, g = rows_of(gen, n, k, dtype, pad, lead), rows_of(gen, n, m, dtype, pad, lead)
+        for transposed in (False, True):
+            w = rows_of(gen, m, k, dtype) if transposed else rows_of(gen, k, m, dtype)
+            dx, dw, db = dense.linear_backward(g, x, w, transposed=transposed)
+            wd = w.double().t() if transposed else w.double()
+            want, bound = x.double().t() @ g.double(), (n + 16) * STEP * (x.double().abs().t() @ g.double().abs())
+            check_rounded(dw, want.t() if transposed else want, bound.t() if transposed else bound, dtype)
+            check_rounded(dx, g.double() @ wd.t(), (m + 16) * STEP * (g.double().abs() @ wd.t().abs()), dtype)
+            check_rounded(db, g.double().sum(dim=0), (n + 16) * STEP * g.double().abs().sum(dim=0), torch.float32)
+            again = dense.linear_backward(g, x, w, transposed=transposed)
+            assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))
 
 
 @pytest.mark.parametrize("transposed", [False, True])
