@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(TRANSPOSED ? 256 : 1024) few_rows_kernel(Opera
 }
 
 // Many rows, few products each: a block keeps W and some rows of X in shared memory as floats, a thread an output at a time, so that X and Y go
-// over neighbouring lanes whatever their widths and distances.  Bound: two reads of shared memory a product.  us here / with tiles: 1.38 M x 5 x 1
-// floats 28 / 149, bfloat16 28 / 228; 410,000 x 3 x 20 35 / 60 and 37 / 57; 3,000 x 16 x 7 18 / 25 and 18 / 24; but 192,000 x 154 x 2 floats 101 / 62,
-// 400,000 x 16 x 64 158 / 72.
+// over neighbouring lanes whatever their widths and distances.  Bound: two reads of shared memory a product; where one side is of a few values and the other long
+// thin_products.cuh is faster.  us here / with tiles: 410,000 x 3 x 20 floats 35 / 60, bfloat16 37 / 57; 3,000 x 16 x 7 18 / 25 and 18 / 24; but 400,000 x 16 x
+// 64 158 / 72.
 constexpr int kNarrowProducts = 128, kNarrowValues = 8192;
 static bool narrow_rows(int K, int N) { return (long long)K * N <= kNarrowProducts; }
 template <typename T>
@@ -312,7 +312,7 @@ int drone_linear_scratch(int type, int n_rows, int K, int N, const void *d_X, in
     DRONE_REQUIRE(DRONE_TYPE_OK(type) && DRONE_LINEAR_SIZES(n_rows, K, N) && (transposed == 0 || transposed == 1) && n_floats,
                   "drone_linear_scratch: type=%d n_rows=%d K=%d N=%d transposed=%d", type, n_rows, K, N, transposed);
     using S = TileShape<float>;
-    if (few_rows(type, n_rows, N, K) || narrow_rows(K, N) || few_columns(K, N) || short_rows(type, K)) *n_floats = 0;
+    if (few_rows(type, n_rows, N, K) || narrow_rows(K, N) || few_columns(K, N) || short_rows(type, K, N)) *n_floats = 0;
     else if (type == DRONE_F32) *n_floats = (long long)ceil_div(N, S::BN) * ceil_div(K, S::KS) * (S::B_BYTES / 4);      // the image of the weights
     else *n_floats = padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_W, ldw, transposed ? N : K, transposed ? K : N);
     return DRONE_OK;
@@ -353,6 +353,8 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
             DRONE_LAUNCH_CHECK("few_rows_kernel");
             return DRONE_OK;
         }
+        if (few_columns(K, N)) return launch_few_columns<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
+        if (short_rows(type, K, N)) return launch_short_rows<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
         if (narrow_rows(K, N)) {
             const int rows_at_once = narrow_rows_at_once(K, 1);
             narrow_rows_kernel<T><<<(int)std::min<long long>(((long long)n_rows + rows_at_once - 1) / rows_at_once, sms * 5), 256, 0, st>>>(x, w, transposed != 0, n_rows, N,
@@ -360,8 +362,6 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
             DRONE_LAUNCH_CHECK("narrow_rows_kernel");
             return DRONE_OK;
         }
-        if (few_columns(K, N)) return launch_few_columns<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
-        if (short_rows(type, K)) return launch_short_rows<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
         if constexpr (sizeof(T) == 2) {
             Operand<T> a, b;
             float *scratch = d_scratch;
@@ -438,7 +438,7 @@ int drone_linear_weight_gradient_scratch(int type, int n_rows, int K, int N, con
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    const bool narrow = narrow_rows(K, N), thin = !narrow && thin_gradient(type, K, N);
+    const bool thin = thin_gradient(type, K, N), narrow = !thin && narrow_rows(K, N);
     const int shares = thin ? thin_gradient_grid(n_rows, K, N, sms).rows : narrow ? narrow_blocks(n_rows, narrow_rows_at_once(std::max(K, N), 2), sms) : product_shares(type, transposed ? N : K, transposed ? K : N, n_rows, sms).count;
     *n_floats = n_rows == 0 ? 0 : (long long)shares * K * N;
     if (type != DRONE_F32 && !narrow && !thin) *n_floats = (*n_floats + 3) / 4 * 4 + padded_floats(d_X, ldx, n_rows, K) + padded_floats(d_dZ, ldz, n_rows, N);
@@ -472,15 +472,15 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
         Operand<T> x = operand<T>(d_X, ldx), dz = operand<T>(d_dZ, ldz);
+        if (thin_gradient(type, K, N)) {
+            const int failed = launch_thin_gradient<T>(x, dz, n_rows, N, K, transposed != 0, d_scratch, sms, st);
+            return failed ? failed : add_product_shares<T>(d_scratch, thin_gradient_grid(n_rows, K, N, sms).rows, rows, columns, (T *)d_dW, ldw, st);
+        }
         if (narrow_rows(K, N)) {
             const int rows_at_once = narrow_rows_at_once(std::max(K, N), 2), blocks = narrow_blocks(n_rows, rows_at_once, sms);
             narrow_gradient_kernel<T><<<blocks, 256, 0, st>>>(x, dz, n_rows, N, K, transposed != 0, rows_at_once, d_scratch);
             DRONE_LAUNCH_CHECK("narrow_gradient_kernel");
             return add_product_shares<T>(d_scratch, blocks, rows, columns, (T *)d_dW, ldw, st);
-        }
-        if (thin_gradient(type, K, N)) {
-            const int failed = launch_thin_gradient<T>(x, dz, n_rows, N, K, transposed != 0, d_scratch, sms, st);
-            return failed ? failed : add_product_shares<T>(d_scratch, thin_gradient_grid(n_rows, K, N, sms).rows, rows, columns, (T *)d_dW, ldw, st);
         }
         if constexpr (sizeof(T) == 2) {
             float *scratch = d_scratch + ((long long)s.count * K * N + 3) / 4 * 4;

@@ -175,15 +175,19 @@ void with_thin(int values, const F &f) {
     else f(std::integral_constant<int, 4>());
 }
 
-// Where that is faster than tiles: us here / with tiles.
+// Where that is faster than tiles, and than the narrow kernels, which read shared memory twice a product: us here / there.
 // Few columns, bias and ReLU: floats 461,538 x 130 x 1 49 / 118, 234,375 x 256 x 2 45 / 76, 100,000 x 600 x 3 53 / 100, 14,648 x 4096 x 2 55 / 90, but 7,324 x 8192 x 1 185 / 164 (too few
 // warps); 600,000 x 100 x 4 137 / 123, 234,375 x 256 x 5 125 / 78; bfloat16 39 / 185, 37 / 64, 47 / 109, 52 / 45, 145 / 57; 137 / 168, 122 / 80.
-inline bool few_columns(int K, int N) { return N <= 2 ? 2 * K <= kThinWeights : N <= 4 && K >= 128 && 4 * K <= kThinWeights; }
-// Short rows, without an epilogue, and with bias, GELU and residual: floats 763,358 x 1 x 131 224 / 376, 319 / 869; 390,625 x 3 x 256 130 / 162, 222 / 331; 2.3 M x 4 x 43
+// Narrow, floats without an epilogue: 465,116 x 128 x 1 64 / 182, 1.8 M x 32 x 1 71 / 173, 3.5 M x 16 x 1 130 / 177, 1.8 M x 32 x 2 132 / 180, but 6.7 M x 8 x 1 238 / 188, 3.3 M x
+// 16 x 2 243 / 179; bfloat16 within 10 of these.
+inline bool few_columns(int K, int N) { return N <= 2 ? K >= 16 * N && 2 * K <= kThinWeights : N <= 4 && K >= 128 && 4 * K <= kThinWeights; }
+// Short rows, floats without an epilogue, and with bias, GELU and residual: 763,358 x 1 x 131 224 / 376, 319 / 869; 390,625 x 3 x 256 130 / 162, 222 / 331; 2.3 M x 4 x 43
 // 290 / 329, 480 / 645; but 1.6 M x 5 x 64 280 / 214, 432 / 367; 16 bits, a column a thread, 458,015 x 1 x 131 with residual 404 / 256.
-inline bool short_rows(int type, int K) { return type == DRONE_F32 && K <= 4; }
+// Narrow: 465,116 x 1 x 128 60 / 161, 109 / 293; 1.8 M x 1 x 32 144 / 164, 222 / 268; 1.7 M x 3 x 32 178 / 180, 285 / 273; but 3.5 M x 1 x 16 270 / 172.
+inline bool short_rows(int type, int K, int N) { return type == DRONE_F32 && K <= 4 && N >= 32; }
 // Gradients: floats 125,523 x 1 x 477 59 / 154, 230,769 x 4 x 256 75 / 107, 99,833 x 600 x 1 56 / 129, 99,337 x 600 x 4 74 / 114; bfloat16 142 / 86, 154 / 37, 96 / 45, 152 / 45.
-inline bool thin_gradient(int type, int K, int N) { return type == DRONE_F32 && (K <= 4 || N <= 4); }
+// Narrow: floats 465,116 x 1 x 128 66 / 311, 3.5 M x 1 x 16 215 / 306, 3.2 M x 3 x 16 332 / 324, but 6.7 M x 1 x 8 390 / 313.
+inline bool thin_gradient(int type, int K, int N) { return type == DRONE_F32 && (K <= 4 || N <= 4) && (K >= 16 || N >= 16); }
 
 template <typename T>
 int launch_few_columns(const Operand<T> &x, const Operand<T> &w, bool transposed, int n, int N, int K, const LinearOut<T> &out, int sms, cudaStream_t st) {
