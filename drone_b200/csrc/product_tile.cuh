@@ -439,40 +439,47 @@ __device__ __forceinline__ void put_vectors(const LinearOut<T> &out, const float
         *reinterpret_cast<Values<T, W> *>(out.y + row * out.ldy + col0 + c) = y;
     }
 }
-// The same a value a lane: a row at a time with a lane for each column, or, of at most 16 columns, rows one after the other over the lanes.  What eight values of a
-// lane add is on its way at once.  (Four rows at a time, and only the first of the warps with the same rows at work where a tile has few columns: 2.4 M x 8 x 47 floats, GELU, residual
-// 2190 us, now 713; 971,522 x 19 x 35 half 757, now 261; 200,000 x 128 x 301 bfloat16 179, now 143.)
+// The same a value a lane: a row at a time with a lane for each column, or, of at most 16 columns, rows one after the other over the lanes.  What four values of a
+// lane add is on its way at once (where there is a residual).  (Four rows at a time, and only the first of the warps with the same rows at work where a tile has few columns: 2.4 M x 8 x 47 floats, GELU, residual
+// 2190 us, now 740; 971,522 x 19 x 35 half 757, now 236; 200,000 x 128 x 301 bfloat16 179, now 111; but 232,965 x 128 x 602 floats 257, now 262 to 270: more code.)
 template <typename T, int PITCH, int ACTIVATION, bool SHORT>
 __device__ __forceinline__ void put_values(const LinearOut<T> &out, const float *piece, long long row0, int rows, int col0, int width) {
-    constexpr int AT_ONCE = sizeof(T) == 4 ? 8 : 4;
     const int lane = threadIdx.x & 31;
     int r = SHORT ? lane / width : 0, c = SHORT ? lane % width : lane;
     if (c >= width) return;
     const int down = SHORT ? 32 / width : 1, along = SHORT ? 32 % width : 0;
     float b = !SHORT && out.bias ? __ldg(out.bias + col0 + c) : 0.f;
+    auto put = [&](int r, int c, float added) {
+        const long long row = row0 + r;
+        const float z = piece[r * PITCH + c] + (SHORT && out.bias ? __ldg(out.bias + col0 + c) : b);
+        const float w = activate<T, ACTIVATION>(z, added);
+        if (out.pre) out.pre[row * out.ldp + col0 + c] = from_float<T>(z);
+        out.y[row * out.ldy + col0 + c] = from_float<T>(w);
+    };
+    auto next = [&](int &r, int &c) {
+        r += down, c += along;
+        if (SHORT && c >= width) c -= width, ++r;
+    };
+    if (!out.residual) {
+#pragma unroll 4
+        for (; r < rows; next(r, c)) put(r, c, -0.f);      // no addition
+        return;
+    }
+    constexpr int AT_ONCE = 4;
 #pragma unroll 1
     while (r < rows) {
         float added[AT_ONCE];
-        if (out.residual) {
-            int ahead = r, column = c;
+        int ahead = r, column = c;
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) {
-                if (ahead < rows) added[u] = to_float(out.residual[(row0 + ahead) * out.ldr + col0 + column]);
-                ahead += down, column += along;
-                if (SHORT && column >= width) column -= width, ++ahead;
-            }
+        for (int u = 0; u < AT_ONCE; ++u) {
+            if (ahead < rows) added[u] = to_float(out.residual[(row0 + ahead) * out.ldr + col0 + column]);
+            next(ahead, column);
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
             if (r >= rows) break;
-            const long long row = row0 + r;
-            if (SHORT && out.bias) b = __ldg(out.bias + col0 + c);
-            const float z = piece[r * PITCH + c] + b;
-            const float w = activate<T, ACTIVATION>(z, out.residual ? added[u] : 0.f);
-            if (out.pre) out.pre[row * out.ldp + col0 + c] = from_float<T>(z);
-            out.y[row * out.ldy + col0 + c] = from_float<T>(w);
-            r += down, c += along;
-            if (SHORT && c >= width) c -= width, ++r;
+            put(r, c, added[u]);
+            next(r, c);
         }
     }
 }
