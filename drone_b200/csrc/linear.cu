@@ -44,9 +44,11 @@ static int add_product_shares(const float *parts, int shares, int M, int N, T *o
 constexpr int kFewRows = 8;
 // Where that is faster than a few tiles, whose steps of K follow one another however few rows there are.  us here / with tiles: floats 602 x 128
 // 256 rows 7.9 / 21.8, 512 rows 14 / 21.8, 1024 rows 26 / 21.8; 256 x 256 256 rows 7.9 / 12.9, 512 rows 14 / 12.9; 2048 x 2048 32 rows 36 / 58, 64
-// rows 68 / 58; bfloat16 256 x 256 32 rows 5.1 / 6.8, 256 rows 9.2 / 7.2; 2048 x 2048 1 row 6.6 / 13.9, 4 rows 24 / 13.9.
+// rows 68 / 58; with a call's image of the weights, 1400 rows 600 x 32 16 / 29, 2048 rows 600 x 8 16 / 23, 4096 rows 164 x 21 15 / 19, 4096 rows 300 x 25 19 / 20, 8192
+// rows 100 x 12 15 / 19, 8192 rows 164 x 21 25 / 20, 4096 rows 600 x 32 29 / 23; bfloat16 256 x 256 32 rows 5.1 / 6.8, 256 rows 9.2 / 7.2; 2048 x 2048 1 row 6.6 / 13.9, 4 rows 24 / 13.9.
 static bool few_rows(int type, int n, int N, int K) {
     const long long outputs = (long long)n * N;
+    if (type == DRONE_F32 && N <= 32 && n <= 8192 && (long long)ceil_div(n, kFewRows) * K <= 1 << 17) return true;
     return n == 1 || (type == DRONE_F32 ? n <= 512 && outputs <= 1 << 16 : outputs <= 1 << 13 && outputs * K <= 1 << 22);
 }
 template <typename T, bool TRANSPOSED>

@@ -154,8 +154,8 @@ def test_tiles_of_few_columns(cuda_device, m, dtype):
     apart are taken out a value a lane, the others 4 or 8."""
     gen = torch.Generator(cuda_device).manual_seed(m)
     for pad, lead in ((0, 0), (1, 0), (3, 1), (8, 0)):
-        check_linear(gen, 2100, 40, m, dtype, bias=True, residual=True, activation="gelu", keep=True, pad=pad, lead=lead)
-        check_linear(gen, 20011, 33, m, dtype, activation="silu", transposed=True, pad=pad, lead=lead)
+        check_linear(gen, 40011, 40, m, dtype, bias=True, residual=True, activation="gelu", keep=True, pad=pad, lead=lead)
+        check_linear(gen, 40011, 33, m, dtype, activation="silu", transposed=True, pad=pad, lead=lead)
         check_linear(gen, 2100, 600, m, dtype, residual=True, pad=pad, lead=lead)
 
 
@@ -179,6 +179,16 @@ def test_split_products_one_by_one(cuda_device, transposed):
     assert in_tiles(x, given, transposed)
     want, got = x.double() @ w.double(), dense.linear(x, given, transposed=transposed)
     assert ((got - want).abs() <= 2 * STEP * want.abs() + 6 * 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("n,k,m", [(513, 255, 33), (1400, 600, 32), (1744, 601, 9), (1745, 601, 9), (8192, 100, 33), (8192, 128, 32), (8192, 129, 32), (8192, 3, 31), (8193, 17, 30), (20011, 9, 17)])
+def test_more_rows_of_few_columns(cuda_device, n, k, m, transposed):
+    """Floats of at most 32 columns, on both sides of the number of rows up to which they go eight at a time."""
+    gen = torch.Generator(cuda_device).manual_seed(n)
+    for pad, lead in ((0, 0), (3, 1)):
+        check_linear(gen, n, k, m, torch.float32, bias=True, residual=True, activation="gelu", keep=True, transposed=transposed, pad=pad, lead=lead)
+        check_linear(gen, n, k, m, torch.float32, transposed=transposed, pad=pad, lead=lead)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
