@@ -439,9 +439,10 @@ __device__ __forceinline__ void put_vectors(const LinearOut<T> &out, const float
         *reinterpret_cast<Values<T, W> *>(out.y + row * out.ldy + col0 + c) = y;
     }
 }
-// The same a value a lane: a row at a time with a lane for each column, or, of at most 16 columns, rows one after the other over the lanes.  What four values of a
-// lane add is on its way at once (where there is a residual).  (Four rows at a time, and only the first of the warps with the same rows at work where a tile has few columns: 2.4 M x 8 x 47 floats, GELU, residual
-// 2190 us, now 740; 971,522 x 19 x 35 half 757, now 236; 200,000 x 128 x 301 bfloat16 179, now 111; but 232,965 x 128 x 602 floats 257, now 262 to 270: more code.)
+// The same a value a lane: a row at a time with a lane for each column, or, of at most 16 columns of 16 bits, rows one after the other over the lanes (606,060 x 19 x 47
+// half, GELU, residual 203 us, 253 without; floats gain as much, 333,333 x 108 x 12 100 and 134, but where the kernel holds that code too wide products are slower, 232,965 x 128 x
+// 602 270 and 257).  What four values of a lane add is on its way at once.
+// Before, and before the warps with the same rows shared a narrow tile: 606,060 x 19 x 47 half 588, floats 575 and now 213; 200,000 x 128 x 301 bfloat16 179 and now 111.
 template <typename T, int PITCH, int ACTIVATION, bool SHORT>
 __device__ __forceinline__ void put_values(const LinearOut<T> &out, const float *piece, long long row0, int rows, int col0, int width) {
     const int lane = threadIdx.x & 31;
@@ -490,8 +491,12 @@ __device__ __forceinline__ void put_piece(const LinearOut<T> &out, const float *
     } else if (out.at_once == 4) {
         put_vectors<T, PITCH, ACTIVATION, 4>(out, piece, residual, row0, rows, col0, width);
     } else {
-        if (width > 16) put_values<T, PITCH, ACTIVATION, false>(out, piece, row0, rows, col0, width);
-        else put_values<T, PITCH, ACTIVATION, true>(out, piece, row0, rows, col0, width);
+        bool is_short = false;
+        if constexpr (sizeof(T) == 2) {
+            is_short = width <= 16;
+            if (is_short) put_values<T, PITCH, ACTIVATION, true>(out, piece, row0, rows, col0, width);
+        }
+        if (!is_short) put_values<T, PITCH, ACTIVATION, false>(out, piece, row0, rows, col0, width);
     }
 }
 
