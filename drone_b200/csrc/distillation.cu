@@ -14,7 +14,7 @@
 namespace drone {
 
 constexpr int kMaxTop = DRONE_DISTILLATION_MAX_TOP;
-constexpr int kRowBlocks = DRONE_DISTILLATION_SCRATCH / 4;
+constexpr int kRowBlocks = DRONE_DISTILLATION_SCRATCH / 4;      // eight for each of 148 SMs; the results are right for any number
 
 // The sums of a block's rows: soft losses, rows that have one, hard losses, rows that have one.
 struct LossSums {
@@ -112,7 +112,7 @@ struct LongSum {
 
 // Rows of (PER - 1) * L + 1 to PER * L classes, L lanes a row: logits and exponentials stay in registers, the teacher's shares are added up in
 // shared memory, where the lane of an entry finds its class.
-// 2.4 M rows of 47 classes, 8 entries, labels: 1.18 GB in 341 us (53 % of the copy rate; instructions, and the round trips of a row's
+// 2.4 M rows of 47 classes, 8 entries, labels: 1.18 GB in 344 us (53 % of the copy rate; instructions, and the round trips of a row's
 // reductions); with 74 registers instead of 64 421; as exponentials by division and expf, computed twice, and every entry shown to every
 // lane 1171 us.
 template <typename T, int L, int PER, bool HARD>
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(256, 4) distillation_rows_kernel(Distillation<
 // Rows of any number of classes, a block a row: one pass for maximum and sums (every thread its own maximum, so that the sums are scaled when
 // it grows), one for the gradient that finds the row in L2.  16 bytes at a time behind the first values up to a multiple of 16, where logits
 // and gradient lie alike; VEC = false: single values.
-// 8,192 rows of 32,000 bfloat16 classes, 64 entries: 1.05 GB in 246 us (66 % of the copy rate; two exponentials a value); in three passes of single values
+// 8,192 rows of 32,000 bfloat16 classes, 64 entries: 1.05 GB in 249 us (65 % of the copy rate; two exponentials a value); in three passes of single values
 // 845 us, with blocks of 512 threads 316.
 template <typename T, int THREADS, bool HARD, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distillation_block_kernel(Distillation<T> p) {

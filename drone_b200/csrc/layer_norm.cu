@@ -7,7 +7,7 @@
 // where rows allow it), so that mean, variance and the two means of the backward pass cost shuffles and no second read; the
 // variance is that of the differences from the mean, in 32 bits.  The sums over rows stay in a thread's registers for all rows it
 // takes, are added within the block in shared memory and over the blocks in double, always in the same order.
-// us: 2.4 M rows of 256 floats with ReLU 863 (90 % of the copy rate); backward 232,965 rows of 128 floats with ReLU 83 (90 %), 98 without reading a
+// us: 2.4 M rows of 256 floats with ReLU 870 (90 % of the copy rate); backward 232,965 rows of 128 floats with ReLU 83 (90 %), 98 without reading a
 // row ahead; 65,537 rows of 1024 bfloat16 110 (57 %): a lane's 32 values and their two sums take 255 registers; four warps a row with a
 // barrier took 150 to 162.
 #include "row_shape.cuh"

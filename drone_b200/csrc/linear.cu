@@ -356,7 +356,9 @@ int drone_linear(int type, int n_rows, int K, int N, const void *d_X, int ldx, c
             return DRONE_OK;
         }
         if (few_columns(K, N)) return launch_few_columns<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
-        if (short_rows(type, K, N)) return launch_short_rows<T>(x, w, transposed != 0, n_rows, N, K, out, sms, st);
+        if constexpr (sizeof(T) == 4) {
+            if (short_rows(type, K, N)) return launch_short_rows(x, w, transposed != 0, n_rows, N, K, out, sms, st);
+        }
         if (narrow_rows(K, N)) {
             const int rows_at_once = narrow_rows_at_once(K, 1);
             narrow_rows_kernel<T><<<(int)std::min<long long>(((long long)n_rows + rows_at_once - 1) / rows_at_once, sms * 5), 256, 0, st>>>(x, w, transposed != 0, n_rows, N,
@@ -474,9 +476,11 @@ int drone_linear_weight_gradient(int type, int n_rows, int K, int N, const void 
     return with_type(type, [&](auto tag) {
         using T = typename decltype(tag)::T;
         Operand<T> x = operand<T>(d_X, ldx), dz = operand<T>(d_dZ, ldz);
-        if (thin_gradient(type, K, N)) {
-            const int failed = launch_thin_gradient<T>(x, dz, n_rows, N, K, transposed != 0, d_scratch, sms, st);
-            return failed ? failed : add_product_shares<T>(d_scratch, thin_gradient_grid(n_rows, K, N, sms).rows, rows, columns, (T *)d_dW, ldw, st);
+        if constexpr (sizeof(T) == 4) {
+            if (thin_gradient(type, K, N)) {
+                const int failed = launch_thin_gradient(x, dz, n_rows, N, K, transposed != 0, d_scratch, sms, st);
+                return failed ? failed : add_product_shares<T>(d_scratch, thin_gradient_grid(n_rows, K, N, sms).rows, rows, columns, (T *)d_dW, ldw, st);
+            }
         }
         if (narrow_rows(K, N)) {
             const int rows_at_once = narrow_rows_at_once(std::max(K, N), 2), blocks = narrow_blocks(n_rows, rows_at_once, sms);

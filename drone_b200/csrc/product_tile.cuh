@@ -19,9 +19,9 @@
 //
 // All waits end after two seconds; a block whose wait did leaves NaN in its outputs.
 //
-// us: 232,965 x 602 x 128 floats with bias and ReLU 273 (floor 128, of six bfloat16 products; 305 as two blocks an SM that bring, multiply and take out
-// in turn; matrix instructions alone about 180: of 128 columns they read operands from shared memory at its rate); the weight gradient of the
-// same 286, 349 with 8 warps that bring; 2.4 M x 256 x 256 bfloat16 with GELU, residual and the values before it 1084 (72 % of the copy
+// us: 232,965 x 602 x 128 floats with bias and ReLU 276 among other inputs, 252 on the same again (floor 128, of six bfloat16 products; 305 as two blocks an SM that bring,
+// multiply and take out in turn; matrix instructions alone about 180: of 128 columns they read operands from shared memory at its rate); the weight gradient of the
+// same 310, 349 with 8 warps that bring; 2.4 M x 256 x 256 bfloat16 with GELU, residual and the values before it 1074 (72 % of the copy
 // rate; 2363 with 8 warps that take out, 1393 without the residual ahead and 8 bytes a lane).
 #pragma once
 

@@ -2,8 +2,8 @@
 // of the long operand meets a few others, so that nothing is to be gained from tiles, of which most would be empty.
 //
 //   few columns   a warp has some rows, its lanes every 32nd k; W lies in shared memory as floats, the lanes' sums are added by shuffles
-//   short rows    a warp has some rows and up to 128 columns, W's values of them in its registers
-//   gradient      the same of the wide operand, whose values are added up over a block's rows for each of the thin one's; shares[block]
+//   short rows    (floats) a warp has some rows and up to 128 columns, W's values of them in its registers
+//   gradient      (floats) the same of the wide operand, whose values are added up over a block's rows for each of the thin one's; shares[block]
 //
 // Bound: HBM, the long operand read or written once: 60 M floats in 45 us where two columns are formed of rows of 256 (83 % of the copy rate), in 59 in the gradient of
 // 125,523 x 1 x 477; 100 M written in 97 us from rows of one value to 256 (64 %).
@@ -77,8 +77,8 @@ __global__ void __launch_bounds__(256, 4) few_columns_kernel(Operand<T> X, Opera
 
 // A warp has some rows, four at once, and 128 columns at most, its lanes every 32nd of them: what they read of X serves four outputs.
 // S: K rounded up to a power of two
-template <typename T, int S>
-__global__ void __launch_bounds__(256) short_rows_kernel(Operand<T> X, Operand<T> W, bool transposed, int n, int N, int K, int width, LinearOut<T> out) {
+template <int S>
+__global__ void __launch_bounds__(256) short_rows_kernel(Operand<float> X, Operand<float> W, bool transposed, int n, int N, int K, int width, LinearOut<float> out) {
     constexpr int AT_ONCE = 4, EACH = 4;
     const int c0 = blockIdx.y * width + (threadIdx.x & 31), limit = min(N, ((int)blockIdx.y + 1) * width);
     float w[EACH][S], b[EACH];
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256) short_rows_kernel(Operand<T> X, Operand<T
     for (int i = 0; i < EACH; ++i) {
         const int c = c0 + i * 32;
 #pragma unroll
-        for (int k = 0; k < S; ++k) w[i][k] = k < K && c < limit ? to_float(W.at[transposed ? c * W.ld + k : k * W.ld + c]) : 0.f;
+        for (int k = 0; k < S; ++k) w[i][k] = k < K && c < limit ? W.at[transposed ? c * W.ld + k : k * W.ld + c] : 0.f;
         b[i] = out.bias && c < limit ? __ldg(out.bias + c) : 0.f;
     }
     const long long step = gridDim.x * 8LL;
@@ -97,9 +97,9 @@ __global__ void __launch_bounds__(256) short_rows_kernel(Operand<T> X, Operand<T
             for (int u = 0; u < AT_ONCE; ++u) {
                 const long long row = min(row0 + u * step, n - 1LL);      // a row that does not exist reads the last one
 #pragma unroll
-                for (int k = 0; k < S; ++k) x[u][k] = k < K ? to_float(X.at[row * X.ld + k]) : 0.f;
+                for (int k = 0; k < S; ++k) x[u][k] = k < K ? X.at[row * X.ld + k] : 0.f;
 #pragma unroll
-                for (int i = 0; i < EACH; ++i) added[u][i] = out.residual && c0 + i * 32 < limit ? to_float(out.residual[row * out.ldr + c0 + i * 32]) : 0.f;
+                for (int i = 0; i < EACH; ++i) added[u][i] = out.residual && c0 + i * 32 < limit ? out.residual[row * out.ldr + c0 + i * 32] : 0.f;
             }
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(256) short_rows_kernel(Operand<T> X, Operand<T
 #pragma unroll
                     for (int k = 0; k < S; ++k) z = fmaf(x[u][k], w[i][k], z);
                     z += b[i];
-                    if (out.pre) out.pre[row * out.ldp + c] = from_float<T>(z);
-                    out.y[row * out.ldy + c] = from_float<T>(activate<T, decltype(act)::value>(z, added[u][i]));
+                    if (out.pre) out.pre[row * out.ldp + c] = z;
+                    out.y[row * out.ldy + c] = activate<float, decltype(act)::value>(z, added[u][i]);
                 }
             }
         }
@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(256) short_rows_kernel(Operand<T> X, Operand<T
 
 // thin [n, S] and wide [n, columns]: shares[block][s * apart_s + c * apart_c] = the sums of thin[r, s] wide[r, c] over the block's rows.  A warp has some rows, four at
 // once, and 128 columns at most.  S: rounded up to a power of two
-template <typename T, int S>
-__global__ void __launch_bounds__(256) thin_gradient_kernel(Operand<T> thin, Operand<T> wide, int n, int count, int columns, int width, int apart_s, int apart_c, float *shares) {
+template <int S>
+__global__ void __launch_bounds__(256) thin_gradient_kernel(Operand<float> thin, Operand<float> wide, int n, int count, int columns, int width, int apart_s, int apart_c, float *shares) {
     constexpr int AT_ONCE = 4, EACH = 4;
     __shared__ float of_warp[8][S][EACH * 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.y * width, limit = min(columns - c0, width);
@@ -141,9 +141,9 @@ __global__ void __launch_bounds__(256) thin_gradient_kernel(Operand<T> thin, Ope
             const long long row = row0 + u * step;
             const bool live = row < n;
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) b[u][i] = live && lane + i * 32 < limit ? to_float(wide.at[row * wide.ld + c0 + lane + i * 32]) : 0.f;
+            for (int i = 0; i < EACH; ++i) b[u][i] = live && lane + i * 32 < limit ? wide.at[row * wide.ld + c0 + lane + i * 32] : 0.f;
 #pragma unroll
-            for (int s = 0; s < S; ++s) a[u][s] = live && s < count ? to_float(thin.at[row * thin.ld + s]) : 0.f;
+            for (int s = 0; s < S; ++s) a[u][s] = live && s < count ? thin.at[row * thin.ld + s] : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u)
@@ -207,23 +207,21 @@ struct ThinGrid {
         rows = (int)std::max<long long>(1, std::min<long long>(((long long)n + 8 * of_warp - 1) / (8 * of_warp), std::max(1, sms * blocks_per_sm / columns)));
     }
 };
-template <typename T>
-int launch_short_rows(const Operand<T> &x, const Operand<T> &w, bool transposed, int n, int N, int K, const LinearOut<T> &out, int sms, cudaStream_t st) {
+inline int launch_short_rows(const Operand<float> &x, const Operand<float> &w, bool transposed, int n, int N, int K, const LinearOut<float> &out, int sms, cudaStream_t st) {
     const ThinGrid g(n, N, 1, 8, sms);
-    with_thin(K, [&](auto values) { short_rows_kernel<T, decltype(values)::value><<<dim3(g.rows, g.columns), 256, 0, st>>>(x, w, transposed, n, N, K, g.width, out); });
+    with_thin(K, [&](auto values) { short_rows_kernel<decltype(values)::value><<<dim3(g.rows, g.columns), 256, 0, st>>>(x, w, transposed, n, N, K, g.width, out); });
     DRONE_LAUNCH_CHECK("short_rows_kernel");
     return DRONE_OK;
 }
 inline ThinGrid thin_gradient_grid(int n, int K, int N, int sms) { return ThinGrid(n, std::max(K, N), 4, 6, sms); }
-template <typename T>
-int launch_thin_gradient(const Operand<T> &x, const Operand<T> &dz, int n, int N, int K, bool transposed, float *shares, int sms, cudaStream_t st) {
+inline int launch_thin_gradient(const Operand<float> &x, const Operand<float> &dz, int n, int N, int K, bool transposed, float *shares, int sms, cudaStream_t st) {
     const bool short_k = K <= N;      // dW[k, c], or with `transposed` [c, k]
-    const Operand<T> &thin = short_k ? x : dz, &wide = short_k ? dz : x;
+    const Operand<float> &thin = short_k ? x : dz, &wide = short_k ? dz : x;
     const int apart_k = transposed ? 1 : N, apart_n = transposed ? K : 1, apart_s = short_k ? apart_k : apart_n, apart_c = short_k ? apart_n : apart_k;
     const ThinGrid g = thin_gradient_grid(n, K, N, sms);
     const dim3 grid(g.rows, g.columns);
     with_thin(std::min(K, N), [&](auto values) {
-        thin_gradient_kernel<T, decltype(values)::value><<<grid, 256, 0, st>>>(thin, wide, n, std::min(K, N), std::max(K, N), g.width, apart_s, apart_c, shares);
+        thin_gradient_kernel<decltype(values)::value><<<grid, 256, 0, st>>>(thin, wide, n, std::min(K, N), std::max(K, N), g.width, apart_s, apart_c, shares);
     });
     DRONE_LAUNCH_CHECK("thin_gradient_kernel");
     return DRONE_OK;
