@@ -425,8 +425,10 @@ int drone_layer_norm_backward(int type, int n_rows, int F, const void *d_G, int 
  *   d_grad    = soft * t (p - q) + hard * (softmax(logits) - one-hot) * labelled, not divided by the numbers of rows
  * as drone_softmax_loss has it.  Entries with a negative class or a value of minus infinity are left out, a class that is there
  * twice has the sum of both; a row without entries has no soft part.  An entry's class of `classes` or more, or a d_truth outside
- * 0..classes-1 in a labelled row, makes that part of the loss and the row's gradient NaN; in other rows d_truth may be anything.  d_scratch: DRONE_DISTILLATION_SCRATCH doubles.  d_grad
- * may be d_logits with the same leading dimension. */
+ * 0..classes-1 in a labelled row, makes that part of the loss and the row's gradient NaN; in other rows d_truth may be
+ * anything.  The gradient of a row without entry and label is 0 whatever its logits are.  d_loss[0] is t^2 times a difference of 32-bit
+ * logarithms, good to about t^2 2^-22.  d_scratch: DRONE_DISTILLATION_SCRATCH doubles.  d_grad may be d_logits with the same leading
+ * dimension. */
 #define DRONE_DISTILLATION_MAX_TOP 256
 #define DRONE_DISTILLATION_SCRATCH 4736
 int drone_distillation_loss(int type, int n_rows, int classes, const void *d_logits, int ld, int teacher_type, int top,
